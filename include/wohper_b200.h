@@ -549,6 +549,98 @@ wh_status wh_lm_head_topk_batch(wh_ctx* ctx, const uint16_t* weight, long long r
                                 wh_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Paged key/value cache in 4 bits                                            */
+/* ------------------------------------------------------------------------ */
+/* No reference counterpart: the reference keeps f32 rows, one contiguous cache
+ * per sequence.  A pool of `blocks` blocks; a block holds `page` rows of every
+ * kv head.  A row of head_dim values is head_dim/2 bytes of E2M1 codes (OCP
+ * values 0 0.5 1 1.5 2 3 4 6, low nibble = even column) and head_dim/32 UE8M0
+ * scale bytes b: 2^(b-127), 0 for b = 0, and a block of 32 with b >= 253 reads
+ * as NaN.  Slot s (0 <= s < blocks * page) is row s % page of block s / page. */
+typedef struct wh_kv_cache {
+  int blocks, page, kv_heads, head_dim; /* head_dim: a multiple of 32, at most 512 */
+  uint8_t* keys;         /* [blocks][kv_heads][page][head_dim/2], 16-byte aligned */
+  uint8_t* key_scales;   /* [blocks][kv_heads][page][head_dim/32], 16-byte aligned */
+  uint8_t* values;       /* as keys; NULL: the values are the keys (one latent row) */
+  uint8_t* value_scales;
+  /* bytes from one block to the next (0: dense), for a pool that interleaves
+   * layers; multiples of 16 and of head_dim/32 */
+  long long block_stride, scale_block_stride;
+} wh_kv_cache;
+
+#define WH_DTYPE_F32 0
+#define WH_DTYPE_BF16 1
+#define WH_DTYPE_F16 2
+
+/* Device scratch bytes of wh_kv_plan. */
+size_t wh_kv_plan_scratch_bytes(int requests);
+/* The bookkeeping of one serving step, on the device.  Request r has kv_lens[r]
+ * cached rows and gets q_lens[r] new tokens; finished (nullable) [requests]
+ * marks requests that end with this step: their blocks go back, their q_lens
+ * must be 0 and their length becomes 0.  block_table [requests][max_blocks]
+ * holds each request's blocks in order; free_blocks [capacity] is a stack of
+ * free block ids whose height is *free_top.  Blocks of finished requests are
+ * pushed in the order of requests and pages, then each new page pops one, in
+ * the same order; block_table and free_blocks are updated in place, the new
+ * height goes to *free_top_out (which may not be free_top).  Outputs:
+ * kv_lens_out [requests] (may be kv_lens), cu_q [requests + 1] (exclusive sums
+ * of q_lens), and per token of [0, tokens): slots (where its row goes),
+ * positions, token_requests; -1 for tokens from cu_q[requests] on.
+ * All or nothing: a step that does not fit (too few free blocks, a length
+ * negative or beyond max_blocks * page, more than `tokens` new tokens, a stack
+ * height outside [0, capacity] or that would outgrow it) changes nothing, gives
+ * the old lengths and height, cu_q all 0 and every token -1, and records
+ * WH_ERR_DEVICE_ARG for wh_ctx_sync. */
+wh_status wh_kv_plan(wh_ctx* ctx, int requests, int page, int max_blocks, int tokens,
+                     const int32_t* kv_lens, const int32_t* q_lens, const uint8_t* finished,
+                     int32_t* block_table, int32_t* free_blocks, int capacity,
+                     const int32_t* free_top, int32_t* free_top_out, int32_t* kv_lens_out,
+                     int32_t* cu_q, int64_t* slots, int32_t* positions, int32_t* token_requests,
+                     void* scratch, size_t scratch_bytes, wh_stream_t stream);
+
+/* Quantises rows [rows][kv_heads][head_dim] of `dtype` (row and head strides in
+ * elements, rows 16-byte aligned) into the cache's slots.  Per 32 values: the
+ * least power of two 2^k in [2^-126, 2^125] with max|x| <= 6 * 2^k (scale byte
+ * 0 for an all-zero block, 255 where a value is not finite), codes rounded to
+ * nearest, ties to even, saturated.  slots < 0 are skipped, slots past the pool
+ * are skipped and recorded as WH_ERR_DEVICE_ARG; two rows with one slot leave
+ * either.  v: the values' rows (NULL exactly when the cache's values are). */
+wh_status wh_kv_append(wh_ctx* ctx, const wh_kv_cache* cache, const int64_t* slots, int rows,
+                       const void* k, const void* v, int dtype, long long k_row_stride,
+                       long long k_head_stride, long long v_row_stride, long long v_head_stride,
+                       wh_stream_t stream);
+/* The rows of `slots` as values: k, v [rows][kv_heads][head_dim] of `dtype`,
+ * dense (v nullable).  A slot < 0 gives zeros; one past the pool gives zeros
+ * and records WH_ERR_DEVICE_ARG. */
+wh_status wh_kv_gather(wh_ctx* ctx, const wh_kv_cache* cache, const int64_t* slots, int rows,
+                       void* k, void* v, int dtype, wh_stream_t stream);
+
+/* Device scratch bytes of wh_kv_attention. */
+size_t wh_kv_attention_scratch_bytes(const wh_ctx* ctx, const wh_kv_cache* cache, int tokens,
+                                     int heads, int requests, int dtype);
+/* Softmax attention of `tokens` queries q [tokens][heads][head_dim] over the
+ * cached rows; query head h reads kv head h / (heads / kv_heads).  Request r
+ * owns the queries [cu_q[r], cu_q[r + 1]) (cu_q NULL: one each, tokens ==
+ * requests) and kv_lens[r] rows, its own new ones included, in the blocks of
+ * block_table [requests][max_blocks]: query j of n sits at position p =
+ * kv_lens[r] - n + j and sees row i when i <= p and (window == 0, or i > p -
+ * window, or i < first).  sink (nullable) [heads]: a logit that takes part in
+ * each softmax and has no value.  A query that sees no row gives zeros.
+ *   out [tokens][heads][head_dim] of q's dtype; strides in elements, rows of q
+ * and out 16-byte aligned and contiguous.  Rows of tokens from cu_q[requests]
+ * on are not written.  Sums, maxima and normalisers are f32; f32 queries give
+ * f32 accuracy.  Not-finite rows reach only the queries that see them.
+ * Block ids outside the pool and lengths beyond max_blocks * page are recorded
+ * as WH_ERR_DEVICE_ARG; such rows count as not seen. */
+wh_status wh_kv_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void* q, int dtype,
+                          int tokens, int heads, long long q_token_stride,
+                          long long q_head_stride, int requests, const int32_t* cu_q,
+                          const int32_t* kv_lens, const int32_t* block_table, int max_blocks,
+                          float scale, int window, int first, const float* sink, void* out,
+                          long long out_token_stride, long long out_head_stride, void* scratch,
+                          size_t scratch_bytes, wh_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* ZCBLK01 tensor blocks (host memory; no device work)                        */
 /* ------------------------------------------------------------------------ */
 /* A block is [header 40 B][records 52 B each][names][data][shapes]; all

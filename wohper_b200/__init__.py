@@ -82,7 +82,8 @@ EXPORTS = (
     "wh_mla_attention", "wh_debug_expf_table", "wh_debug_expf_near", "wh_debug_ref_expf", "wh_hc_pre",
     "wh_hc_post", "wh_hc_head", "wh_rms_norm", "wh_fp8_gemv_grouped",
     "wh_v4_attention_scratch_len", "wh_v4_attention", "wh_lm_head_batch_scratch_bytes",
-    "wh_lm_head_topk_batch",
+    "wh_lm_head_topk_batch", "wh_kv_plan_scratch_bytes", "wh_kv_plan", "wh_kv_append",
+    "wh_kv_gather", "wh_kv_attention_scratch_bytes", "wh_kv_attention",
 )
 
 
@@ -202,6 +203,14 @@ def lib(build_if_missing: bool = True) -> C.CDLL:
         "wh_lm_head_batch_scratch_bytes": (sz, [C.c_longlong, i, i]),
         "wh_lm_head_topk_batch": (st, [vp, vp, C.c_longlong, i, C.c_uint32, vp, i, i, i, vp, vp,
                                        vp, vp, sz, vp]),
+        "wh_kv_plan_scratch_bytes": (sz, [i]),
+        "wh_kv_plan": (st, [vp, i, i, i, i, vp, vp, vp, vp, vp, i, vp, vp, vp, vp, vp, vp, vp, vp,
+                            sz, vp]),
+        "wh_kv_append": (st, [vp, vp, vp, i, vp, vp, i] + [C.c_longlong] * 4 + [vp]),
+        "wh_kv_gather": (st, [vp, vp, vp, i, vp, vp, i, vp]),
+        "wh_kv_attention_scratch_bytes": (sz, [vp, vp, i, i, i, i]),
+        "wh_kv_attention": (st, [vp, vp, vp, i, i, i, C.c_longlong, C.c_longlong, i, vp, vp, vp,
+                                 i, f, i, i, vp, vp, C.c_longlong, C.c_longlong, vp, sz, vp]),
         "wh_zcblk_parse": (st, [vp, sz, vp]),
         "wh_zcblk_tensor_at": (st, [vp, sz, C.c_uint32, vp]),
         "wh_zcblk_tensor_dim": (st, [vp, sz, vp, C.c_uint32, vp]),
@@ -789,3 +798,7 @@ class MoeLayer:
             self.close()
         except Exception:
             pass
+
+
+from .kvcache import (KvPlan, PagedKvCache, kv_append, kv_attention, kv_gather,  # noqa: E402,F401
+                      kv_plan)

@@ -1,0 +1,241 @@
+// kvattn.cu -- attention over the paged 4-bit key/value cache.
+//
+// Query row (token t of request r at position p, head h), over the rows i it
+// sees (kv_span):
+//   s_i = scale * q . k_i        m = max_i s_i       l = sum_i e^(s_i - m)
+//   o = sum_i e^(s_i - m) v_i / (l + e^(sink - m))
+// in one pass over the rows with a running maximum: when m grows, l and o
+// shrink by e^(m_old - m).
+#include "kvattn.cuh"
+
+namespace wh {
+
+// ---------------------------------------------------------------------------
+// One query row per CTA on the CUDA cores, f32 throughout: any head_dim that is
+// a multiple of 32, any scale byte, any value of q.
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 128;
+struct KvRowSmem {
+  float q[512];
+  float p[kRowThreads];
+  long long row[kRowThreads];    // row index in its block (code and scale offsets follow)
+  int block[kRowThreads];
+  float red[8];
+  float acc[kRowThreads * 8];
+};
+
+__device__ __forceinline__ float row_reduce_max(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+__device__ __forceinline__ float row_reduce_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+template <class T>
+__device__ void kv_attend_row(const KvAttnArgs& a, int r, int t, int h, KvRowSmem& sm) {
+  const int tid = threadIdx.x;
+  const int D = a.c.head_dim, parts = D / 8;
+  const int kvh = h / a.group;
+  const int2 tq = kv_queries(a, r);
+  const int p = a.kv_lens[r] - tq.y + (t - tq.x);
+  const int n = kv_rows_of(a, r);
+  if (tid == 0 && n != a.kv_lens[r]) flag(a.status, WH_DEV_BADARG);
+  const KvSpan sp = kv_span(a, p, n);
+  const int seen = sp.head + sp.end - sp.start;
+  const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_token_stride + h * a.q_head_stride;
+  __syncthreads();
+  if (tid < parts) {
+    float v[8];
+    kv_load8(q + tid * 8, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sm.q[tid * 8 + j] = v[j];
+  }
+  // value columns: lane group `part` of 8 columns, keys sub, sub + subs, ...
+  const int subs = kRowThreads / parts, part = tid % parts, sub = tid / parts;
+  const float inf = __int_as_float(0x7f800000);
+  float m = -inf, l = 0.0f;
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int u0 = 0; u0 < seen; u0 += kRowThreads) {
+    __syncthreads();
+    const int u = u0 + tid;
+    float s = -inf;
+    int block = -1;
+    long long row = 0;
+    if (u < seen) {
+      const int i = u < sp.head ? u : sp.start + (u - sp.head);
+      block = a.block_table[(long long)r * a.max_blocks + i / a.c.page];
+      if (block < 0 || block >= a.c.blocks) {
+        flag(a.status, WH_DEV_BADARG);
+        block = -1;
+      }
+      row = (long long)kvh * a.c.page + i % a.c.page;
+    }
+    if (block >= 0) {
+      const uint8_t* codes = a.c.keys + block * a.c.block_stride + row * (D / 2);
+      const uint8_t* scales = a.c.key_scales + block * a.c.scale_block_stride + row * (D / 32);
+      float dot = 0.0f;
+      for (int b = 0; b < D / 32; ++b) {
+        const uint4 w = reinterpret_cast<const uint4*>(codes)[b];
+        const uint32_t sb = scales[b];
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        float part_sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v[8];
+          kv_decode8(ws[j], sb, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) part_sum = fmaf(v[e], sm.q[b * 32 + j * 8 + e], part_sum);
+        }
+        dot += part_sum;
+      }
+      s = dot * a.scale;
+    }
+    sm.block[tid] = block;
+    sm.row[tid] = row;
+    const float mx = fmaxf(m, row_reduce_max(s, sm.red));  // fmaxf passes over NaN
+    const float base = mx == -inf ? 0.0f : mx;
+    const float shrink = m == -inf ? 0.0f : exp2f((m - base) * kLog2e);
+    const float w = block >= 0 ? exp2f((s - base) * kLog2e) : 0.0f;
+    sm.p[tid] = w;
+    l = l * shrink + row_reduce_sum(w, sm.red);
+    m = mx;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= shrink;
+    const int cnt = min(kRowThreads, seen - u0);
+    if (sub < subs)
+      for (int k = sub; k < cnt; k += subs) {
+        if (sm.block[k] < 0) continue;
+        const uint8_t* codes = a.c.values + sm.block[k] * a.c.block_stride + sm.row[k] * (D / 2);
+        const uint8_t* scales =
+            a.c.value_scales + sm.block[k] * a.c.scale_block_stride + sm.row[k] * (D / 32);
+        float v[8];
+        kv_decode8(reinterpret_cast<const uint32_t*>(codes)[part], scales[part >> 2], v);
+        const float w = sm.p[k];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+      }
+  }
+  // the sink's share, then the sum over the key subsets
+  float o_scale = 1.0f;
+  if (a.sink && seen > 0) {
+    const float sk = a.sink[h];
+    const float mx = fmaxf(m, sk), base = mx == -inf ? 0.0f : mx;
+    o_scale = m == -inf ? 0.0f : exp2f((m - base) * kLog2e);
+    l = l * o_scale + exp2f((sk - base) * kLog2e);
+  }
+  o_scale = l == 0.0f ? 0.0f : o_scale / l;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sm.acc[tid * 8 + e] = acc[e];
+  __syncthreads();
+  if (tid < parts) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = 0.0f;
+      for (int k = 0; k < subs; ++k) x += sm.acc[(k * parts + tid) * 8 + e];
+      v[e] = x * o_scale;
+    }
+    kv_store8(reinterpret_cast<T*>(a.out) + t * a.out_token_stride + h * a.out_head_stride +
+                  tid * 8,
+              v);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(KvAttnArgs a) {
+  __shared__ KvRowSmem sm;
+  pdl_wait_prior();
+  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int r = kv_request_of(a, t);
+  if (r < 0) return;
+  kv_attend_row<T>(a, r, t, h, sm);
+}
+
+}  // namespace wh
+
+// ---------------------------------------------------------------------------
+// C entry points
+// ---------------------------------------------------------------------------
+extern "C" {
+
+size_t wh_kv_attention_scratch_bytes(const wh_ctx* c, const wh_kv_cache* cache, int tokens,
+                                     int heads, int requests, int dtype) {
+  if (!c || !cache || tokens < 1 || heads < 1 || requests < 1) return 0;
+  (void)dtype;
+  return 256;
+}
+
+wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, int dtype,
+                          int tokens, int heads, long long q_token_stride,
+                          long long q_head_stride, int requests, const int32_t* cu_q,
+                          const int32_t* kv_lens, const int32_t* block_table, int max_blocks,
+                          float scale, int window, int first, const float* sink, void* out,
+                          long long out_token_stride, long long out_head_stride, void* scratch,
+                          size_t scratch_bytes, wh_stream_t stream) {
+  if (!c) return fail(WH_ERR_INVALID_POINTER, "ctx is null");
+  KvAttnArgs a{};
+  if (wh_status st = kv_cache_check(cache, &a.c)) return st;
+  int size;
+  if (!kv_dtype_size(dtype, &size)) return fail(WH_ERR_UNSUPPORTED, "attention: dtype");
+  if (requests < 1 || heads < 1 || max_blocks < 1)
+    return fail(WH_ERR_EMPTY_SHAPE, "attention: requests, heads, max_blocks");
+  if (tokens < 0 || heads % cache->kv_heads != 0 || window < 0 || first < 0 ||
+      (!cu_q && tokens != requests))
+    return fail(WH_ERR_INVALID_SHAPE, "attention: tokens, heads % kv_heads, window, first");
+  if (tokens == 0) return WH_OK;
+  if ((long long)max_blocks * cache->page > 0x7fffffffLL)
+    return fail(WH_ERR_UNSUPPORTED, "attention: max_blocks * page > 2^31 - 1");
+  if ((long long)tokens * heads > 0x7fffffffLL)
+    return fail(WH_ERR_UNSUPPORTED, "attention: tokens * heads > 2^31 - 1");
+  if (!(scale == scale) || scale - scale != 0.0f)
+    return fail(WH_ERR_INVALID_SHAPE, "attention: scale is not finite");
+  if (!q || !kv_lens || !block_table || !out || !scratch)
+    return fail(WH_ERR_INVALID_POINTER, "attention: null pointer");
+  if (!kv_rows_aligned(q, q_token_stride, q_head_stride, size) ||
+      !kv_rows_aligned(out, out_token_stride, out_head_stride, size))
+    return fail(WH_ERR_INVALID_POINTER, "attention: rows of q and out must start on 16 bytes");
+  if (scratch_bytes < wh_kv_attention_scratch_bytes(c, cache, tokens, heads, requests, dtype))
+    return fail(WH_ERR_SCRATCH_TOO_SMALL, "attention: scratch too small");
+  a.q = q;
+  a.out = out;
+  a.dtype = dtype;
+  a.tokens = tokens;
+  a.heads = heads;
+  a.group = heads / cache->kv_heads;
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.out_token_stride = out_token_stride;
+  a.out_head_stride = out_head_stride;
+  a.requests = requests;
+  a.cu_q = cu_q;
+  a.kv_lens = kv_lens;
+  a.block_table = block_table;
+  a.max_blocks = max_blocks;
+  a.scale = scale;
+  a.window = window;
+  a.first = first;
+  a.sink = sink;
+  a.status = c->status;
+  const cudaStream_t s = (cudaStream_t)stream;
+  const dim3 grid((unsigned)((long long)tokens * heads));
+  if (dtype == WH_DTYPE_F32)
+    WH_CUDA(launch_pdl(kv_attend_row_kernel<float>, grid, kRowThreads, 0, s, c->pdl(), a));
+  else if (dtype == WH_DTYPE_BF16)
+    WH_CUDA(launch_pdl(kv_attend_row_kernel<__nv_bfloat16>, grid, kRowThreads, 0, s, c->pdl(), a));
+  else
+    WH_CUDA(launch_pdl(kv_attend_row_kernel<__half>, grid, kRowThreads, 0, s, c->pdl(), a));
+  return WH_OK;
+}
+
+}  // extern "C"

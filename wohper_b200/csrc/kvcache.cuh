@@ -1,0 +1,98 @@
+// kvcache.cuh -- layout and decoding of the paged 4-bit key/value cache, shared
+// by its kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace wh {
+
+struct KvCacheDev {
+  int blocks, page, kv_heads, head_dim;
+  int shared;  // the values are the keys
+  uint8_t *keys, *key_scales, *values, *value_scales;
+  long long block_stride, scale_block_stride;  // bytes
+};
+
+// Slot s holds row s % page of block s / page; a head's rows are contiguous in
+// their block.  kv_row: the row's index among its block's rows.
+__device__ __forceinline__ long long kv_row(const KvCacheDev& c, int64_t slot, int head) {
+  return (long long)head * c.page + (long long)(slot % c.page);
+}
+__device__ __forceinline__ long long kv_code_offset(const KvCacheDev& c, int64_t slot,
+                                                    long long row) {
+  return (slot / c.page) * c.block_stride + row * (c.head_dim / 2);
+}
+__device__ __forceinline__ long long kv_scale_offset(const KvCacheDev& c, int64_t slot,
+                                                     long long row) {
+  return (slot / c.page) * c.scale_block_stride + row * (c.head_dim / 32);
+}
+
+constexpr uint32_t kKvScaleNan = 253;  // scale bytes from here on: the block is not finite
+
+// The scale a byte stands for, NaN from kKvScaleNan on.
+__device__ __forceinline__ float kv_scale(uint32_t b) {
+  return b >= kKvScaleNan ? __uint_as_float(0x7fc00000u) : decode_ue8m0(b);
+}
+// One byte of codes -> the two OCP E2M1 values, low nibble first.
+__device__ __forceinline__ float2 e2m1x2_to_f2(uint32_t byte) {
+  uint32_t h;
+  asm("{ .reg .b8 t; cvt.u8.u32 t, %1; cvt.rn.f16x2.e2m1x2 %0, t; }" : "=r"(h) : "r"(byte));
+  return h2_to_f2(h);
+}
+// 8 codes of one block of 32 (code i in bits 4i..4i+3) -> values
+__device__ __forceinline__ void kv_decode8(uint32_t w, uint32_t scale_byte, float (&v)[8]) {
+  const float s = kv_scale(scale_byte);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = e2m1x2_to_f2((w >> (8 * j)) & 0xFFu);
+    v[2 * j] = __fmul_rn(f.x, s);
+    v[2 * j + 1] = __fmul_rn(f.y, s);
+  }
+}
+
+// 8 consecutive elements, 16-byte aligned
+__device__ __forceinline__ void kv_load8(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void kv_load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(w[j] << 16);
+    v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void kv_load8(const __half* p, float (&v)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = h2_to_f2(w[j]);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void kv_store8(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void kv_store8(__nv_bfloat16* p, const float (&v)[8]) {
+  union { uint4 u; __nv_bfloat162 h[4]; } o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o.h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<uint4*>(p) = o.u;
+}
+__device__ __forceinline__ void kv_store8(__half* p, const float (&v)[8]) {
+  union { uint4 u; __half2 h[4]; } o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o.h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<uint4*>(p) = o.u;
+}
+
+}  // namespace wh
