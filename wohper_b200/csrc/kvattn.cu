@@ -47,10 +47,10 @@ __device__ void kv_attend_row(const KvAttnArgs& a, int r, int t, int h, KvRowSme
   const int D = a.c.head_dim, parts = D / 8;
   const int kvh = h / a.group;
   const int2 tq = kv_queries(a, r);
-  const int p = a.kv_lens[r] - tq.y + (t - tq.x);
+  const int p = max(a.kv_lens[r], 0) - tq.y + (t - tq.x);
   const int n = kv_rows_of(a, r);
   if (tid == 0 && n != a.kv_lens[r]) flag(a.status, WH_DEV_BADARG);
-  const KvSpan sp = kv_span(a, p, n);
+  const KvSpan sp = kv_span(a, p, p, n);
   const int seen = sp.head + sp.end - sp.start;
   const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_token_stride + h * a.q_head_stride;
   __syncthreads();
@@ -162,18 +162,166 @@ __global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(KvAttnArgs a
   kv_attend_row<T>(a, r, t, h, sm);
 }
 
+// ---------------------------------------------------------------------------
+// Joins the tensor-core kernel's partial sums of items that lie in several CTAs
+// (one query row and 128 columns a CTA; a row in one piece leaves at once), and
+// computes rows again that the f16 tiles cannot hold.  The parts are added in
+// the order of the rows they cover.
+// ---------------------------------------------------------------------------
+template <class T>
+__global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWork w) {
+  __shared__ KvRowSmem sm;
+  pdl_wait_prior();
+  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int first = a.cu_q ? max(a.cu_q[0], 0) : 0;
+  const int past = a.cu_q ? a.cu_q[a.requests] : a.requests;
+  if (t < first || t >= past) return;
+  const int4 mt = w.meta[blockIdx.x];
+  const int parts = mt.y, row = mt.z >> 1;
+  if (mt.x < 0 || parts < 1 || mt.x + parts > w.ctas || row < 0 || row >= w.rn) {
+    flag(a.status, WH_DEV_BADARG);  // the tensor-core kernel gave up on a wait
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto slot_of = [&](int p) { return 2 * (mt.x + p) + (p == 0 ? mt.z & 1 : 0); };
+  const float inf = __int_as_float(0x7f800000);
+  int redo = mt.w;
+  float top = -inf;
+  if (parts > 1)
+    for (int p = lane; p < parts; p += 32) {
+      redo |= w.part_redo[slot_of(p)];
+      top = fmaxf(top, w.part_ml[(long long)slot_of(p) * w.rn + row].x);
+    }
+  redo = __any_sync(0xffffffffu, redo);
+  if (redo) {
+    const int r = kv_request_of(a, t);
+    if (blockIdx.y == 0 && r >= 0) kv_attend_row<T>(a, r, t, h, sm);
+    return;
+  }
+  if (parts == 1) return;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float sk = a.sink ? a.sink[h] * kLog2e : -inf;
+  const float to = fmaxf(top, sk), base = to == -inf ? 0.0f : to;
+  float z = 0.0f;
+  for (int p = lane; p < parts; p += 32) {
+    const float2 ml = w.part_ml[(long long)slot_of(p) * w.rn + row];
+    z += ml.x == -inf ? 0.0f : ml.y * exp2f(ml.x - base);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  if (a.sink) z += exp2f(sk - base + kLift);
+  const int D = a.c.head_dim, dim = blockIdx.y * 128 + lane * 4;
+  float acc[4] = {0, 0, 0, 0};
+  if (dim < D) {
+#pragma unroll 4
+    for (int p = warp; p < parts; p += kRowThreads / 32) {
+      const long long at = (long long)slot_of(p) * w.rn + row;
+      const float m = w.part_ml[at].x;
+      const float f = m == -inf ? 0.0f : exp2f(m - base);
+      const float4 o = *reinterpret_cast<const float4*>(w.part_o + at * D + dim);
+      acc[0] = fmaf(f, o.x, acc[0]);
+      acc[1] = fmaf(f, o.y, acc[1]);
+      acc[2] = fmaf(f, o.z, acc[2]);
+      acc[3] = fmaf(f, o.w, acc[3]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sm.acc[(warp * 32 + lane) * 4 + e] = acc[e];
+  __syncthreads();
+  if (warp == 0 && dim < D) {
+    const float inv = z == 0.0f ? 0.0f : 1.0f / z;
+    T* out = reinterpret_cast<T*>(a.out) + t * a.out_token_stride + h * a.out_head_stride + dim;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kRowThreads / 32; ++k) v += sm.acc[(k * 32 + lane) * 4 + e];
+      out[e] = T(v * inv);
+    }
+  }
+}
+
 }  // namespace wh
 
 // ---------------------------------------------------------------------------
 // C entry points
 // ---------------------------------------------------------------------------
+namespace {
+
+// How the tensor-core kernel cuts the call's queries; false where head_dim has
+// no instance (the row kernel then takes the call).
+struct KvTcPlan {
+  int n;       // columns of the products
+  bool split;  // two columns a query row
+  KvWork w;
+};
+bool kv_tc_plan(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads, int requests,
+                int dtype, KvTcPlan* p) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512) return false;
+  const int group = heads / kv_heads;
+  p->split = dtype == WH_DTYPE_F32;
+  const long long each = (long long)group * ((tokens + requests - 1) / requests);
+  p->n = each * (p->split ? 2 : 1) <= 16 ? 16 : 64;
+  p->w = KvWork{};
+  p->w.rn = p->split ? p->n / 2 : p->n;
+  p->w.tt = std::max(1, p->w.rn / group);
+  p->w.ht = (group + p->w.rn - 1) / p->w.rn;
+  p->w.ctas = c->num_sms;
+  p->w.min_tiles = head_dim == 512 ? 2 : 4;
+  return true;
+}
+// Places the scratch arrays; returns their bytes.
+size_t kv_tc_scratch(KvTcPlan* p, int head_dim, int tokens, int heads, uint8_t* base) {
+  KvWork& w = p->w;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* q = base + at;
+    at += align256(bytes);
+    return q;
+  };
+  const size_t slots = 2 * (size_t)w.ctas;
+  w.meta = reinterpret_cast<int4*>(take(sizeof(int4) * tokens * heads));
+  w.part_o = reinterpret_cast<float*>(take(sizeof(float) * slots * w.rn * head_dim));
+  w.part_ml = reinterpret_cast<float2*>(take(sizeof(float2) * slots * w.rn));
+  w.part_redo = reinterpret_cast<int*>(take(sizeof(int) * slots));
+  return at;
+}
+template <int kD>
+cudaError_t kv_launch_tc(const KvAttnArgs& a, const KvTcPlan& p, cudaStream_t s, bool pdl) {
+  if (p.n == 16)
+    return p.split ? launch_attend_tc<kD, 16, true>(a, p.w, s, pdl)
+                   : launch_attend_tc<kD, 16, false>(a, p.w, s, pdl);
+  return p.split ? launch_attend_tc<kD, 64, true>(a, p.w, s, pdl)
+                 : launch_attend_tc<kD, 64, false>(a, p.w, s, pdl);
+}
+template <class T>
+cudaError_t kv_launch(const KvAttnArgs& a, const KvTcPlan* p, cudaStream_t s, bool pdl) {
+  const unsigned rows = (unsigned)((long long)a.tokens * a.heads);
+  if (!p) return launch_pdl(kv_attend_row_kernel<T>, dim3(rows), kRowThreads, 0, s, pdl, a);
+  const int d = a.c.head_dim;
+  const cudaError_t e = d == 512   ? kv_launch_tc<512>(a, *p, s, pdl)
+                        : d == 256 ? kv_launch_tc<256>(a, *p, s, pdl)
+                        : d == 128 ? kv_launch_tc<128>(a, *p, s, pdl)
+                                   : kv_launch_tc<64>(a, *p, s, pdl);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kv_join_kernel<T>, dim3(rows, std::max(1, d / 128)), kRowThreads, 0, s, pdl, a,
+                    p->w);
+}
+
+}  // namespace
+
 extern "C" {
 
 size_t wh_kv_attention_scratch_bytes(const wh_ctx* c, const wh_kv_cache* cache, int tokens,
                                      int heads, int requests, int dtype) {
-  if (!c || !cache || tokens < 1 || heads < 1 || requests < 1) return 0;
-  (void)dtype;
-  return 256;
+  if (!c || !cache || tokens < 1 || heads < 1 || requests < 1 || cache->kv_heads < 1 ||
+      heads % cache->kv_heads != 0)
+    return 0;
+  KvTcPlan p;
+  if (!kv_tc_plan(c, cache->head_dim, cache->kv_heads, tokens, heads, requests, dtype, &p))
+    return 256;
+  return kv_tc_scratch(&p, cache->head_dim, tokens, heads, nullptr);
 }
 
 wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, int dtype,
@@ -202,6 +350,8 @@ wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, in
     return fail(WH_ERR_INVALID_SHAPE, "attention: scale is not finite");
   if (!q || !kv_lens || !block_table || !out || !scratch)
     return fail(WH_ERR_INVALID_POINTER, "attention: null pointer");
+  if (!aligned(scratch, 16))
+    return fail(WH_ERR_INVALID_POINTER, "attention: scratch must be 16-byte aligned");
   if (!kv_rows_aligned(q, q_token_stride, q_head_stride, size) ||
       !kv_rows_aligned(out, out_token_stride, out_head_stride, size))
     return fail(WH_ERR_INVALID_POINTER, "attention: rows of q and out must start on 16 bytes");
@@ -227,14 +377,18 @@ wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, in
   a.first = first;
   a.sink = sink;
   a.status = c->status;
+  // a window that holds every row the table can is none
+  if (window >= (long long)max_blocks * cache->page) a.window = 0;
   const cudaStream_t s = (cudaStream_t)stream;
-  const dim3 grid((unsigned)((long long)tokens * heads));
+  KvTcPlan p;
+  const bool tc = kv_tc_plan(c, cache->head_dim, cache->kv_heads, tokens, heads, requests, dtype, &p);
+  if (tc) kv_tc_scratch(&p, cache->head_dim, tokens, heads, static_cast<uint8_t*>(scratch));
   if (dtype == WH_DTYPE_F32)
-    WH_CUDA(launch_pdl(kv_attend_row_kernel<float>, grid, kRowThreads, 0, s, c->pdl(), a));
+    WH_CUDA(kv_launch<float>(a, tc ? &p : nullptr, s, c->pdl()));
   else if (dtype == WH_DTYPE_BF16)
-    WH_CUDA(launch_pdl(kv_attend_row_kernel<__nv_bfloat16>, grid, kRowThreads, 0, s, c->pdl(), a));
+    WH_CUDA(kv_launch<__nv_bfloat16>(a, tc ? &p : nullptr, s, c->pdl()));
   else
-    WH_CUDA(launch_pdl(kv_attend_row_kernel<__half>, grid, kRowThreads, 0, s, c->pdl(), a));
+    WH_CUDA(kv_launch<__half>(a, tc ? &p : nullptr, s, c->pdl()));
   return WH_OK;
 }
 
