@@ -20,7 +20,7 @@
 // one f16 for 16-bit queries (11 bits), two for f32.  Sums are f32.
 //
 // Warps: 0-3 softmax and epilogue (TMEM lane quadrants), 4-11 decode, 12 MMA,
-// 13 addresses (walks the work list, looks up blocks, asks L2 for the rows).
+// 13 addresses (walks the work list, looks up blocks).
 #include "kvattn.cuh"
 #include "tc.cuh"
 
@@ -138,9 +138,6 @@ __device__ __forceinline__ bool decode_block(const uint4& c, uint32_t sb, bool s
   return in;
 }
 
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -374,11 +371,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           all = all && b >= 0 && ck[k] <= x.p0 &&
                 (a.window == 0 || ck[k] > p1 - a.window || ck[k] < a.first);
           f.row[lane + 32 * k] = make_int2(b, row);
-          if (b >= 0) {
-            prefetch_l2(a.c.keys + b * a.c.block_stride + (long long)row * (kD / 2), kD / 2);
-            if (sep)
-              prefetch_l2(a.c.values + b * a.c.block_stride + (long long)row * (kD / 2), kD / 2);
-          }
         }
         all = __all_sync(0xffffffffu, all);
         if (lane == 0) {
