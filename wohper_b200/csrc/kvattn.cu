@@ -252,19 +252,15 @@ namespace {
 // How the tensor-core kernel cuts the call's queries; false where head_dim has
 // no instance (the row kernel then takes the call).
 struct KvTcPlan {
-  int n;       // columns of the products
   bool split;  // two columns a query row
   KvWork w;
 };
-bool kv_tc_plan(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads, int requests,
-                int dtype, KvTcPlan* p) {
+bool kv_tc_plan(const wh_ctx* c, int head_dim, int kv_heads, int heads, int dtype, KvTcPlan* p) {
   if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512) return false;
   const int group = heads / kv_heads;
   p->split = dtype == WH_DTYPE_F32;
-  const long long each = (long long)group * ((tokens + requests - 1) / requests);
-  p->n = each * (p->split ? 2 : 1) <= 16 ? 16 : 64;
   p->w = KvWork{};
-  p->w.rn = p->split ? p->n / 2 : p->n;
+  p->w.rn = p->split ? kTcCols / 2 : kTcCols;
   p->w.tt = std::max(1, p->w.rn / group);
   p->w.ht = (group + p->w.rn - 1) / p->w.rn;
   p->w.ctas = c->num_sms;
@@ -289,11 +285,11 @@ size_t kv_tc_scratch(KvTcPlan* p, int head_dim, int tokens, int heads, uint8_t* 
 }
 template <int kD>
 cudaError_t kv_launch_tc(const KvAttnArgs& a, const KvTcPlan& p, cudaStream_t s, bool pdl) {
-  if (p.n == 16)
-    return p.split ? launch_attend_tc<kD, 16, true>(a, p.w, s, pdl)
-                   : launch_attend_tc<kD, 16, false>(a, p.w, s, pdl);
-  return p.split ? launch_attend_tc<kD, 64, true>(a, p.w, s, pdl)
-                 : launch_attend_tc<kD, 64, false>(a, p.w, s, pdl);
+  if (a.c.shared)
+    return p.split ? launch_attend_tc<kD, true, false>(a, p.w, s, pdl)
+                   : launch_attend_tc<kD, false, false>(a, p.w, s, pdl);
+  return p.split ? launch_attend_tc<kD, true, true>(a, p.w, s, pdl)
+                 : launch_attend_tc<kD, false, true>(a, p.w, s, pdl);
 }
 template <class T>
 cudaError_t kv_launch(const KvAttnArgs& a, const KvTcPlan* p, cudaStream_t s, bool pdl) {
@@ -319,7 +315,7 @@ size_t wh_kv_attention_scratch_bytes(const wh_ctx* c, const wh_kv_cache* cache, 
       heads % cache->kv_heads != 0)
     return 0;
   KvTcPlan p;
-  if (!kv_tc_plan(c, cache->head_dim, cache->kv_heads, tokens, heads, requests, dtype, &p))
+  if (!kv_tc_plan(c, cache->head_dim, cache->kv_heads, heads, dtype, &p))
     return 256;
   return kv_tc_scratch(&p, cache->head_dim, tokens, heads, nullptr);
 }
@@ -381,7 +377,7 @@ wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, in
   if (window >= (long long)max_blocks * cache->page) a.window = 0;
   const cudaStream_t s = (cudaStream_t)stream;
   KvTcPlan p;
-  const bool tc = kv_tc_plan(c, cache->head_dim, cache->kv_heads, tokens, heads, requests, dtype, &p);
+  const bool tc = kv_tc_plan(c, cache->head_dim, cache->kv_heads, heads, dtype, &p);
   if (tc) kv_tc_scratch(&p, cache->head_dim, tokens, heads, static_cast<uint8_t*>(scratch));
   if (dtype == WH_DTYPE_F32)
     WH_CUDA(kv_launch<float>(a, tc ? &p : nullptr, s, c->pdl()));

@@ -75,7 +75,6 @@ struct KvWork {
   int tt;  // tokens of an item
   int ht;  // items that one token's heads of one kv head take
   int ctas, min_tiles;
-  int kstages, vstages;
   int4* meta;       // [tokens][heads]: first CTA, CTAs, its slot, redo
   float* part_o;    // [2 * ctas][rn][head_dim]
   float2* part_ml;  // [2 * ctas][rn]: maximum (base 2), sum

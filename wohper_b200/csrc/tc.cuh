@@ -121,6 +121,13 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_mn, bool b
   return 1u << 4 | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | (uint32_t(n) >> 3) << 17 |
          (uint32_t(m) >> 4) << 24;
 }
+// One lane of the converged warp.  Code under it stays uniform to the compiler,
+// which then keeps the descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(ok));
+  return ok != 0;
+}
 // D[tmem_d] (+)= A * B; accumulate = 0 overwrites D.
 __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -132,23 +139,13 @@ __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t da, uint64_t d
 }
 // 16 lanes x 8 * kX columns: thread t gets, for each 8-column group j, row t / 4
 // columns 2 (t % 4), + 1 in v[4j], v[4j + 1] and row t / 4 + 8 in v[4j + 2], v[4j + 3].
-__device__ __forceinline__ void ld_16x256b(uint32_t taddr, uint32_t (&v)[8]) {
+__device__ __forceinline__ void ld_16x256b(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void ld_16x256b(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
         "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
-        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
 }
 __device__ __forceinline__ void st_32x32b_x16(uint32_t taddr, const uint32_t (&v)[16]) {
