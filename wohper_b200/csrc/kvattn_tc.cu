@@ -83,7 +83,8 @@ struct KvTc {
   struct Misc {
     KvTileInfo info[kTcInfo];
     float fac[kTcFrag][kRn];   // accumulator -> log2 score, per query row
-    float red[2][4][kRn];
+    float red[2][4][kRn];      // a tile's maxima, a fragment's sums
+    float top[kRn];
     float out_scale[kRn];
     float shrink[kRn];
     long long out_row[kRn];    // where a row goes, in elements
@@ -112,15 +113,14 @@ struct KvTcSmem {
   static_assert(kStages >= (kSep ? 1 : 2), "shared memory over 227 KB");
 };
 
-// 8 codes (code i in bits 4i..4i+3) -> 8 f16 with the high bytes of their
-// magnitudes looked up in t0 (codes 0-3) and t1 (4-7); every value has a zero low byte.
-__device__ __forceinline__ uint4 e2m1x8_to_f16(uint32_t w, uint32_t t0, uint32_t t1) {
-  const uint32_t mag = w & 0x77777777u, w4 = w << 4;
-  uint32_t lo = __byte_perm(t0, t1, mag), hi = __byte_perm(t0, t1, mag >> 16);
-  lo |= __byte_perm(w4, w, 0x5140) & 0x80808080u;  // sign of code i at bit 7 of byte i
-  hi |= __byte_perm(w4, w, 0x7362) & 0x80808080u;
-  return make_uint4(__byte_perm(lo, 0, 0x1404), __byte_perm(lo, 0, 0x3424),
-                    __byte_perm(hi, 0, 0x1404), __byte_perm(hi, 0, 0x3424));
+// 8 codes (code i in bits 4i..4i+3) -> 8 f16
+__device__ __forceinline__ uint4 e2m1x8_to_f16(uint32_t w) {
+  uint4 v;
+  asm("{ .reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a;"
+      " cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d; }"
+      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+      : "r"(w));
+  return v;
 }
 __device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -129,33 +129,24 @@ __device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
 
 // One block of 32 codes into four 16-byte pieces of a tile row, piece j at
 // row + at[j].  seen = false: zeros.  Returns false where the scale byte has no
-// exact f16 form.  Whole warps call it; lanes with on = false write nothing.
+// exact f16 form.  Lanes with on = false write nothing.
 __device__ __forceinline__ bool decode_block(const uint4& c, uint32_t sb, bool seen, bool on,
                                              uint8_t* row, const uint32_t (&at)[4]) {
   const int k = int(sb) - kKvBias;
   const bool zero = !seen || sb == 0;
   const bool in = zero || (k >= -23 && k <= 13);
-  const bool sub = !zero && in && k < -13;  // 2^k times a code may be subnormal: multiply
-  // high bytes of 0 0.5 1 1.5 and 2 3 4 6; 2^k adds k to the exponents of all but 0
-  const uint32_t step = sub ? 0u : uint32_t(k);
-  const bool none = zero || !in;
-  const uint32_t t0 = none ? 0u : 0x3E3C3800u + step * 0x04040400u;
-  const uint32_t t1 = none ? 0u : 0x46444240u + step * 0x04040404u;
+  // 2^k as f16, subnormal below 2^-14; the products with codes are exact
+  const uint32_t one = k >= -14 ? uint32_t(k + 15) << 10 : 1u << ((k + 24) & 31);
+  const uint32_t scale = zero || !in ? 0u : one | one << 16;
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
   uint4 v[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = e2m1x8_to_f16(w[j], t0, t1);
-  if (__any_sync(0xffffffffu, sub)) {
-    // 2^k as f16: subnormal below 2^-14
-    const uint32_t m = !sub ? 0x3C00u : k >= -14 ? uint32_t(k + 15) << 10 : 1u << (k + 24);
-    const uint32_t mm = m | m << 16;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j].x = hmul2_u(v[j].x, mm);
-      v[j].y = hmul2_u(v[j].y, mm);
-      v[j].z = hmul2_u(v[j].z, mm);
-      v[j].w = hmul2_u(v[j].w, mm);
-    }
+  for (int j = 0; j < 4; ++j) {
+    v[j] = e2m1x8_to_f16(w[j]);
+    v[j].x = hmul2_u(v[j].x, scale);
+    v[j].y = hmul2_u(v[j].y, scale);
+    v[j].z = hmul2_u(v[j].z, scale);
+    v[j].w = hmul2_u(v[j].w, scale);
   }
   if (on) {
 #pragma unroll
@@ -550,9 +541,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
 #pragma unroll
       for (int b = 0; b < kRows; ++b) {
         const int row = dw + kTcDec * b;
+        // the largest magnitude, as an integer: a NaN or infinity is at least 0x7f800000
         float v[kLoads][8];
-        float top = 0.0f;
-        bool fin = true;
+        uint32_t top = 0;
 #pragma unroll
         for (int g = 0; g < kLoads; ++g) {
           if (kSplit) {
@@ -563,17 +554,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
             kv_widen(raw[b][g], a.dtype, v[g]);
           }
 #pragma unroll
-          for (int e = 0; e < kElems; ++e) {
-            top = fmaxf(top, fabsf(v[g][e]));
-            fin &= isfinite(v[g][e]);
-          }
+          for (int e = 0; e < kElems; ++e) top = max(top, __float_as_uint(v[g][e]) & 0x7fffffffu);
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        fin = __all_sync(0xffffffffu, fin);
+        top = __reduce_max_sync(0xffffffffu, top);
+        const bool fin = top < 0x7f800000u;
         // 2^14 <= top * mul < 2^15; below 2^-100 the row's scores vanish anyway
-        const int ex = max(int(__float_as_uint(top) >> 23) - 127, -100);
+        const int ex = max(int(top >> 23) - 127, -100);
         const float mul = fin ? exp2i(14 - ex) : 0.0f;
+        if (!fin) {
+#pragma unroll
+          for (int g = 0; g < kLoads; ++g)
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) v[g][e] = 0.0f;
+        }
         if (lane == 0) {
           if (!fin) m.redo[frag % kTcRedo] = 1;
           m.fac[frag % kTcFrag][row] = a.scale * kLog2e * exp2i(max(ex - 18, -126));
@@ -586,7 +579,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           uint32_t hi[4], lo[2];
 #pragma unroll
           for (int e = 0; e < kElems / 2; ++e) {
-            const float x = fin ? v[g][2 * e] * mul : 0.0f, y = fin ? v[g][2 * e + 1] * mul : 0.0f;
+            const float x = v[g][2 * e] * mul, y = v[g][2 * e + 1] * mul;
             const __half2 h = __floats2half2_rn(x, y);
             hi[e] = half2_bits(h);
             if (kSplit) lo[e] = half2_bits(__floats2half2_rn(x - __low2float(h), y - __high2float(h)));
@@ -606,19 +599,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       }
     };
     int frag = -1;
+    auto begin_item = [&](const KvTileInfo& f) {
+      ++frag;
+      if (frag > 0 && !warp_wait(&m.q_empty, (frag - 1) & 1, a.status)) return false;
+      // the mark four fragments on is the one four fragments back, whose rows are out
+      if (dw == 0 && lane == 0) m.redo[(frag + 4) % kTcRedo] = 0;
+      load_q(f, frag);
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.q_full[frag % kTcFrag]);
+      return true;
+    };
     auto step = [&](int n, const Raw& x) {
       const int slot = n % kTcInfo, st = n % kStages;
       const KvTileInfo& f = m.info[slot];
-      if (f.flags & kFragFirst) {
-        ++frag;
-        if (frag > 0 && !warp_wait(&m.q_empty, (frag - 1) & 1, a.status)) return false;
-        // the mark four fragments on is the one four fragments back, whose rows are out
-        if (dw == 0 && lane == 0) m.redo[(frag + 4) % kTcRedo] = 0;
-        load_q(f, frag);
-        tc::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m.q_full[frag % kTcFrag]);
-      }
+      if (n > 0 && (f.flags & kFragFirst) && !begin_item(f)) return false;
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.info_empty[slot]);
       bool in = true;
@@ -647,9 +642,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       return true;
     };
     Raw raw[kAhead];
-    bool ok = true;
+    // the first tile's codes travel while the queries are brought in
+    bool ok = ntiles == 0 || (load(0, raw[0]) && begin_item(m.info[0]));
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
+    for (int u = 1; u < kAhead; ++u)
       if (ok && u < ntiles) ok = load(u, raw[u]);
     for (int n0 = 0; ok && n0 < ntiles; n0 += kAhead) {
 #pragma unroll
@@ -677,7 +673,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
     auto product_done = [&](int n) { return warp_wait(&m.p_empty[n & 1], (n >> 1) & 1, a.status); };
     float fac[kMax], mx[kMax], sum[kMax];
     int frag = -1;
-    uint32_t parity = 0;
     bool ok = true;
     for (int n = 0; n < ntiles; ++n) {
       const int slot = n % kTcInfo, b = n & 1;
@@ -726,42 +721,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           }
         }
       }
-      // the tile's maximum per query row: over the warp's 16 keys, then over the warps
-      float* red = &m.red[parity][quad][0];
+      // The running maxima may lag: while no score is more than kLag above its
+      // row's, they stay and the half's warps need only agree on that.
+      bool stay = ok;
 #pragma unroll
-      for (int e = 0; e < kMax; ++e) {
-        float t = fmaxf(s[e][0], s[e][1]);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-        if (g8 == 0) red[row_of(e)] = t;
-      }
+      for (int e = 0; e < kMax; ++e) stay = stay && fmaxf(s[e][0], s[e][1]) <= mx[e] + kLag;
       tc::fence_before_sync();
-      if (!bar_and(bar, 128, ok)) break;
-      float tm[kMax];
-      bool grow = false;
-#pragma unroll
-      for (int e = 0; e < kMax; ++e) {
-        const int r = row_of(e);
-        tm[e] = fmaxf(fmaxf(m.red[parity][0][r], m.red[parity][1][r]),
-                      fmaxf(m.red[parity][2][r], m.red[parity][3][r]));
-        grow |= tm[e] > mx[e] + kLag;
-      }
-      parity ^= 1;
-      // every warp of the half sees every row's maximum, so all four decide alike
-      if (__any_sync(0xffffffffu, grow)) {
+      if (!bar_and(bar, 128, stay)) {
+        // the tile's maxima, over the warp's 16 keys, then over the warps
 #pragma unroll
         for (int e = 0; e < kMax; ++e) {
-          const float to = fmaxf(mx[e], tm[e]);
+          float t = fmaxf(s[e][0], s[e][1]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+          if (g8 == 0) m.red[0][quad][row_of(e)] = t;
+        }
+        if (!bar_and(bar, 128, ok)) break;
+#pragma unroll
+        for (int e = 0; e < kMax; ++e) {
+          const int r = row_of(e);
+          const float t = fmaxf(fmaxf(m.red[0][0][r], m.red[0][1][r]), fmaxf(m.red[0][2][r], m.red[0][3][r]));
+          const float to = fmaxf(mx[e], t);
           const float sh = mx[e] == -inf ? 0.0f : ex2(mx[e] - to);
           mx[e] = to;
           sum[e] *= sh;
-          if (quad == 0 && g8 == 0) m.shrink[row_of(e)] = sh;
+          if (quad == 0 && g8 == 0) m.shrink[r] = sh;
         }
+        if (!(flags & kFragFirst)) ok = product_done(n - 1);
+        tc::fence_after_sync();
+        if (!bar_and(bar, 128, ok)) break;
         if (!(flags & kFragFirst)) {
-          // O^T shrinks too, once the previous tile's product is in it
-          ok = product_done(n - 1);
-          tc::fence_after_sync();
-          if (!bar_and(bar, 128, ok)) break;
+          // O^T shrinks too, now that the previous tile's product is in it
 #pragma unroll 1
           for (int c0 = 0; c0 < kNh; c0 += 16)
 #pragma unroll 1
@@ -811,15 +801,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
 
       if (flags & kFragLast) {
         // ---- the fragment's sums, then its rows: out, or a partial slot ----
-        if (!bar_and(bar, 128, ok)) break;  // every warp has read the maxima in red
 #pragma unroll
         for (int e = 0; e < kMax; ++e) {
           float t = sum[e];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
           if (g8 == 0) {
-            m.red[0][quad][row_of(e)] = t;
-            if (quad == 0) m.red[1][0][row_of(e)] = mx[e];
+            m.red[1][quad][row_of(e)] = t;
+            if (quad == 0) m.top[row_of(e)] = mx[e];
           }
         }
         ok = product_done(n);
@@ -828,13 +817,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         const bool whole = (flags & kItemFirst) && (flags & kItemLast);
         const int rows = w.ht > 1 ? min(kRn, a.group - f.ht * kRn) : f.nt * a.group;
         const int row = half * kRh + quad * 32 + lane;
+        if (quad * 32 + lane < kRh && row >= rows) m.out_row[row] = 0;
         if (quad * 32 + lane < kRh && row < rows) {
           const int redo = m.redo[frag % kTcRedo];
           const int part = 2 * blockIdx.x + (flags & kSlot1 ? 1 : 0);
           const int h = f.kvh * a.group + f.ht * kRn + m.row_head[row];
           const int t = f.t0 + m.row_tok[row];
-          const float l = (m.red[0][0][row] + m.red[0][1][row]) + (m.red[0][2][row] + m.red[0][3][row]);
-          const float top = m.red[1][0][row];
+          const float l = (m.red[1][0][row] + m.red[1][1][row]) + (m.red[1][2][row] + m.red[1][3][row]);
+          const float top = m.top[row];
           float os = 1.0f / 16.0f;  // the tiles hold 16 times the values
           if (whole) {
             float z = l;
@@ -862,25 +852,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         }
         if (!bar_and(bar, 128, ok)) break;
         const int dim = quad * 32 + lane;
+        // eight rows at a time, a 128-row block of O^T after the other
         auto write = [&](auto* out) {
+          if (kD < 128 && quad * 32 >= kD) return;
 #pragma unroll 1
-          for (int c0 = 0; c0 < kNh; c0 += 16) {
-            constexpr int kR = kSplit ? 8 : 16;  // query rows of 16 columns
-            const int row0 = half * kRh + (kSplit ? c0 / 2 : c0);
-            if (row0 >= rows) break;
-#pragma unroll 2
-            for (int blk = 0; blk < L::kBlocks; ++blk) {
-              uint32_t o[16];
-              tc::ld_32x32b_x16(tmem_w + L::kTmemO + blk * kN + c0, o);
-              tc::wait_ld_of(o);
-              if (kD < 128 && dim >= kD) continue;
+          for (int r0 = half * kRh; r0 < half * kRh + kRh; r0 += 8) {
+            if (r0 >= rows) break;
+            long long to[8];
+            float by[8];
 #pragma unroll
-              for (int e = 0; e < kR; ++e) {
-                if (row0 + e >= rows) continue;
-                const float v = kSplit ? __uint_as_float(o[2 * e & 15]) + __uint_as_float(o[(2 * e + 1) & 15])
-                                       : __uint_as_float(o[e]);
-                kv_put(out + m.out_row[row0 + e] + blk * 128 + dim, v * m.out_scale[row0 + e]);
+            for (int e = 0; e < 8; ++e) {
+              to[e] = m.out_row[r0 + e] + dim;
+              by[e] = m.out_scale[r0 + e];
+            }
+            const int live = rows - r0;
+            const uint32_t col = tmem_w + L::kTmemO + (r0 - half * kRh) * (kSplit ? 2 : 1);
+#pragma unroll
+            for (int blk = 0; blk < L::kBlocks; ++blk) {
+              float v[8];
+              if (kSplit) {
+                uint32_t o[16];
+                tc::ld_32x32b_x16(col + blk * kN, o);
+                tc::wait_ld_of(o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[2 * e]) + __uint_as_float(o[2 * e + 1]);
+              } else {
+                uint32_t o[8];
+                tc::ld_32x32b_x8(col + blk * kN, o);
+                tc::wait_ld_of(o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[e]);
               }
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (e < live) kv_put(out + to[e] + blk * 128, v[e] * by[e]);
             }
           }
         };
@@ -895,8 +900,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.o_empty);
-        if (!bar_and(bar, 128, ok)) break;  // red and out_scale may be written again
-        parity = 0;
+        if (!bar_and(bar, 128, ok)) break;  // sums and row tables may be written again
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.info_empty[slot]);
