@@ -34,6 +34,11 @@ namespace wh {
 constexpr int kTcSoft = 8, kTcDec = 16;
 constexpr int kTcMma = kTcSoft + kTcDec, kTcAddr = kTcMma + 1;
 constexpr int kTcThreads = (kTcAddr + 1) * 32;
+// Registers: 72 a thread at launch (26 warps); the decode warps give 8 up, the
+// softmax warps take 16: 8 x 88 + 16 x 64 + 2 x 72 = 26 x 72.
+constexpr int kTcSoftRegs = 88, kTcDecRegs = 64, kTcRegs = 72;
+static_assert(kTcSoft * kTcSoftRegs + kTcDec * kTcDecRegs <= (kTcSoft + kTcDec) * kTcRegs, "registers");
+static_assert(kTcSoft % 4 == 0 && kTcDec % 4 == 0, "whole warpgroups");
 constexpr int kTcInfo = 8;   // tiles the address warp may run ahead
 constexpr int kTcFrag = 4;   // fragments whose query factors are kept
 constexpr int kTcRedo = 8;   // fragments whose redo marks are kept
@@ -155,6 +160,15 @@ __device__ __forceinline__ bool decode_block(const uint4& c, uint32_t sb, bool s
   return in || !on;
 }
 
+// Registers of this warpgroup from here on (every warp of it executes this).
+template <int kRegs>
+__device__ __forceinline__ void regs_more() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_less() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -478,6 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
     mbar_wait(&m.all_done, 0, a.status);
   } else if (warp >= kTcSoft) {
     // ---------------- decode ----------------
+    regs_less<kTcDecRegs>();
     constexpr int kPer = L::kPer, kAhead = L::kAhead;
     const int dw = warp - kTcSoft, rg = dw & 7, dh = dw >> 3;
     const int r7 = lane & 7, pq = lane >> 3;
@@ -521,12 +536,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       constexpr int kLoads = kG > 32 ? kG / 32 : 1;  // of them a lane takes
       constexpr int kRows = kRn / kTcDec;
       constexpr int kElems = kSplit ? 4 : 8;
+      constexpr int kBatch = kLoads >= 4 ? 1 : kRows < 4 / kLoads ? kRows : 4 / kLoads;
       const int rows = w.ht > 1 ? min(kRn, a.group - f.ht * kRn) : f.nt * a.group;
       const uint8_t* q = static_cast<const uint8_t*>(a.q);
-      uint4 raw[kRows][kLoads];
+#pragma unroll 1
+      for (int b0 = 0; b0 < kRows; b0 += kBatch) {
+      uint4 raw[kBatch][kLoads];
 #pragma unroll
-      for (int b = 0; b < kRows; ++b) {
-        const int row = dw + kTcDec * b;
+      for (int b = 0; b < kBatch; ++b) {
+        const int row = dw + kTcDec * (b0 + b);
         const bool real = row < rows;
         const long long off = real ? (f.t0 + m.row_tok[row]) * a.q_token_stride +
                                          (f.kvh * a.group + f.ht * kRn + m.row_head[row]) * a.q_head_stride
@@ -539,8 +557,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         }
       }
 #pragma unroll
-      for (int b = 0; b < kRows; ++b) {
-        const int row = dw + kTcDec * b;
+      for (int b = 0; b < kBatch; ++b) {
+        const int row = dw + kTcDec * (b0 + b);
         // the largest magnitude, as an integer: a NaN or infinity is at least 0x7f800000
         float v[kLoads][8];
         uint32_t top = 0;
@@ -596,6 +614,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
                 make_uint4(hi[0], hi[1], hi[2], hi[3]);
           }
         }
+      }
       }
     };
     int frag = -1;
@@ -657,6 +676,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
     }
   } else {
     // ---------------- softmax, epilogue ----------------
+    regs_more<kTcSoftRegs>();
     constexpr int kMax = L::kMax;
     const float inf = __int_as_float(0x7f800000);
     const int quad = warp & 3, half = warp >> 2, bar = 1 + half;
@@ -667,11 +687,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       return half * kRh + (kSplit ? 4 * e + c4 : 8 * (e >> 1) + 2 * c4 + (e & 1));
     };
     const uint32_t tmem_w = tmem + ((uint32_t)(quad * 32) << 16) + half * kNh;
-    // Tile n's product is in O^T and its weights may be overwritten.  Asked for
-    // n - 2 before tile n's weights are written, so that the phase of p_empty
-    // is never more than one ahead of the one asked for.
+    // Tile n's second product is in O^T.  Once tile n's scores are there, that of
+    // n - 2 is (it was issued before them), so the phase of p_empty is never
+    // more than one ahead of the one asked for.
     auto product_done = [&](int n) { return warp_wait(&m.p_empty[n & 1], (n >> 1) & 1, a.status); };
-    float fac[kMax], mx[kMax], sum[kMax];
+    // log2 weight = score * fac + off, off = kLift - the row's running maximum
+    float fac[kMax], off[kMax], sum[kMax];
+    uint32_t live = 0;  // bit e: the row has seen a key
     int frag = -1;
     bool ok = true;
     for (int n = 0; n < ntiles; ++n) {
@@ -683,11 +705,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       const int flags = ok ? f.flags : 0;
       if (flags & kFragFirst) {
         ++frag;
+        live = 0;
         ok = ok && warp_wait(&m.q_full[frag % kTcFrag], (frag / kTcFrag) & 1, a.status);
 #pragma unroll
         for (int e = 0; e < kMax; ++e) {
           fac[e] = m.fac[frag % kTcFrag][row_of(e)];
-          mx[e] = -inf;
+          off[e] = 0.0f;
           sum[e] = 0.0f;
         }
       }
@@ -696,16 +719,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       uint32_t raw[16];
       tc::ld_16x256b(tmem_w + L::kTmemS + b * kN, raw);
       tc::wait_ld_of(raw);
-      // log2 scores: s[e][0] of key0, s[e][1] of key0 + 8
+      // log2 weights: s[e][0] of key0, s[e][1] of key0 + 8
       float s[kMax][2];
 #pragma unroll
       for (int e = 0; e < kMax; ++e)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (kSplit)
-            s[e][k] = (__uint_as_float(raw[4 * e + 2 * k]) + __uint_as_float(raw[4 * e + 2 * k + 1])) * fac[e];
+            s[e][k] = fmaf(__uint_as_float(raw[4 * e + 2 * k]) + __uint_as_float(raw[4 * e + 2 * k + 1]),
+                           fac[e], off[e]);
           else
-            s[e][k] = __uint_as_float(raw[4 * (e >> 1) + 2 * k + (e & 1)]) * fac[e];
+            s[e][k] = fmaf(__uint_as_float(raw[4 * (e >> 1) + 2 * k + (e & 1)]), fac[e], off[e]);
         }
       if (flags & kTileMasked) {
 #pragma unroll
@@ -721,11 +745,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           }
         }
       }
-      // The running maxima may lag: while no score is more than kLag above its
-      // row's, they stay and the half's warps need only agree on that.
-      bool stay = ok;
+      // The running maxima may lag: while no weight is past 2^(kLift + kLag)
+      // they stay, and the half's warps need only agree on that.
+      float most = -inf;
 #pragma unroll
-      for (int e = 0; e < kMax; ++e) stay = stay && fmaxf(s[e][0], s[e][1]) <= mx[e] + kLag;
+      for (int e = 0; e < kMax; ++e) most = fmaxf(most, fmaxf(s[e][0], s[e][1]));
+      const bool stay = ok && !(flags & kFragFirst) && most <= kLift + kLag;
       tc::fence_before_sync();
       if (!bar_and(bar, 128, stay)) {
         // the tile's maxima, over the warp's 16 keys, then over the warps
@@ -739,11 +764,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         if (!bar_and(bar, 128, ok)) break;
 #pragma unroll
         for (int e = 0; e < kMax; ++e) {
+          // by: how far the row's log2 weights move so that the largest so far is kLift.
+          // A row that has seen nothing has off = 0 and no sum; one that has, moves down only.
           const int r = row_of(e);
           const float t = fmaxf(fmaxf(m.red[0][0][r], m.red[0][1][r]), fmaxf(m.red[0][2][r], m.red[0][3][r]));
-          const float to = fmaxf(mx[e], t);
-          const float sh = mx[e] == -inf ? 0.0f : ex2(mx[e] - to);
-          mx[e] = to;
+          const bool none = t == -inf, was = live >> e & 1;
+          const float by = none ? 0.0f : fminf(kLift - t, was ? 0.0f : inf);
+          const float sh = ex2(was ? by : 0.0f);
+          live |= none ? 0u : 1u << e;
+          off[e] += by;
+          s[e][0] += by;
+          s[e][1] += by;
           sum[e] *= sh;
           if (quad == 0 && g8 == 0) m.shrink[r] = sh;
         }
@@ -770,14 +801,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           if (!bar_and(bar, 128, ok)) break;  // shrink may be written again
         }
       }
-      // weights
-      if (n >= 2) ok = product_done(n - 2);
+      // weights; their buffer is free: the scores' product was issued after the one that read it
       uint8_t* pt = ps + b * L::kPBytes;
 #pragma unroll
       for (int e = 0; e < kMax; ++e) {
-        const float off = mx[e] == -inf ? 0.0f : kLift - mx[e];
-        s[e][0] = ex2(s[e][0] + off);
-        s[e][1] = ex2(s[e][1] + off);
+        s[e][0] = ex2(s[e][0]);
+        s[e][1] = ex2(s[e][1]);
         sum[e] += s[e][0] + s[e][1];
       }
 #pragma unroll
@@ -808,7 +837,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           for (int o = 4; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
           if (g8 == 0) {
             m.red[1][quad][row_of(e)] = t;
-            if (quad == 0) m.top[row_of(e)] = mx[e];
+            if (quad == 0) m.top[row_of(e)] = live >> e & 1 ? kLift - off[e] : -inf;
           }
         }
         ok = product_done(n);
