@@ -48,7 +48,7 @@ __device__ void kv_attend_row(const KvAttnArgs& a, int r, int t, int h, KvRowSme
   const int kvh = h / a.group;
   const int2 tq = kv_queries(a, r);
   const int p = max(a.kv_lens[r], 0) - tq.y + (t - tq.x);
-  const int n = kv_rows_of(a, r);
+  const int n = kv_clip(a, a.kv_lens[r]);
   if (tid == 0 && n != a.kv_lens[r]) flag(a.status, WH_DEV_BADARG);
   const KvSpan sp = kv_span(a, p, p, n);
   const int seen = sp.head + sp.end - sp.start;
@@ -164,81 +164,103 @@ __global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(KvAttnArgs a
 
 // ---------------------------------------------------------------------------
 // Joins the tensor-core kernel's partial sums of items that lie in several CTAs
-// (one query row and 128 columns a CTA; a row in one piece leaves at once), and
-// computes rows again that the f16 tiles cannot hold.  The parts are added in
-// the order of the rows they cover.
+// and computes rows again that its f16 tiles cannot hold.  kWpr warps share a
+// row's parts (added in the order of the rows they cover within a warp, then
+// over the warps), a lane has kV groups of 4 columns.  Many rows: a warp each,
+// all columns; few rows (long contexts, many parts): a CTA each and 128 columns.
+// Bound by the latency of four dependent loads (row, parts' maxima, sums, store).
 // ---------------------------------------------------------------------------
-template <class T>
+template <class T, int kV, int kWpr>
 __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWork w) {
   __shared__ KvRowSmem sm;
-  pdl_wait_prior();
-  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-  const int first = a.cu_q ? max(a.cu_q[0], 0) : 0;
-  const int past = a.cu_q ? a.cu_q[a.requests] : a.requests;
-  if (t < first || t >= past) return;
-  const int4 mt = w.meta[blockIdx.x];
-  const int parts = mt.y, row = mt.z >> 1;
-  if (mt.x < 0 || parts < 1 || mt.x + parts > w.ctas || row < 0 || row >= w.rn) {
-    flag(a.status, WH_DEV_BADARG);  // the tensor-core kernel gave up on a wait
-    return;
-  }
+  __shared__ int redo_row[4];
+  constexpr int kRows = kRowThreads / 32 / kWpr;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = warp % kWpr;
+  const long long id = (long long)blockIdx.x * kRows + warp / kWpr;
+  const int t = int(id / a.heads), h = int(id % a.heads);
+  pdl_wait_prior();
+  const int first = a.cu_q ? max(a.cu_q[0], 0) : 0;
+  const int past = min(a.cu_q ? a.cu_q[a.requests] : a.requests, a.tokens);
+  const bool mine = t >= first && t < past;
+  const int4 mt = mine ? w.meta[id] : make_int4(0, 1, 0, 0);
+  const int parts = mt.y, row = mt.z >> 1;
+  // a meta that the tensor-core kernel did not write: it gave up on a wait
+  const bool bad = mt.x < 0 || parts < 1 || mt.x + parts > w.ctas || row < 0 || row >= w.rn;
+  if (bad) flag(a.status, WH_DEV_BADARG);
   auto slot_of = [&](int p) { return 2 * (mt.x + p) + (p == 0 ? mt.z & 1 : 0); };
   const float inf = __int_as_float(0x7f800000);
-  int redo = mt.w;
-  float top = -inf;
-  if (parts > 1)
+  int redo = bad ? 0 : mt.w;
+  const bool join = !bad && parts > 1;
+  float top = -inf, base = 0.0f, z = 0.0f;
+  if (join) {
     for (int p = lane; p < parts; p += 32) {
       redo |= w.part_redo[slot_of(p)];
       top = fmaxf(top, w.part_ml[(long long)slot_of(p) * w.rn + row].x);
     }
-  redo = __any_sync(0xffffffffu, redo);
-  if (redo) {
-    const int r = kv_request_of(a, t);
-    if (blockIdx.y == 0 && r >= 0) kv_attend_row<T>(a, r, t, h, sm);
-    return;
-  }
-  if (parts == 1) return;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float sk = a.sink ? a.sink[h] * kLog2e : -inf;
-  const float to = fmaxf(top, sk), base = to == -inf ? 0.0f : to;
-  float z = 0.0f;
-  for (int p = lane; p < parts; p += 32) {
-    const float2 ml = w.part_ml[(long long)slot_of(p) * w.rn + row];
-    z += ml.x == -inf ? 0.0f : ml.y * exp2f(ml.x - base);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    redo = __any_sync(0xffffffffu, redo);
   }
+  float4 acc[kV];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-  if (a.sink) z += exp2f(sk - base + kLift);
+  for (int v = 0; v < kV; ++v) acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const int D = a.c.head_dim, dim = blockIdx.y * 128 + lane * 4;
-  float acc[4] = {0, 0, 0, 0};
-  if (dim < D) {
-#pragma unroll 4
-    for (int p = warp; p < parts; p += kRowThreads / 32) {
-      const long long at = (long long)slot_of(p) * w.rn + row;
-      const float m = w.part_ml[at].x;
-      const float f = m == -inf ? 0.0f : exp2f(m - base);
-      const float4 o = *reinterpret_cast<const float4*>(w.part_o + at * D + dim);
-      acc[0] = fmaf(f, o.x, acc[0]);
-      acc[1] = fmaf(f, o.y, acc[1]);
-      acc[2] = fmaf(f, o.z, acc[2]);
-      acc[3] = fmaf(f, o.w, acc[3]);
+  if (join && !redo) {
+    const float sk = a.sink ? a.sink[h] * kLog2e : -inf;
+    const float to = fmaxf(top, sk);
+    base = to == -inf ? 0.0f : to;
+    for (int p = lane; p < parts; p += 32) {
+      const float2 ml = w.part_ml[(long long)slot_of(p) * w.rn + row];
+      z += ml.x == -inf ? 0.0f : ml.y * exp2f(ml.x - base);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if (a.sink) z += exp2f(sk - base + kLift);
+    if (dim < D) {
+#pragma unroll(kV == 1 ? 8 : 8 / kV)
+      for (int p = sub; p < parts; p += kWpr) {
+        const long long at = (long long)slot_of(p) * w.rn + row;
+        const float m = w.part_ml[at].x;
+        const float f = m == -inf ? 0.0f : exp2f(m - base);
+#pragma unroll
+        for (int v = 0; v < kV; ++v) {
+          const float4 o = *reinterpret_cast<const float4*>(w.part_o + at * D + dim + v * 128);
+          acc[v].x = fmaf(f, o.x, acc[v].x);
+          acc[v].y = fmaf(f, o.y, acc[v].y);
+          acc[v].z = fmaf(f, o.z, acc[v].z);
+          acc[v].w = fmaf(f, o.w, acc[v].w);
+        }
+      }
     }
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sm.acc[(warp * 32 + lane) * 4 + e] = acc[e];
-  __syncthreads();
-  if (warp == 0 && dim < D) {
+  if (kWpr > 1) {
+    static_assert(kWpr == 1 || kV == 1, "one group of columns where warps share a row");
+    *reinterpret_cast<float4*>(&sm.acc[threadIdx.x * 4]) = acc[0];
+    __syncthreads();
+    acc[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = 0; k < kWpr; ++k) {
+      const float4 o = *reinterpret_cast<const float4*>(&sm.acc[(k * 32 + lane) * 4]);
+      acc[0].x += o.x;
+      acc[0].y += o.y;
+      acc[0].z += o.z;
+      acc[0].w += o.w;
+    }
+  }
+  if (join && !redo && sub == 0 && dim < D) {
     const float inv = z == 0.0f ? 0.0f : 1.0f / z;
     T* out = reinterpret_cast<T*>(a.out) + t * a.out_token_stride + h * a.out_head_stride + dim;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float v = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kRowThreads / 32; ++k) v += sm.acc[(k * 32 + lane) * 4 + e];
-      out[e] = T(v * inv);
-    }
+    for (int v = 0; v < kV; ++v) kv_store4(out + v * 128, acc[v], inv);
+  }
+  // rows to be computed again, one after the other by the whole CTA
+  if (lane == 0 && sub == 0) redo_row[warp / kWpr] = redo && mine && blockIdx.y == 0;
+  __syncthreads();
+  for (int k = 0; k < kRows; ++k) {
+    if (!redo_row[k]) continue;
+    const long long i = (long long)blockIdx.x * kRows + k;
+    const int r = kv_request_of(a, int(i / a.heads));
+    if (r >= 0) kv_attend_row<T>(a, r, int(i / a.heads), int(i % a.heads), sm);
   }
 }
 
@@ -264,7 +286,8 @@ bool kv_tc_plan(const wh_ctx* c, int head_dim, int kv_heads, int heads, int dtyp
   p->w.tt = std::max(1, p->w.rn / group);
   p->w.ht = (group + p->w.rn - 1) / p->w.rn;
   p->w.ctas = c->num_sms;
-  p->w.min_tiles = head_dim == 512 ? 2 : 4;
+  p->w.lead = head_dim == 512 ? 4 : 8;
+  p->w.min_units = p->w.lead + 2;
   return true;
 }
 // Places the scratch arrays; returns their bytes.
@@ -301,8 +324,13 @@ cudaError_t kv_launch(const KvAttnArgs& a, const KvTcPlan* p, cudaStream_t s, bo
                         : d == 128 ? kv_launch_tc<128>(a, *p, s, pdl)
                                    : kv_launch_tc<64>(a, *p, s, pdl);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kv_join_kernel<T>, dim3(rows, std::max(1, d / 128)), kRowThreads, 0, s, pdl, a,
-                    p->w);
+  if (rows <= 4u * p->w.ctas)
+    return launch_pdl(kv_join_kernel<T, 1, 4>, dim3(rows, std::max(1, d / 128)), kRowThreads, 0, s,
+                      pdl, a, p->w);
+  const dim3 grid((rows + 3) / 4);
+  return d == 512   ? launch_pdl(kv_join_kernel<T, 4, 1>, grid, kRowThreads, 0, s, pdl, a, p->w)
+         : d == 256 ? launch_pdl(kv_join_kernel<T, 2, 1>, grid, kRowThreads, 0, s, pdl, a, p->w)
+                    : launch_pdl(kv_join_kernel<T, 1, 1>, grid, kRowThreads, 0, s, pdl, a, p->w);
 }
 
 }  // namespace

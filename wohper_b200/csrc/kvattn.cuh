@@ -41,9 +41,9 @@ __device__ __forceinline__ int kv_request_of(const KvAttnArgs& a, int t) {
   }
   return lo;
 }
-// Rows of the request, clipped to what its block table can hold.
-__device__ __forceinline__ int kv_rows_of(const KvAttnArgs& a, int r) {
-  return min(max(a.kv_lens[r], 0), a.max_blocks * a.c.page);
+// A request's rows, clipped to what its block table can hold.
+__device__ __forceinline__ int kv_clip(const KvAttnArgs& a, int len) {
+  return min(max(len, 0), a.max_blocks * a.c.page);
 }
 // What the queries at positions p0 .. p1 see of n rows, taken together:
 // [0, head) and [start, end).
@@ -63,19 +63,21 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ---------------------------------------------------------------------------
 // The tensor-core kernel's work list.  An item is the query rows of `tt` tokens
 // of a request (or a part of one token's heads) that share a kv head; its rows
-// of the cache, in order of position, are cut into tiles of kKvTile.  The tiles
-// of all items, in the order request, tokens, kv head, head part, form one
-// sequence that the CTAs share evenly; an item that lies in several CTAs is
-// joined afterwards from their partial sums.
+// of the cache, in order of position, are cut into tiles of kKvTile.  The items,
+// in the order request, tokens, kv head, head part, lie on one line, each
+// w.lead units (what starting and ending an item costs, in tiles) and then one
+// unit a tile; the CTAs share the line evenly.  An item that lies in several
+// CTAs is joined afterwards from their partial sums.
 // ---------------------------------------------------------------------------
 constexpr int kKvTile = 64;
 
 struct KvWork {
-  int rn;  // query rows an item has room for
-  int tt;  // tokens of an item
-  int ht;  // items that one token's heads of one kv head take
-  int ctas, min_tiles;
-  int4* meta;       // [tokens][heads]: first CTA, CTAs, its slot, redo
+  int rn;    // query rows an item has room for
+  int tt;    // tokens of an item
+  int ht;    // items that one token's heads of one kv head take
+  int lead;  // units ahead of an item's tiles
+  int ctas, min_units;
+  int4* meta;       // [tokens][heads]: first CTA, CTAs, its slot and row, redo
   float* part_o;    // [2 * ctas][rn][head_dim]
   float2* part_ml;  // [2 * ctas][rn]: maximum (base 2), sum
   int* part_redo;   // [2 * ctas]
@@ -87,37 +89,46 @@ struct KvItem {
   int head, start, seen;  // rows [0, head) and [start, start + seen - head)
   int tiles;
 };
-__device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, const KvWork& w, int r, int2 tq,
+__device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, const KvWork& w, int len, int2 tq,
                                           int i) {
   KvItem it;
   it.t0 = tq.x + i * w.tt;
   it.nt = min(w.tt, tq.y - i * w.tt);
-  it.p0 = max(a.kv_lens[r], 0) - tq.y + i * w.tt;
-  const KvSpan s = kv_span(a, it.p0, it.p0 + it.nt - 1, kv_rows_of(a, r));
+  it.p0 = max(len, 0) - tq.y + i * w.tt;
+  const KvSpan s = kv_span(a, it.p0, it.p0 + it.nt - 1, kv_clip(a, len));
   it.head = s.head;
   it.start = s.start;
   it.seen = s.head + s.end - s.start;
   it.tiles = max(1, (it.seen + kKvTile - 1) / kKvTile);
   return it;
 }
-// Tiles of request r over all its items.
-__device__ __forceinline__ long long kv_request_tiles(const KvAttnArgs& a, const KvWork& w, int r) {
-  const int2 tq = kv_queries(a, r);
-  long long n = 0;
-  for (int i = 0; i * w.tt < tq.y; ++i) n += kv_item(a, w, r, tq, i).tiles;
-  return n * a.c.kv_heads * w.ht;
-}
-// CTAs that the sequence of `total` tiles is shared by, and the first tile of CTA i.
-__device__ __forceinline__ int kv_ctas(const KvWork& w, long long total) {
-  const long long n = (total + w.min_tiles - 1) / w.min_tiles;
-  return n < w.ctas ? (int)n : w.ctas;
-}
-__device__ __forceinline__ long long kv_cta_start(long long total, int ctas, int i) {
-  return total * i / ctas;
-}
-// The CTA that holds tile g: the last i with total * i / ctas <= g.
-__device__ __forceinline__ int kv_cta_of(long long total, int ctas, long long g) {
-  return (int)(((g + 1) * ctas - 1) / total);
-}
+// The line, cut into ctas parts: CTA i has [start(i), start(i + 1)).  In 32 bits
+// where it fits (a 64-bit division is some hundred cycles).
+struct KvCut {
+  long long total;
+  int ctas;
+  long long each;  // units of a CTA; the first `more` have one more
+  int more;
+  __device__ __forceinline__ KvCut(const KvWork& w, long long units) : total(units) {
+    if (units <= 0x7fffffffLL) {
+      const int u = (int)units;
+      ctas = min(w.ctas, u / w.min_units + (u % w.min_units != 0));
+      each = u / max(ctas, 1);
+      more = u - (int)each * ctas;
+    } else {
+      ctas = w.ctas;
+      each = units / ctas;
+      more = (int)(units - each * ctas);
+    }
+  }
+  __device__ __forceinline__ long long start(int i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int cta_of(long long x) const {
+    const long long big = (each + 1) * more;
+    const bool in = x < big;
+    const long long y = in ? x : x - big, d = in ? each + 1 : each;
+    const int q = total <= 0x7fffffffLL ? (int)y / (int)d : (int)(y / d);
+    return in ? q : more + q;
+  }
+};
 
 }  // namespace wh

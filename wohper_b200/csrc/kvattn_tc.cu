@@ -59,8 +59,8 @@ enum : int {
 
 struct KvTileInfo {
   int2 row[kKvTile];  // block (-1: not seen) and row in the block
-  long long end;      // the tile after the item's last one
-  int r, t0, nt, p0, kvh, ht, head, start, u0, flags;
+  long long first;    // where the item's tiles begin on the line
+  int tiles, r, t0, nt, p0, kvh, ht, head, start, u0, flags;
 };
 
 template <int kD, bool kSplit>
@@ -100,10 +100,12 @@ struct KvTc {
     uint64_t k_full[kTcRing], k_empty[kTcRing], v_full[kTcRing], v_empty[kTcRing];
     uint64_t s_full[2], p_full[2], p_empty[2];
     uint64_t q_full[kTcFrag], q_empty, o_empty, all_done;
-    long long part[32];
-    KvItem item;               // the item of the CTA's first tile
+    long long part[2][32];
+    long long total, begin, end;  // units of the line, the CTA's piece of it
+    long long first_tile, last_tile;
+    KvItem item;               // the item at the piece's start, and where in it
     int2 tq;
-    int r, i, kvh, ht, j;
+    int r, len, i, kvh, ht, j, into;
     uint32_t tmem;
   };
 };
@@ -249,82 +251,152 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
   }
   pdl_wait_prior();
 
-  // ---- where this CTA's tiles begin: a scan of the requests' tile counts ----
-  long long total, begin = 0, end = 0;
+  // ---- this CTA's piece of the line: a scan of the requests' units and tiles ----
   {
     constexpr int kWarps = kTcThreads / 32;
-    // inclusive sums of x over the CTA's threads; all: the sum of all
-    auto scan = [&](long long x, long long* all) {
+    // a request's length and tokens, its units and tiles
+    struct Req {
+      int len;
+      int2 tq;
+      long long units, tiles;
+    };
+    auto request = [&](int r) {
+      Req q{0, make_int2(0, 0), 0, 0};
+      if (r >= a.requests) return q;
+      q.len = a.kv_lens[r];
+      q.tq = kv_queries(a, r);
+      int items = 0;
+      for (int i = 0; i * w.tt < q.tq.y; ++i, ++items) q.tiles += kv_item(a, w, q.len, q.tq, i).tiles;
+      q.units = (q.tiles + (long long)items * w.lead) * (a.c.kv_heads * w.ht);
+      q.tiles *= a.c.kv_heads * w.ht;
+      if (q.tq.y > 0 && kv_clip(a, q.len) != q.len) flag(a.status, WH_DEV_BADARG);
+      return q;
+    };
+    // x becomes the inclusive sums over the CTA's threads; returns the sum of all
+    auto scan = [&](long long (&x)[2], long long (&all)[2]) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long p = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += p;
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long p = __shfl_up_sync(0xffffffffu, x[k], o);
+          if (lane >= o) x[k] += p;
+        }
+        if (lane == 31) m.part[k][warp] = x[k];
       }
-      if (lane == 31) m.part[warp] = x;
       tc::fence_before_sync();
       __syncthreads();
       tc::fence_after_sync();
-      long long y = lane < kWarps ? m.part[lane] : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long p = __shfl_up_sync(0xffffffffu, y, o);
-        if (lane >= o) y += p;
+      for (int k = 0; k < 2; ++k) {
+        long long y = lane < kWarps ? m.part[k][lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long p = __shfl_up_sync(0xffffffffu, y, o);
+          if (lane >= o) y += p;
+        }
+        all[k] = __shfl_sync(0xffffffffu, y, 31);
+        const long long before = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
+        if (warp > 0) x[k] += before;
       }
-      *all = __shfl_sync(0xffffffffu, y, 31);
-      return x + (warp > 0 ? __shfl_sync(0xffffffffu, y, warp - 1) : 0);
     };
-    // the item, its kv head, head part and tile at tile `off` of request r
-    auto enter = [&](int r, long long off) {
-      const int2 tq = kv_queries(a, r);
+    // Unit x of the line is unit `off` of request r, whose tiles follow `tiles`
+    // earlier ones: the first tile at or after x, and (where) the item it is in.
+    auto find = [&](int r, const Req& q, long long off, long long tiles, bool where) {
       const int per = a.c.kv_heads * w.ht;  // items of the same tokens
       int i = 0;
-      KvItem it = kv_item(a, w, r, tq, 0);
-      while (off >= (long long)it.tiles * per) {
-        off -= (long long)it.tiles * per;
-        it = kv_item(a, w, r, tq, ++i);
+      KvItem it = kv_item(a, w, q.len, q.tq, 0);
+      while (off >= (long long)(it.tiles + w.lead) * per) {
+        off -= (long long)(it.tiles + w.lead) * per;
+        tiles += (long long)it.tiles * per;
+        it = kv_item(a, w, q.len, q.tq, ++i);
       }
-      const int u = (int)(off / it.tiles);
-      m.item = it;
-      m.tq = tq;
-      m.r = r;
-      m.i = i;
-      m.kvh = u / w.ht;
-      m.ht = u % w.ht;
-      m.j = (int)(off % it.tiles);
+      const int one = it.tiles + w.lead;
+      const int u = off <= 0x7fffffffLL ? (int)off / one : (int)(off / one);
+      const int in = (int)(off - (long long)u * one);
+      const int j = max(0, in - w.lead);
+      if (where) {
+        m.item = it;
+        m.tq = q.tq;
+        m.r = r;
+        m.len = q.len;
+        m.i = i;
+        m.kvh = u / w.ht;
+        m.ht = u % w.ht;
+        m.j = j;
+        m.into = in;
+      }
+      return tiles + (long long)u * it.tiles + j;
     };
-    long long mine = 0;
-    for (int r = tid; r < a.requests; r += kTcThreads) mine += kv_request_tiles(a, w, r);
-    long long x = scan(mine, &total);
-    const int ctas = total > 0 ? kv_ctas(w, total) : 0;
-    if ((int)blockIdx.x < ctas) {
-      begin = kv_cta_start(total, ctas, blockIdx.x);
-      end = kv_cta_start(total, ctas, blockIdx.x + 1);
-      if (a.requests <= kTcThreads) {
-        if (x - mine <= begin && begin < x) enter(tid, begin - (x - mine));
-      } else {  // several requests a thread: again, in their order
-        long long base = 0, all;
-        for (int r0 = 0; r0 < a.requests && base <= begin; r0 += kTcThreads) {
-          const int r = r0 + tid;
-          mine = r < a.requests ? kv_request_tiles(a, w, r) : 0;
+    Req q = request(tid);
+    long long x[2] = {q.units, q.tiles};
+    for (int r = tid + kTcThreads; r < a.requests; r += kTcThreads) {
+      const Req p = request(r);
+      x[0] += p.units;
+      x[1] += p.tiles;
+    }
+    long long all[2];
+    scan(x, all);
+    const KvCut cut(w, all[0]);
+    if (tid == 0) {
+      const bool in = (int)blockIdx.x < cut.ctas;
+      m.total = all[0];
+      m.begin = in ? cut.start(blockIdx.x) : 0;
+      m.end = in ? cut.start(blockIdx.x + 1) : 0;
+    }
+    if ((int)blockIdx.x < cut.ctas) {
+      const long long b = cut.start(blockIdx.x), e = cut.start(blockIdx.x + 1);
+      if (tid == 0 && e == all[0]) m.last_tile = all[1];
+      long long base[2] = {0, 0};
+      for (int r0 = 0; r0 < a.requests && base[0] <= e; r0 += kTcThreads) {
+        if (a.requests > kTcThreads) {  // several requests a thread: again, in their order
+          q = request(r0 + tid);
+          x[0] = q.units;
+          x[1] = q.tiles;
           __syncthreads();
-          x = base + scan(mine, &all);
-          if (x - mine <= begin && begin < x) enter(r, begin - (x - mine));
-          base += all;
+          scan(x, all);
+          x[0] += base[0];
+          x[1] += base[1];
+          base[0] += all[0];
+          base[1] += all[1];
+        } else {
+          base[0] = e + 1;
         }
+        const long long u0 = x[0] - q.units, t0 = x[1] - q.tiles;
+        if (u0 <= b && b < x[0]) m.first_tile = find(r0 + tid, q, b - u0, t0, true);
+        if (u0 <= e && e < x[0]) m.last_tile = find(r0 + tid, q, e - u0, t0, false);
       }
     }
   }
   __syncthreads();
   const uint32_t tmem = m.tmem;
-  const int ntiles = (int)(end - begin);
+  const int ntiles = m.end > m.begin ? (int)(m.last_tile - m.first_tile) : 0;
 
   if (warp == kTcAddr) {
     // ---------------- addresses ----------------
     if (ntiles > 0) {
-      int r = m.r, i = m.i, kvh = m.kvh, ht = m.ht, j = m.j;
+      int r = m.r, len = m.len, i = m.i, kvh = m.kvh, ht = m.ht, j = m.j;
       int2 tq = m.tq;
       KvItem it = m.item;
-      if (lane == 0 && kv_rows_of(a, r) != a.kv_lens[r]) flag(a.status, WH_DEV_BADARG);
+      long long at = m.begin - m.into;  // where the item begins
+      // the item after this one
+      auto next_item = [&]() {
+        at += it.tiles + w.lead;
+        j = 0;
+        if (++ht < w.ht) return;
+        ht = 0;
+        if (++kvh < a.c.kv_heads) return;
+        kvh = 0;
+        ++i;
+        if (i * w.tt >= tq.y) {
+          i = 0;
+          do {
+            ++r;
+            tq = kv_queries(a, r);
+          } while (tq.y == 0);
+          len = a.kv_lens[r];
+        }
+        it = kv_item(a, w, len, tq, i);
+      };
       bool frag_first = true;
       int slot1 = 0;
       int key[2], blk[2];
@@ -343,29 +415,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         if (n >= kTcInfo && !warp_wait(&m.info_empty[slot], ((n / kTcInfo) - 1) & 1, a.status)) break;
         // this tile's rows; the next tile's look-up starts before they are written down
         const int r_ = r, j_ = j, kvh_ = kvh, ht_ = ht;
+        const long long at_ = at + w.lead;  // its tiles
         const KvItem x = it;
         const int ck[2] = {key[0], key[1]}, cb[2] = {blk[0], blk[1]};
         const bool frag_last = j + 1 == it.tiles || n + 1 == ntiles;
         if (n + 1 < ntiles) {
-          if (++j == it.tiles) {
-            j = 0;
-            if (++ht == w.ht) {
-              ht = 0;
-              if (++kvh == a.c.kv_heads) {
-                kvh = 0;
-                ++i;
-                if (i * w.tt >= tq.y) {
-                  i = 0;
-                  do {
-                    ++r;
-                    tq = kv_queries(a, r);
-                  } while (tq.y == 0);
-                  if (lane == 0 && kv_rows_of(a, r) != a.kv_lens[r]) flag(a.status, WH_DEV_BADARG);
-                }
-                it = kv_item(a, w, r, tq, i);
-              }
-            }
-          }
+          if (++j == it.tiles) next_item();
           look_up(r, it, j);
         }
         KvTileInfo& f = m.info[slot];
@@ -386,9 +441,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         }
         all = __all_sync(0xffffffffu, all);
         if (lane == 0) {
-          const long long g = begin + n;
-          const long long past = g + (x.tiles - j_);
-          f.end = past;
+          f.first = at_;
+          f.tiles = x.tiles;
           f.r = r_;
           f.t0 = x.t0;
           f.nt = x.nt;
@@ -399,8 +453,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           f.start = x.start;
           f.u0 = j_ * kKvTile;
           f.flags = (frag_first ? kFragFirst : 0) | (frag_last ? kFragLast : 0) |
-                    (all ? 0 : kTileMasked) | (g - j_ >= begin ? kItemFirst : 0) |
-                    (past <= end ? kItemLast : 0) | slot1;
+                    (all ? 0 : kTileMasked) | (at_ >= m.begin ? kItemFirst : 0) |
+                    (at_ + x.tiles <= m.end ? kItemLast : 0) | slot1;
         }
         frag_first = frag_last;
         if (frag_last) slot1 = kSlot1;
@@ -531,13 +585,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       return true;
     };
     // The item's queries as f16 rows; warp dw takes rows dw, dw + 16, ...
-    auto load_q = [&](const KvTileInfo& f, int frag) {
+    auto load_q = [&](int t0, int nt, int kvh, int ht, int frag) {
       constexpr int kG = kD / (kSplit ? 4 : 8);     // 16-byte groups of a row
       constexpr int kLoads = kG > 32 ? kG / 32 : 1;  // of them a lane takes
       constexpr int kRows = kRn / kTcDec;
       constexpr int kElems = kSplit ? 4 : 8;
       constexpr int kBatch = kLoads >= 4 ? 1 : kRows < 4 / kLoads ? kRows : 4 / kLoads;
-      const int rows = w.ht > 1 ? min(kRn, a.group - f.ht * kRn) : f.nt * a.group;
+      const int rows = w.ht > 1 ? min(kRn, a.group - ht * kRn) : nt * a.group;
       const uint8_t* q = static_cast<const uint8_t*>(a.q);
 #pragma unroll 1
       for (int b0 = 0; b0 < kRows; b0 += kBatch) {
@@ -546,8 +600,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       for (int b = 0; b < kBatch; ++b) {
         const int row = dw + kTcDec * (b0 + b);
         const bool real = row < rows;
-        const long long off = real ? (f.t0 + m.row_tok[row]) * a.q_token_stride +
-                                         (f.kvh * a.group + f.ht * kRn + m.row_head[row]) * a.q_head_stride
+        const long long off = real ? (t0 + m.row_tok[row]) * a.q_token_stride +
+                                         (kvh * a.group + ht * kRn + m.row_head[row]) * a.q_head_stride
                                    : 0;
 #pragma unroll
         for (int g = 0; g < kLoads; ++g) {
@@ -618,12 +672,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       }
     };
     int frag = -1;
-    auto begin_item = [&](const KvTileInfo& f) {
+    auto begin_item = [&](int t0, int nt, int kvh, int ht) {
       ++frag;
       if (frag > 0 && !warp_wait(&m.q_empty, (frag - 1) & 1, a.status)) return false;
       // the mark four fragments on is the one four fragments back, whose rows are out
       if (dw == 0 && lane == 0) m.redo[(frag + 4) % kTcRedo] = 0;
-      load_q(f, frag);
+      load_q(t0, nt, kvh, ht, frag);
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.q_full[frag % kTcFrag]);
@@ -632,7 +686,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
     auto step = [&](int n, const Raw& x) {
       const int slot = n % kTcInfo, st = n % kStages;
       const KvTileInfo& f = m.info[slot];
-      if (n > 0 && (f.flags & kFragFirst) && !begin_item(f)) return false;
+      if (n > 0 && (f.flags & kFragFirst) && !begin_item(f.t0, f.nt, f.kvh, f.ht)) return false;
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.info_empty[slot]);
       bool in = true;
@@ -661,10 +715,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       return true;
     };
     Raw raw[kAhead];
-    // the first tile's codes travel while the queries are brought in
-    bool ok = ntiles == 0 || (load(0, raw[0]) && begin_item(m.info[0]));
+    // the first item's queries while the first rows are looked up
+    bool ok = true;
+    if (ntiles > 0) ok = begin_item(m.item.t0, m.item.nt, m.kvh, m.ht);
 #pragma unroll
-    for (int u = 1; u < kAhead; ++u)
+    for (int u = 0; u < kAhead; ++u)
       if (ok && u < ntiles) ok = load(u, raw[u]);
     for (int n0 = 0; ok && n0 < ntiles; n0 += kAhead) {
 #pragma unroll
@@ -874,7 +929,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           m.out_scale[row] = os;
           if (flags & kItemFirst) {  // where the item's parts lie
             const int parts =
-                whole ? 1 : kv_cta_of(total, kv_ctas(w, total), f.end - 1) - (int)blockIdx.x + 1;
+                whole ? 1 : KvCut(w, m.total).cta_of(f.first + f.tiles - 1) - (int)blockIdx.x + 1;
             w.meta[(long long)t * a.heads + h] =
                 make_int4(blockIdx.x, parts, (flags & kSlot1 ? 1 : 0) | row << 1, redo);
           }

@@ -94,5 +94,21 @@ __device__ __forceinline__ void kv_store8(__half* p, const float (&v)[8]) {
   for (int j = 0; j < 4; ++j) o.h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
   *reinterpret_cast<uint4*>(p) = o.u;
 }
+// 4 consecutive elements of x * by, aligned to their size
+__device__ __forceinline__ void kv_store4(float* p, const float4& x, float by) {
+  *reinterpret_cast<float4*>(p) = make_float4(x.x * by, x.y * by, x.z * by, x.w * by);
+}
+__device__ __forceinline__ void kv_store4(__nv_bfloat16* p, const float4& x, float by) {
+  union { uint2 u; __nv_bfloat162 h[2]; } o;
+  o.h[0] = __floats2bfloat162_rn(x.x * by, x.y * by);
+  o.h[1] = __floats2bfloat162_rn(x.z * by, x.w * by);
+  *reinterpret_cast<uint2*>(p) = o.u;
+}
+__device__ __forceinline__ void kv_store4(__half* p, const float4& x, float by) {
+  union { uint2 u; __half2 h[2]; } o;
+  o.h[0] = __floats2half2_rn(x.x * by, x.y * by);
+  o.h[1] = __floats2half2_rn(x.z * by, x.w * by);
+  *reinterpret_cast<uint2*>(p) = o.u;
+}
 
 }  // namespace wh
