@@ -800,5 +800,17 @@ class MoeLayer:
             pass
 
 
-from .kvcache import (KvPlan, PagedKvCache, kv_append, kv_attention, kv_gather,  # noqa: E402,F401
-                      kv_plan)
+# --------------------------------------------------------------------------
+# Paged 4-bit key/value cache (wohper_b200/kvcache.py), imported with torch on
+# first use
+# --------------------------------------------------------------------------
+_KV_NAMES = ("KvPlan", "PagedKvCache", "kv_plan", "kv_append", "kv_gather", "kv_attention")
+
+
+def __getattr__(name: str):
+    if name in _KV_NAMES:
+        from . import kvcache
+
+        globals().update({n: getattr(kvcache, n) for n in _KV_NAMES})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -12,13 +12,25 @@ per 32.  The reference engine keeps f32 rows and has no counterpart.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from dataclasses import dataclass
 from typing import Optional
 
-from . import Context, WohperError, _check, _ptr, _stream, lib
+import torch
+
+from . import Context, WohperError, _check, _ptr, lib
 
 _INVALID_SHAPE, _INVALID_POINTER, _UNSUPPORTED = 2, 9, 10
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _current_stream(index: int) -> int:
+    return int(torch.cuda.current_stream(index).cuda_stream)
+
+
+# torch's own short cut to the same handle, where this torch has it
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
 class KvCacheSpec(C.Structure):
@@ -29,33 +41,41 @@ class KvCacheSpec(C.Structure):
                 ("block_stride", C.c_longlong), ("scale_block_stride", C.c_longlong)]
 
 
-def _need(ok: bool, status: int, why: str) -> None:
-    if not ok:
-        raise WohperError(status, why)
+def _fail(status: int, why: str):
+    raise WohperError(status, why)
 
 
 def _dtype_code(dtype) -> int:
-    import torch
+    code = _DTYPES.get(dtype)
+    if code is None:
+        _fail(_UNSUPPORTED, f"dtype {dtype}: float32, bfloat16 or float16")
+    return code
 
-    codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    _need(dtype in codes, _UNSUPPORTED, f"dtype {dtype}: float32, bfloat16 or float16")
-    return codes[dtype]
+
+def _dense(t, dtype, n, device, what: str) -> None:
+    """Raises unless t is a dense tensor of n elements of `dtype` on `device`."""
+    if t.dtype is dtype and t.numel() == n and t.is_contiguous() and t.device == device:
+        return
+    if t.dtype is not dtype:
+        _fail(_UNSUPPORTED, f"{what}: {t.dtype}, not {dtype}")
+    if t.device != device:
+        _fail(_INVALID_POINTER, f"{what}: on {t.device}, not {device}")
+    _fail(_INVALID_SHAPE, f"{what}: {n} dense elements")
 
 
-def _ints(t, dtype, n, device, what: str) -> None:
-    """A dense CUDA tensor of n elements of `dtype` on `device`."""
-    _need(t.dtype == dtype, _UNSUPPORTED, f"{what}: {t.dtype}, not {dtype}")
-    _need(t.numel() == n and t.is_contiguous(), _INVALID_SHAPE, f"{what}: {n} dense elements")
-    _need(t.device == device, _INVALID_POINTER, f"{what}: on {t.device}, not {device}")
+def _handle(stream, device) -> int:
+    """The cudaStream_t of stream, or of the current stream (in one call of torch's)."""
+    if stream is not None:
+        return int(stream.cuda_stream)
+    return _current_stream(device.index)
 
 
 def _on(stream):
     """Allocations inside belong to the stream that the call runs on."""
-    import contextlib
+    return _HERE if stream is None else torch.cuda.stream(stream)
 
-    import torch
 
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+_HERE = contextlib.nullcontext()
 
 
 @dataclass
@@ -71,43 +91,45 @@ class PagedKvCache:
     value_scales: Optional[object] = None
 
     def __post_init__(self):
-        import torch
-
-        _need((self.values is None) == (self.value_scales is None), _INVALID_POINTER,
-              "values and value_scales go together")
-        _need(self.keys.dim() == 4, _INVALID_SHAPE, "keys: [blocks, kv_heads, page, head_dim / 2]")
-        b, h, p, half = self.keys.shape
-        for t, last, what in ((self.keys, half, "keys"), (self.key_scales, half // 16, "key_scales"),
-                              (self.values, half, "values"),
-                              (self.value_scales, half // 16, "value_scales")):
+        k, ks, v, vs = self.keys, self.key_scales, self.values, self.value_scales
+        if (v is None) != (vs is None):
+            _fail(_INVALID_POINTER, "values and value_scales go together")
+        if k.dim() != 4:
+            _fail(_INVALID_SHAPE, "keys: [blocks, kv_heads, page, head_dim / 2]")
+        b, h, p, half = k.shape
+        if half % 16:
+            _fail(_INVALID_SHAPE, f"keys: {tuple(k.shape)}: head_dim % 32 != 0")
+        rest, scales = (b, h, p, half), (b, h, p, half // 16)
+        for t, shape, what in ((k, rest, "keys"), (ks, scales, "key_scales"), (v, rest, "values"),
+                               (vs, scales, "value_scales")):
             if t is None:
                 continue
-            _need(t.dtype == torch.uint8, _UNSUPPORTED, f"{what}: {t.dtype}, not torch.uint8")
-            _need(half % 16 == 0 and tuple(t.shape) == (b, h, p, last), _INVALID_SHAPE,
-                  f"{what}: {tuple(t.shape)}")
-            _need(t[0].is_contiguous(), _INVALID_SHAPE, f"{what}: dense inside a block")
-            _need(t.device == self.keys.device, _INVALID_POINTER, f"{what}: on {t.device}")
-        if self.values is not None:
-            _need(self.values.stride(0) == self.keys.stride(0) and
-                  self.value_scales.stride(0) == self.key_scales.stride(0), _INVALID_SHAPE,
-                  "keys and values: one block stride")
-        # a stride means nothing where there is a single block
-        wide = b > 1
-        self._spec = KvCacheSpec(b, p, h, 2 * half, _ptr(self.keys), _ptr(self.key_scales),
-                                 _ptr(self.values), _ptr(self.value_scales),
-                                 self.keys.stride(0) if wide else 0,
-                                 self.key_scales.stride(0) if wide else 0)
+            if t.dtype is not torch.uint8:
+                _fail(_UNSUPPORTED, f"{what}: {t.dtype}, not torch.uint8")
+            if t.shape != shape:
+                _fail(_INVALID_SHAPE, f"{what}: {tuple(t.shape)}, not {shape}")
+            if not t.is_contiguous() and not t[0].is_contiguous():
+                _fail(_INVALID_SHAPE, f"{what}: dense inside a block")
+            if t.device != k.device:
+                _fail(_INVALID_POINTER, f"{what}: on {t.device}, not {k.device}")
+        step, scale_step = k.stride(0), ks.stride(0)
+        if v is not None and (v.stride(0) != step or vs.stride(0) != scale_step):
+            _fail(_INVALID_SHAPE, "keys and values: one block stride")
+        if b == 1:  # a stride means nothing where there is a single block
+            step = scale_step = 0
+        self._spec = KvCacheSpec(b, p, h, 2 * half, k.data_ptr(), ks.data_ptr(), _ptr(v), _ptr(vs),
+                                 step, scale_step)
+        self._ref = C.byref(self._spec)
 
     @classmethod
     def empty(cls, blocks: int, page: int, kv_heads: int, head_dim: int,
               separate_values: bool = False, device="cuda") -> "PagedKvCache":
         """A zeroed pool (every row reads as zeros)."""
-        import torch
-
         def z(last):
             return torch.zeros(blocks, kv_heads, page, last, dtype=torch.uint8, device=device)
 
-        _need(head_dim % 32 == 0, _INVALID_SHAPE, "head_dim % 32 != 0")
+        if head_dim % 32:
+            _fail(_INVALID_SHAPE, "head_dim % 32 != 0")
         args = [z(head_dim // 2), z(head_dim // 32)]
         if separate_values:
             args += [z(head_dim // 2), z(head_dim // 32)]
@@ -155,79 +177,102 @@ def kv_plan(ctx: Context, page: int, kv_lens, q_lens, block_table, free_blocks, 
     free_top [1]) are updated in place; tokens is the step's token count, or a
     larger fixed one (a captured graph).  A step that does not fit changes
     nothing, gives no tokens, and ctx.sync() raises DeviceArg."""
-    import torch
-
     n, dev = kv_lens.numel(), kv_lens.device
-    _ints(kv_lens, torch.int32, n, dev, "kv_lens")
-    _ints(q_lens, torch.int32, n, dev, "q_lens")
-    _need(block_table.dim() == 2 and block_table.shape[0] == n, _INVALID_SHAPE,
-          "block_table: [requests, max_blocks]")
-    _ints(block_table, torch.int32, block_table.numel(), dev, "block_table")
-    _ints(free_blocks, torch.int32, free_blocks.numel(), dev, "free_blocks")
-    _ints(free_top, torch.int32, 1, dev, "free_top")
+    i32 = torch.int32
+    _dense(kv_lens, i32, n, dev, "kv_lens")
+    _dense(q_lens, i32, n, dev, "q_lens")
+    if block_table.dim() != 2 or block_table.shape[0] != n:
+        _fail(_INVALID_SHAPE, "block_table: [requests, max_blocks]")
+    _dense(block_table, i32, block_table.numel(), dev, "block_table")
+    capacity = free_blocks.numel()
+    _dense(free_blocks, i32, capacity, dev, "free_blocks")
+    _dense(free_top, i32, 1, dev, "free_top")
     if finished is not None:
-        _need(finished.dtype in (torch.uint8, torch.bool), _UNSUPPORTED, "finished: uint8 or bool")
-        _ints(finished, finished.dtype, n, dev, "finished")
-    _need(tokens >= 0, _INVALID_SHAPE, "tokens < 0")
+        if finished.dtype is not torch.uint8 and finished.dtype is not torch.bool:
+            _fail(_UNSUPPORTED, "finished: uint8 or bool")
+        _dense(finished, finished.dtype, n, dev, "finished")
+    if tokens < 0:
+        _fail(_INVALID_SHAPE, "tokens < 0")
     with _on(stream):
-        # one allocation: lens | cu_q | top | positions | requests | scratch, then the slots
-        ints = torch.empty(3 * n + 2 + 2 * tokens, dtype=torch.int32, device=dev)
+        # lens | cu_q | top | positions | requests | scratch in one allocation, the slots in another
+        ints = kv_lens.new_empty(3 * n + 2 + 2 * tokens)
         slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    lens, cu, top, pos, who, scratch = ints.split((n, n + 1, 1, tokens, tokens, n))
-    base = ints.data_ptr()
-    at = [base + 4 * o for o in (0, n, 2 * n + 1, 2 * n + 2, 2 * n + 2 + tokens,
-                                 2 * n + 2 + 2 * tokens)]
-    _check(lib().wh_kv_plan(ctx.handle, n, page, block_table.shape[1], tokens, _ptr(kv_lens),
-                            _ptr(q_lens), _ptr(finished), _ptr(block_table), _ptr(free_blocks),
-                            free_blocks.numel(), _ptr(free_top), at[2], at[0], at[1],
-                            _ptr(slots), at[3], at[4], at[5], 4 * n, _stream(stream)))
+    lens, cu, top, pos, who, _ = ints.split_with_sizes((n, n + 1, 1, tokens, tokens, n))
+    at = ints.data_ptr()
+    cu_at = at + 4 * n
+    pos_at = cu_at + 4 * (n + 2)
+    _check(lib().wh_kv_plan(ctx.handle, n, page, block_table.shape[1], tokens, kv_lens.data_ptr(),
+                            q_lens.data_ptr(), _ptr(finished), block_table.data_ptr(),
+                            free_blocks.data_ptr(), capacity, free_top.data_ptr(),
+                            cu_at + 4 * (n + 1), at, cu_at, slots.data_ptr(), pos_at,
+                            pos_at + 4 * tokens, pos_at + 8 * tokens, 4 * n,
+                            _handle(stream, dev)))
     return KvPlan(lens, cu, slots, pos, who, top)
 
 
 def _row_strides(x, cache: PagedKvCache, rows: int, what: str):
     """Strides of [rows, kv_heads, head_dim]; a size-1 dimension's stride is free."""
-    _need(tuple(x.shape) == (rows, cache.kv_heads, cache.head_dim), _INVALID_SHAPE,
-          f"{what}: {tuple(x.shape)}, not {(rows, cache.kv_heads, cache.head_dim)}")
-    _need(x.stride(2) == 1, _INVALID_SHAPE, f"{what}: contiguous rows")
-    _need(x.device == cache.keys.device, _INVALID_POINTER, f"{what}: on {x.device}")
-    return (x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0)
+    shape = (rows, cache.kv_heads, cache.head_dim)
+    if x.shape != shape:
+        _fail(_INVALID_SHAPE, f"{what}: {tuple(x.shape)}, not {shape}")
+    a, b, c = x.stride()
+    if c != 1:
+        _fail(_INVALID_SHAPE, f"{what}: contiguous rows")
+    if x.device != cache.keys.device:
+        _fail(_INVALID_POINTER, f"{what}: on {x.device}")
+    return (a if rows > 1 else 0, b if shape[1] > 1 else 0)
 
 
 def kv_append(ctx: Context, cache: PagedKvCache, slots, keys, values=None, stream=None) -> None:
     """Quantises keys (and values) [rows, kv_heads, head_dim], f32, bf16 or f16,
     into the cache's slots (int64 [rows]; negative: skipped)."""
-    import torch
-
-    rows = slots.numel()
-    _ints(slots, torch.int64, rows, cache.keys.device, "slots")
-    _need((values is None) == (cache.values is None), _INVALID_POINTER,
-          "values exactly when the cache has values")
+    rows, dev = slots.numel(), cache.keys.device
+    _dense(slots, torch.int64, rows, dev, "slots")
+    if (values is None) != (cache.values is None):
+        _fail(_INVALID_POINTER, "values exactly when the cache has values")
     ks = _row_strides(keys, cache, rows, "keys")
     vs = (0, 0)
     if values is not None:
-        _need(values.dtype == keys.dtype, _UNSUPPORTED, "keys and values: one dtype")
+        if values.dtype is not keys.dtype:
+            _fail(_UNSUPPORTED, "keys and values: one dtype")
         vs = _row_strides(values, cache, rows, "values")
-    _check(lib().wh_kv_append(ctx.handle, C.byref(cache.spec()), _ptr(slots), rows, _ptr(keys),
-                              _ptr(values), _dtype_code(keys.dtype), *ks, *vs, _stream(stream)))
+    _check(lib().wh_kv_append(ctx.handle, cache._ref, slots.data_ptr(), rows, keys.data_ptr(),
+                              _ptr(values), _dtype_code(keys.dtype), *ks, *vs,
+                              _handle(stream, dev)))
 
 
 def kv_gather(ctx: Context, cache: PagedKvCache, slots, dtype=None, stream=None):
     """The rows of slots (int64 [rows]; negative: zeros) as values: (keys, values)
     [rows, kv_heads, head_dim] of dtype (float32 by default); values is None for
     a cache whose values are its keys."""
-    import torch
-
-    rows = slots.numel()
-    _ints(slots, torch.int64, rows, cache.keys.device, "slots")
+    rows, dev = slots.numel(), cache.keys.device
+    _dense(slots, torch.int64, rows, dev, "slots")
     dtype = torch.float32 if dtype is None else dtype
     code = _dtype_code(dtype)
     shape = (rows, cache.kv_heads, cache.head_dim)
     with _on(stream):
-        k = torch.empty(shape, dtype=dtype, device=slots.device)
-        v = None if cache.values is None else torch.empty(shape, dtype=dtype, device=slots.device)
-    _check(lib().wh_kv_gather(ctx.handle, C.byref(cache.spec()), _ptr(slots), rows, _ptr(k),
-                              _ptr(v), code, _stream(stream)))
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = None if cache.values is None else torch.empty(shape, dtype=dtype, device=dev)
+    _check(lib().wh_kv_gather(ctx.handle, cache._ref, slots.data_ptr(), rows, k.data_ptr(),
+                              _ptr(v), code, _handle(stream, dev)))
     return k, v
+
+
+_scratch_sizes: dict = {}
+
+
+def _scratch_bytes(ctx: Context, cache: PagedKvCache, tokens: int, heads: int, requests: int,
+                   code: int) -> int:
+    """wh_kv_attention_scratch_bytes, asked once for the same device and sizes."""
+    s = cache._spec
+    key = (ctx.device, s.kv_heads, s.head_dim, tokens, heads, requests, code)
+    size = _scratch_sizes.get(key)
+    if size is None:
+        if len(_scratch_sizes) >= 256:
+            _scratch_sizes.clear()
+        size = _scratch_sizes[key] = int(lib().wh_kv_attention_scratch_bytes(
+            ctx.handle, cache._ref, tokens, heads, requests, code))
+    return size
 
 
 def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_table,
@@ -239,38 +284,42 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     query sits at position kv_lens[r] - 1.  A query at p sees rows i <= p and,
     with a window, only i > p - window or i < first.  sink: f32 [heads] or None.
     scale defaults to head_dim ** -0.5.  Returns out, like q."""
-    import torch
-
     dev = cache.keys.device
-    _need(q.dim() == 3 and q.shape[2] == cache.head_dim, _INVALID_SHAPE,
-          "q: [tokens, heads, head_dim]")
+    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+        _fail(_INVALID_SHAPE, "q: [tokens, heads, head_dim]")
     code = _dtype_code(q.dtype)
     tokens, heads, d = q.shape
     n = kv_lens.numel()
-    _need(q.device == dev, _INVALID_POINTER, f"q: on {q.device}, not {dev}")
-    _ints(kv_lens, torch.int32, n, dev, "kv_lens")
+    if q.device != dev:
+        _fail(_INVALID_POINTER, f"q: on {q.device}, not {dev}")
+    _dense(kv_lens, torch.int32, n, dev, "kv_lens")
     if cu_q is not None:
-        _ints(cu_q, torch.int32, n + 1, dev, "cu_q")
-    _need(block_table.dim() == 2 and block_table.shape[0] == n, _INVALID_SHAPE,
-          "block_table: [requests, max_blocks]")
-    _ints(block_table, torch.int32, block_table.numel(), dev, "block_table")
+        _dense(cu_q, torch.int32, n + 1, dev, "cu_q")
+    if block_table.dim() != 2 or block_table.shape[0] != n:
+        _fail(_INVALID_SHAPE, "block_table: [requests, max_blocks]")
+    _dense(block_table, torch.int32, block_table.numel(), dev, "block_table")
     if sink is not None:
-        _ints(sink, torch.float32, heads, dev, "sink")
+        _dense(sink, torch.float32, heads, dev, "sink")
     with _on(stream):
         if out is None:
             out = torch.empty((tokens, heads, d), dtype=q.dtype, device=dev)
-        need = int(lib().wh_kv_attention_scratch_bytes(ctx.handle, C.byref(cache.spec()), tokens,
-                                                       heads, n, code))
         if scratch is None:
-            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev, _INVALID_SHAPE,
-          "out: like q")
-    _need(q.stride(2) == 1 and out.stride(2) == 1, _INVALID_SHAPE, "q, out: contiguous rows")
-    st = [t.stride(i) if t.shape[i] > 1 else 0 for t in (q, out) for i in (0, 1)]
-    _check(lib().wh_kv_attention(ctx.handle, C.byref(cache.spec()), _ptr(q), code, tokens, heads,
-                                 st[0], st[1], n, _ptr(cu_q), _ptr(kv_lens), _ptr(block_table),
+            scratch = torch.empty(_scratch_bytes(ctx, cache, tokens, heads, n, code),
+                                  dtype=torch.uint8, device=dev)
+    if out.shape != q.shape or out.dtype is not q.dtype or out.device != dev:
+        _fail(_INVALID_SHAPE, "out: like q")
+    q0, q1, q2 = q.stride()
+    o0, o1, o2 = out.stride()
+    if q2 != 1 or o2 != 1:
+        _fail(_INVALID_SHAPE, "q, out: contiguous rows")
+    if tokens == 1:  # a size-1 dimension's stride is free
+        q0 = o0 = 0
+    if heads == 1:
+        q1 = o1 = 0
+    _check(lib().wh_kv_attention(ctx.handle, cache._ref, q.data_ptr(), code, tokens, heads, q0, q1,
+                                 n, _ptr(cu_q), kv_lens.data_ptr(), block_table.data_ptr(),
                                  block_table.shape[1], d ** -0.5 if scale is None else scale,
-                                 window, first, _ptr(sink), _ptr(out), st[2], st[3],
-                                 _ptr(scratch), scratch.numel() * scratch.element_size(),
-                                 _stream(stream)))
+                                 window, first, _ptr(sink), out.data_ptr(), o0, o1,
+                                 scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+                                 _handle(stream, dev)))
     return out
