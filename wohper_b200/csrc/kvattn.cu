@@ -271,28 +271,48 @@ __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWo
 // ---------------------------------------------------------------------------
 namespace {
 
-// How the tensor-core kernel cuts the call's queries; false where head_dim has
-// no instance (the row kernel then takes the call).
-struct KvTcPlan {
-  bool split;  // two columns a query row
+// Which kernel takes the call and how it cuts the queries.
+//  - few: at most 16 query rows (8 of f32) to a kv head and request, rows of at
+//    most 256: decoded in registers, bound by the cache's bytes;
+//  - tc: other rows of 64, 128, 256 and 512;
+//  - otherwise one CTA a query row.
+// A call's tokens are taken as evenly spread over its requests, the one thing
+// the host knows; an item with fewer rows than it has room for is still right.
+enum class KvWay { few, tc, row };
+struct KvHow {
+  KvWay way;
+  bool split;  // f32 queries: two f16 to a value
   KvWork w;
 };
-bool kv_tc_plan(const wh_ctx* c, int head_dim, int kv_heads, int heads, int dtype, KvTcPlan* p) {
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512) return false;
-  const int group = heads / kv_heads;
-  p->split = dtype == WH_DTYPE_F32;
-  p->w = KvWork{};
-  p->w.rn = p->split ? kTcCols / 2 : kTcCols;
-  p->w.tt = std::max(1, p->w.rn / group);
-  p->w.ht = (group + p->w.rn - 1) / p->w.rn;
-  p->w.ctas = c->num_sms;
-  p->w.lead = head_dim == 512 ? 4 : 8;
-  p->w.min_units = p->w.lead + 2;
-  return true;
+KvHow kv_how(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads, int requests,
+             int dtype) {
+  KvHow p{};
+  p.way = KvWay::row;
+  const int d = head_dim, group = heads / kv_heads;
+  if (d != 64 && d != 128 && d != 256 && d != 512) return p;
+  p.split = dtype == WH_DTYPE_F32;
+  const long long each = (long long)group * ((tokens + requests - 1) / requests);
+  KvWork& w = p.w;
+  if (d <= 256 && each <= (p.split ? 8 : 16)) {
+    p.way = KvWay::few;
+    w.rn = each <= 8 ? 8 : 16;
+    w.ctas = c->num_sms * (d * w.rn <= 8 * 128 ? 2 : 1);
+    w.lead = 8;
+    w.align = kFewKeys;
+  } else {
+    p.way = KvWay::tc;
+    w.rn = p.split ? kTcCols / 2 : kTcCols;
+    w.ctas = c->num_sms;
+    w.lead = d == 512 ? 4 : 8;
+    w.align = 1;
+  }
+  w.min_units = w.lead + 2;
+  w.tt = std::max(1, w.rn / group);
+  w.ht = (group + w.rn - 1) / w.rn;
+  return p;
 }
 // Places the scratch arrays; returns their bytes.
-size_t kv_tc_scratch(KvTcPlan* p, int head_dim, int tokens, int heads, uint8_t* base) {
-  KvWork& w = p->w;
+size_t kv_scratch(KvWork& w, int head_dim, int tokens, int heads, uint8_t* base) {
   size_t at = 0;
   auto take = [&](size_t bytes) {
     uint8_t* q = base + at;
@@ -307,30 +327,40 @@ size_t kv_tc_scratch(KvTcPlan* p, int head_dim, int tokens, int heads, uint8_t* 
   return at;
 }
 template <int kD>
-cudaError_t kv_launch_tc(const KvAttnArgs& a, const KvTcPlan& p, cudaStream_t s, bool pdl) {
+cudaError_t kv_launch_tc(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool pdl) {
   if (a.c.shared)
     return p.split ? launch_attend_tc<kD, true, false>(a, p.w, s, pdl)
                    : launch_attend_tc<kD, false, false>(a, p.w, s, pdl);
   return p.split ? launch_attend_tc<kD, true, true>(a, p.w, s, pdl)
                  : launch_attend_tc<kD, false, true>(a, p.w, s, pdl);
 }
+template <int kD>
+cudaError_t kv_launch_few(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool pdl) {
+  if (p.split) return launch_attend_few<kD, 1, true>(a, p.w, s, pdl);
+  return p.w.rn == 8 ? launch_attend_few<kD, 1, false>(a, p.w, s, pdl)
+                     : launch_attend_few<kD, 2, false>(a, p.w, s, pdl);
+}
 template <class T>
-cudaError_t kv_launch(const KvAttnArgs& a, const KvTcPlan* p, cudaStream_t s, bool pdl) {
+cudaError_t kv_launch(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool pdl) {
   const unsigned rows = (unsigned)((long long)a.tokens * a.heads);
-  if (!p) return launch_pdl(kv_attend_row_kernel<T>, dim3(rows), kRowThreads, 0, s, pdl, a);
+  if (p.way == KvWay::row)
+    return launch_pdl(kv_attend_row_kernel<T>, dim3(rows), kRowThreads, 0, s, pdl, a);
   const int d = a.c.head_dim;
-  const cudaError_t e = d == 512   ? kv_launch_tc<512>(a, *p, s, pdl)
-                        : d == 256 ? kv_launch_tc<256>(a, *p, s, pdl)
-                        : d == 128 ? kv_launch_tc<128>(a, *p, s, pdl)
-                                   : kv_launch_tc<64>(a, *p, s, pdl);
+  const cudaError_t e = p.way == KvWay::few ? (d == 256   ? kv_launch_few<256>(a, p, s, pdl)
+                                               : d == 128 ? kv_launch_few<128>(a, p, s, pdl)
+                                                          : kv_launch_few<64>(a, p, s, pdl))
+                        : d == 512 ? kv_launch_tc<512>(a, p, s, pdl)
+                        : d == 256 ? kv_launch_tc<256>(a, p, s, pdl)
+                        : d == 128 ? kv_launch_tc<128>(a, p, s, pdl)
+                                   : kv_launch_tc<64>(a, p, s, pdl);
   if (e != cudaSuccess) return e;
-  if (rows <= 4u * p->w.ctas)
+  if (rows <= 4u * p.w.ctas)
     return launch_pdl(kv_join_kernel<T, 1, 4>, dim3(rows, std::max(1, d / 128)), kRowThreads, 0, s,
-                      pdl, a, p->w);
+                      pdl, a, p.w);
   const dim3 grid((rows + 3) / 4);
-  return d == 512   ? launch_pdl(kv_join_kernel<T, 4, 1>, grid, kRowThreads, 0, s, pdl, a, p->w)
-         : d == 256 ? launch_pdl(kv_join_kernel<T, 2, 1>, grid, kRowThreads, 0, s, pdl, a, p->w)
-                    : launch_pdl(kv_join_kernel<T, 1, 1>, grid, kRowThreads, 0, s, pdl, a, p->w);
+  return d == 512   ? launch_pdl(kv_join_kernel<T, 4, 1>, grid, kRowThreads, 0, s, pdl, a, p.w)
+         : d == 256 ? launch_pdl(kv_join_kernel<T, 2, 1>, grid, kRowThreads, 0, s, pdl, a, p.w)
+                    : launch_pdl(kv_join_kernel<T, 1, 1>, grid, kRowThreads, 0, s, pdl, a, p.w);
 }
 
 }  // namespace
@@ -342,10 +372,8 @@ size_t wh_kv_attention_scratch_bytes(const wh_ctx* c, const wh_kv_cache* cache, 
   if (!c || !cache || tokens < 1 || heads < 1 || requests < 1 || cache->kv_heads < 1 ||
       heads % cache->kv_heads != 0)
     return 0;
-  KvTcPlan p;
-  if (!kv_tc_plan(c, cache->head_dim, cache->kv_heads, heads, dtype, &p))
-    return 256;
-  return kv_tc_scratch(&p, cache->head_dim, tokens, heads, nullptr);
+  KvHow p = kv_how(c, cache->head_dim, cache->kv_heads, tokens, heads, requests, dtype);
+  return p.way == KvWay::row ? 256 : kv_scratch(p.w, cache->head_dim, tokens, heads, nullptr);
 }
 
 wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, int dtype,
@@ -404,15 +432,15 @@ wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, in
   // a window that holds every row the table can is none
   if (window >= (long long)max_blocks * cache->page) a.window = 0;
   const cudaStream_t s = (cudaStream_t)stream;
-  KvTcPlan p;
-  const bool tc = kv_tc_plan(c, cache->head_dim, cache->kv_heads, heads, dtype, &p);
-  if (tc) kv_tc_scratch(&p, cache->head_dim, tokens, heads, static_cast<uint8_t*>(scratch));
+  KvHow p = kv_how(c, cache->head_dim, cache->kv_heads, tokens, heads, requests, dtype);
+  if (p.way != KvWay::row)
+    kv_scratch(p.w, cache->head_dim, tokens, heads, static_cast<uint8_t*>(scratch));
   if (dtype == WH_DTYPE_F32)
-    WH_CUDA(kv_launch<float>(a, tc ? &p : nullptr, s, c->pdl()));
+    WH_CUDA(kv_launch<float>(a, p, s, c->pdl()));
   else if (dtype == WH_DTYPE_BF16)
-    WH_CUDA(kv_launch<__nv_bfloat16>(a, tc ? &p : nullptr, s, c->pdl()));
+    WH_CUDA(kv_launch<__nv_bfloat16>(a, p, s, c->pdl()));
   else
-    WH_CUDA(kv_launch<__half>(a, tc ? &p : nullptr, s, c->pdl()));
+    WH_CUDA(kv_launch<__half>(a, p, s, c->pdl()));
   return WH_OK;
 }
 

@@ -76,6 +76,7 @@ struct KvWork {
   int tt;    // tokens of an item
   int ht;    // items that one token's heads of one kv head take
   int lead;  // units ahead of an item's tiles
+  int align;  // rows that an item's list begins at multiples of (a power of two)
   int ctas, min_units;
   int4* meta;       // [tokens][heads]: first CTA, CTAs, its slot and row, redo
   float* part_o;    // [2 * ctas][rn][head_dim]
@@ -86,9 +87,14 @@ struct KvWork {
 struct KvItem {
   int t0, nt;  // its tokens
   int p0;      // position of the first
-  int head, start, seen;  // rows [0, head) and [start, start + seen - head)
+  int lo, from;           // sees rows [0, lo) and [from, ...)
+  int head, start, seen;  // its list: [0, head), [start, start + seen - head), from w.align multiples
   int tiles;
 };
+// The u-th row of an item's list.
+__device__ __forceinline__ int kv_key(int head, int start, int u) {
+  return u < head ? u : start + (u - head);
+}
 __device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, const KvWork& w, int len, int2 tq,
                                           int i) {
   KvItem it;
@@ -96,9 +102,11 @@ __device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, const KvWork& w, 
   it.nt = min(w.tt, tq.y - i * w.tt);
   it.p0 = max(len, 0) - tq.y + i * w.tt;
   const KvSpan s = kv_span(a, it.p0, it.p0 + it.nt - 1, kv_clip(a, len));
-  it.head = s.head;
-  it.start = s.start;
-  it.seen = s.head + s.end - s.start;
+  it.lo = s.head;
+  it.from = s.start;
+  it.head = (s.head + w.align - 1) & -w.align;
+  it.start = s.start & -w.align;
+  it.seen = it.head + s.end - it.start;
   it.tiles = max(1, (it.seen + kKvTile - 1) / kKvTile);
   return it;
 }
@@ -128,6 +136,162 @@ struct KvCut {
     const long long y = in ? x : x - big, d = in ? each + 1 : each;
     const int q = total <= 0x7fffffffLL ? (int)y / (int)d : (int)(y / d);
     return in ? q : more + q;
+  }
+};
+
+// A CTA's piece of the line and the item at its start (shared memory).
+struct KvPlace {
+  long long part[2][32];
+  long long total, begin, end;  // units of the line; the piece
+  long long first_tile, last_tile;
+  KvItem item;
+  int2 tq;
+  int r, len, i, kvh, ht, j, into;  // j: the first tile; into: units into the item
+  __device__ __forceinline__ int ntiles() const { return end > begin ? (int)(last_tile - first_tile) : 0; }
+};
+// Fills m; every thread of the CTA calls it.  A scan of the requests' units and
+// tiles; the thread whose request holds an end of the piece finds the place.
+template <int kThreads>
+__device__ __forceinline__ void kv_place(const KvAttnArgs& a, const KvWork& w, KvPlace& m) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kWarps = kThreads / 32;
+  // a request's length and tokens, its units and tiles
+  struct Req {
+    int len;
+    int2 tq;
+    long long units, tiles;
+  };
+  auto request = [&](int r) {
+    Req q{0, make_int2(0, 0), 0, 0};
+    if (r >= a.requests) return q;
+    q.len = a.kv_lens[r];
+    q.tq = kv_queries(a, r);
+    int items = 0;
+    for (int i = 0; i * w.tt < q.tq.y; ++i, ++items) q.tiles += kv_item(a, w, q.len, q.tq, i).tiles;
+    q.units = (q.tiles + (long long)items * w.lead) * (a.c.kv_heads * w.ht);
+    q.tiles *= a.c.kv_heads * w.ht;
+    if (q.tq.y > 0 && kv_clip(a, q.len) != q.len) flag(a.status, WH_DEV_BADARG);
+    return q;
+  };
+  // x becomes the inclusive sums over the CTA's threads; returns the sum of all
+  auto scan = [&](long long (&x)[2], long long (&all)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long p = __shfl_up_sync(0xffffffffu, x[k], o);
+        if (lane >= o) x[k] += p;
+      }
+      if (lane == 31) m.part[k][warp] = x[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      long long y = lane < kWarps ? m.part[k][lane] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long p = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += p;
+      }
+      all[k] = __shfl_sync(0xffffffffu, y, 31);
+      const long long before = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
+      if (warp > 0) x[k] += before;
+    }
+  };
+  // Unit x of the line is unit `off` of request r, whose tiles follow `tiles`
+  // earlier ones: the first tile at or after x, and (where) the item it is in.
+  auto find = [&](int r, const Req& q, long long off, long long tiles, bool where) {
+    const int per = a.c.kv_heads * w.ht;  // items of the same tokens
+    int i = 0;
+    KvItem it = kv_item(a, w, q.len, q.tq, 0);
+    while (off >= (long long)(it.tiles + w.lead) * per) {
+      off -= (long long)(it.tiles + w.lead) * per;
+      tiles += (long long)it.tiles * per;
+      it = kv_item(a, w, q.len, q.tq, ++i);
+    }
+    const int one = it.tiles + w.lead;
+    const int u = off <= 0x7fffffffLL ? (int)off / one : (int)(off / one);
+    const int in = (int)(off - (long long)u * one);
+    const int j = max(0, in - w.lead);
+    if (where) {
+      m.item = it;
+      m.tq = q.tq;
+      m.r = r;
+      m.len = q.len;
+      m.i = i;
+      m.kvh = u / w.ht;
+      m.ht = u % w.ht;
+      m.j = j;
+      m.into = in;
+    }
+    return tiles + (long long)u * it.tiles + j;
+  };
+  Req q = request(tid);
+  long long x[2] = {q.units, q.tiles};
+  for (int r = tid + kThreads; r < a.requests; r += kThreads) {
+    const Req p = request(r);
+    x[0] += p.units;
+    x[1] += p.tiles;
+  }
+  long long all[2];
+  scan(x, all);
+  const KvCut cut(w, all[0]);
+  if (tid == 0) {
+    const bool in = (int)blockIdx.x < cut.ctas;
+    m.total = all[0];
+    m.begin = in ? cut.start(blockIdx.x) : 0;
+    m.end = in ? cut.start(blockIdx.x + 1) : 0;
+  }
+  if ((int)blockIdx.x < cut.ctas) {
+    const long long b = cut.start(blockIdx.x), e = cut.start(blockIdx.x + 1);
+    if (tid == 0 && e == all[0]) m.last_tile = all[1];
+    long long base[2] = {0, 0};
+    for (int r0 = 0; r0 < a.requests && base[0] <= e; r0 += kThreads) {
+      if (a.requests > kThreads) {  // several requests a thread: again, in their order
+        q = request(r0 + tid);
+        x[0] = q.units;
+        x[1] = q.tiles;
+        __syncthreads();
+        scan(x, all);
+        x[0] += base[0];
+        x[1] += base[1];
+        base[0] += all[0];
+        base[1] += all[1];
+      } else {
+        base[0] = e + 1;
+      }
+      const long long u0 = x[0] - q.units, t0 = x[1] - q.tiles;
+      if (u0 <= b && b < x[0]) m.first_tile = find(r0 + tid, q, b - u0, t0, true);
+      if (u0 <= e && e < x[0]) m.last_tile = find(r0 + tid, q, e - u0, t0, false);
+    }
+  }
+  __syncthreads();
+}
+// Walks the items from a CTA's place on.
+struct KvWalk {
+  int r, len, i, kvh, ht, j;
+  int2 tq;
+  KvItem it;
+  long long at;  // where the item begins on the line
+  __device__ __forceinline__ explicit KvWalk(const KvPlace& p)
+      : r(p.r), len(p.len), i(p.i), kvh(p.kvh), ht(p.ht), j(p.j), tq(p.tq), it(p.item), at(p.begin - p.into) {}
+  __device__ __forceinline__ void next(const KvAttnArgs& a, const KvWork& w) {
+    at += it.tiles + w.lead;
+    j = 0;
+    if (++ht < w.ht) return;
+    ht = 0;
+    if (++kvh < a.c.kv_heads) return;
+    kvh = 0;
+    ++i;
+    if (i * w.tt >= tq.y) {
+      i = 0;
+      do {
+        ++r;
+        tq = kv_queries(a, r);
+      } while (tq.y == 0);
+      len = a.kv_lens[r];
+    }
+    it = kv_item(a, w, len, tq, i);
   }
 };
 

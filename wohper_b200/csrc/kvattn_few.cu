@@ -1,0 +1,530 @@
+// kvattn_few.cu -- attention over the paged 4-bit cache for kv heads with few
+// query rows (decoding with grouped heads).
+//
+// With at most 16 rows a cache row gives so little work that the cache's bytes
+// bound the kernel; what must not happen is that decoding them costs more than
+// reading them.  So nothing passes through shared memory: a warp takes 16 rows
+// of the cache at a time and decodes its codes in registers straight into the
+// operands of mma.m16n8k16:
+//   S [16 x 16 keys]  = Q K^T     Q is A (held), K^T is B: lane (g, t) of a key
+//                                 tile holds key g's columns [t D/4, (t+1) D/4)
+//   O^T [D x 8] += V^T P^T        V^T is A: lane (g, t) holds columns
+//                                 [g D/8, (g+1) D/8) of keys 2t, 2t+1, 2t+8, 2t+9;
+//                                 P^T is B, which is how S leaves its product
+// (the order of the columns within a product is free, so every lane's columns are
+// contiguous in memory).  A decode costs about 1.3 instructions a code, the same
+// as the rest of a step together.  Every warp keeps its own maxima, sums and O^T;
+// the CTA joins them when an item ends.
+//
+// f16 tiles, scales, query halves (kSplit: rows 8-15 of A are the low halves) and
+// rows to be computed again are as in kvattn_tc.cu.  kNt: groups of 8 query rows.
+#include "kvattn.cuh"
+
+namespace wh {
+
+constexpr int kFewWarps = 8, kFewThreads = kFewWarps * 32;
+constexpr int kFewKeys = 16;  // rows of the cache a warp takes at a time
+
+template <int kD, int kNt, bool kSplit>
+struct KvFew {
+  static_assert(!kSplit || kNt == 1, "f32 rows take both halves of A");
+  static constexpr int kRn = 8 * kNt;
+  static constexpr int kSteps = kD / 16;   // products of S along D; 16-column tiles of O^T
+  static constexpr int kA = kSplit || kNt == 2 ? 4 : 2;  // registers of A that are not zero
+  static constexpr int kKBytes = kD / 8, kVBytes = kD / 16;  // of a row's codes a lane has
+  static constexpr int kCtas = kD * kNt <= 128 ? 2 : 1;      // resident CTAs aimed at
+  struct Misc {
+    KvPlace at;
+    float top[kFewWarps][kRn], sum[kFewWarps][kRn];
+    float out_scale[kRn];
+    long long out_row[kRn];
+    int redo;
+  };
+  static constexpr int kBytes = kFewWarps * kRn * kD * 4 + (int)sizeof(Misc);
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// kBytes bytes of codes, as words
+template <int kBytes>
+struct KvWords {
+  static constexpr int n = kBytes / 4;
+  uint32_t w[n];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if (kBytes == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else if (kBytes == 8) {
+      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = x.x;
+      w[1 % n] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < n / 4; ++i) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[(4 * i) % n] = x.x;
+        w[(4 * i + 1) % n] = x.y;
+        w[(4 * i + 2) % n] = x.z;
+        w[(4 * i + 3) % n] = x.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < n; ++i) w[i] = 0;
+  }
+};
+// The scale of a byte in the ordinary range [109, 136] as f16 in both halves:
+// 2^(b - kKvBias); other bytes go through few_scale.
+__device__ __forceinline__ uint32_t few_scale_fast(uint32_t b) { return b * 0x04000400u - 108u * 0x04000400u; }
+__device__ __forceinline__ bool few_ordinary(uint32_t b) { return b - 109u <= 27u; }
+// Any byte: 0 and what f16 does not hold give 0; lost says which.
+__device__ __forceinline__ uint32_t few_scale(uint32_t b, bool& lost) {
+  const int k = int(b) - kKvBias;
+  if (b == 0) return 0;
+  if (k < -23 || k > 13) {
+    lost = true;
+    return 0;
+  }
+  return (k >= -14 ? uint32_t(k + 15) << 10 : 1u << (k + 24)) * 0x10001u;
+}
+__device__ __forceinline__ uint32_t e2m1x2_to_f16(uint32_t w, int byte) {
+  uint32_t h;
+  asm("{ .reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %1; cvt.rn.f16x2.e2m1x2 %0, a; }"
+      : "=r"(h)
+      : "r"(w >> (8 * byte)));
+  return h;
+}
+
+template <int kD, int kNt, bool kSplit>
+__global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
+    kv_attend_few_kernel(KvAttnArgs a, KvWork w) {
+  using L = KvFew<kD, kNt, kSplit>;
+  constexpr int kRn = L::kRn, kSteps = L::kSteps;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  float* merge = reinterpret_cast<float*>(smem_raw);  // [warp][row][column]
+  typename L::Misc& m = *reinterpret_cast<typename L::Misc*>(smem_raw + kFewWarps * kRn * kD * 4);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const float inf = __int_as_float(0x7f800000);
+
+  pdl_wait_prior();
+  kv_place<kFewThreads>(a, w, m.at);
+  int left = m.at.ntiles();
+  if (left == 0) return;
+  KvWalk c(m.at);
+  const long long begin = m.at.begin, end = m.at.end;
+  const KvCut cut(w, m.at.total);
+  const bool even = a.c.page % kFewKeys == 0;  // 16 rows from a multiple of 16 share a block
+  int slot1 = 0;
+
+  while (left > 0) {
+    // ---------------- a fragment: tiles [c.j, c.j + n) of the item c.it ----------------
+    const int n = min(left, c.it.tiles - c.j);
+    const KvItem it = c.it;
+    const int rows = w.ht > 1 ? min(kRn, a.group - c.ht * kRn) : it.nt * a.group;
+    const int h0 = c.kvh * a.group + c.ht * kRn;
+    auto row_tok = [&](int row) { return w.ht > 1 ? 0 : row / a.group; };
+    auto row_head = [&](int row) { return w.ht > 1 ? row : row % a.group; };
+    if (tid == 0) m.redo = 0;
+    __syncthreads();
+
+    // the queries as A: lane (g, t) holds columns [t D/4, (t+1) D/4) of row g (and g + 8)
+    uint32_t qa[kSteps][L::kA];
+    float fac[kNt];
+#pragma unroll
+    for (int u = 0; u < kNt; ++u) {
+      const int row = g + 8 * u;
+      const bool real = row < rows;
+      float v[kD / 4];
+      const long long off = real ? (it.t0 + row_tok(row)) * a.q_token_stride + (h0 + row_head(row)) * a.q_head_stride + t * (kD / 4)
+                                 : 0;
+#pragma unroll
+      for (int e = 0; e < kD / 32; ++e) {
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (real) {
+          if (kSplit)
+            kv_load8(static_cast<const float*>(a.q) + off + 8 * e, x);
+          else if (a.dtype == WH_DTYPE_BF16)
+            kv_load8(static_cast<const __nv_bfloat16*>(a.q) + off + 8 * e, x);
+          else
+            kv_load8(static_cast<const __half*>(a.q) + off + 8 * e, x);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * e + i] = x[i];
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < kD / 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool fin = top < 0x7f800000u;
+      if (!fin) m.redo = 1;
+      const int ex = max(int(top >> 23) - 127, -100);
+      const float mul = fin ? exp2i(14 - ex) : 0.0f;
+      fac[u] = a.scale * kLog2e * exp2i(max(ex - 18, -126));
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // A's registers 2k (row g) and 2k + 1 (row g + 8)
+          const float x = fin ? v[4 * s + 2 * k] * mul : 0.0f, y = fin ? v[4 * s + 2 * k + 1] * mul : 0.0f;
+          const __half2 hi = __floats2half2_rn(x, y);
+          if (L::kA == 2) {
+            qa[s][k] = half2_bits(hi);
+          } else if (kSplit) {
+            qa[s][(2 * k) % L::kA] = half2_bits(hi);
+            qa[s][(2 * k + 1) % L::kA] = half2_bits(__floats2half2_rn(x - __low2float(hi), y - __high2float(hi)));
+          } else {
+            qa[s][(2 * k + u) % L::kA] = half2_bits(hi);
+          }
+        }
+    }
+
+    float o[kSteps][kNt][4];  // tile i: columns g D/8 + 2i (0, 1) and + 2i + 1 (2, 3), rows 2t, 2t + 1
+    float off[kNt], sum[kNt];
+    bool live[kNt];
+#pragma unroll
+    for (int u = 0; u < kNt; ++u) {
+      off[u] = sum[u] = 0.0f;
+      live[u] = false;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[s][u][e] = 0.0f;
+    }
+
+    const int p1 = it.p0 + it.nt - 1;
+    const int len = kv_clip(a, c.len);
+    const int32_t* table = a.block_table + (long long)c.r * a.max_blocks;
+    // groups of 16 rows of the item's list that this warp takes
+    const int past = min((c.j + n) * (kKvTile / kFewKeys), (it.seen + kFewKeys - 1) / kFewKeys);
+    int grp = c.j * (kKvTile / kFewKeys) + warp;
+
+    // where the row that the group's key j lies in begins; false where nothing is there
+    auto locate = [&](int key0, int block0, int j, long long& co, long long& so) {
+      const int key = key0 + j;
+      int block = block0, row = j;
+      if (even) {
+        row += key0 % a.c.page;
+      } else {
+        block = key < len ? table[key / a.c.page] : -1;
+        row = key % a.c.page;
+        if (key < len && (block < 0 || block >= a.c.blocks)) flag(a.status, WH_DEV_BADARG);
+        if (block >= a.c.blocks) block = -1;
+      }
+      const long long r = (long long)c.kvh * a.c.page + row;
+      co = block * a.c.block_stride + r * (kD / 2);
+      so = block * a.c.scale_block_stride + r * (kD / 32);
+      return block >= 0;
+    };
+    auto block_of = [&](int gi) {
+      if (!even || gi >= past) return -1;
+      const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
+      int b = key0 < len ? table[key0 / a.c.page] : -1;
+      if (key0 < len && (b < 0 || b >= a.c.blocks)) {
+        flag(a.status, WH_DEV_BADARG);
+        b = -1;
+      }
+      return b;
+    };
+    KvWords<L::kKBytes> kc[2];
+    uint32_t ksb[2][kD > 128 ? 2 : 1];
+    KvWords<L::kVBytes> vc[4];
+    uint32_t vsb[4];
+    uint32_t have = 0;  // bit j: the keys' loads found a row; bit 8 + j: the values'
+    auto load_k = [&](int gi, int block) {
+      const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
+      have &= ~3u;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        long long co, so;
+        if (locate(key0, block, g + 8 * j, co, so)) {
+          have |= 1u << j;
+          kc[j].load(a.c.keys + co + t * L::kKBytes);
+#pragma unroll
+          for (int i = 0; i < (kD > 128 ? 2 : 1); ++i)
+            ksb[j][i] = __ldg(a.c.key_scales + so + (kD == 64 ? t >> 1 : kD == 128 ? t : 2 * t + i));
+        } else {
+          kc[j].zero();
+#pragma unroll
+          for (int i = 0; i < (kD > 128 ? 2 : 1); ++i) ksb[j][i] = 0;
+        }
+      }
+    };
+    auto load_v = [&](int gi, int block) {
+      const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
+      have &= 3u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        long long co, so;
+        if (locate(key0, block, 2 * t + (j & 1) + 8 * (j >> 1), co, so)) {
+          have |= 256u << j;
+          vc[j].load(a.c.values + co + g * L::kVBytes);
+          vsb[j] = __ldg(a.c.value_scales + so + (kD == 64 ? g >> 2 : kD == 128 ? g >> 1 : g));
+        } else {
+          vc[j].zero();
+          vsb[j] = 0;
+        }
+      }
+    };
+
+    int block = block_of(grp), block_next = block_of(grp + kFewWarps);
+    if (grp < past) {
+      load_k(grp, block);
+      load_v(grp, block);
+    }
+    for (; grp < past; grp += kFewWarps) {
+      const int u0 = grp * kFewKeys;
+      const int key0 = kv_key(it.head, it.start, u0);
+      // every row of the group is there and seen by every query
+      const bool full = key0 + kFewKeys - 1 <= min(it.p0, len - 1) &&
+                        (u0 < it.head ? key0 + kFewKeys <= it.lo : key0 >= it.from) &&
+                        (a.window == 0 || key0 > p1 - a.window || key0 + kFewKeys <= a.first) &&
+                        __all_sync(0xffffffffu, (have & 0xF03u) == 0xF03u);
+      // does any query see the group's key j
+      auto seen_any = [&](int j) {
+        const int key = key0 + j;
+        return key < len && key <= p1 && (u0 < it.head ? key < it.lo : key >= it.from);
+      };
+      // ---- scores ----
+      float s[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        constexpr int kB = kD > 128 ? 2 : 1;
+        uint32_t sc[kB];
+        bool plain = true;
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+          sc[i] = few_scale_fast(ksb[j][i]);
+          plain = plain && few_ordinary(ksb[j][i]);
+        }
+        if (!__all_sync(0xffffffffu, plain)) {
+          bool lost = false;
+#pragma unroll
+          for (int i = 0; i < kB; ++i) sc[i] = few_scale(ksb[j][i], lost);
+          if (lost && seen_any(g + 8 * j)) m.redo = 1;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const uint32_t word = kc[j].w[k / 2];
+          const uint32_t scale = sc[k * kB / kSteps];
+          const uint32_t b0 = hmul2_u(e2m1x2_to_f16(word, 2 * (k & 1)), scale);
+          const uint32_t b1 = hmul2_u(e2m1x2_to_f16(word, 2 * (k & 1) + 1), scale);
+          if (L::kA == 2)
+            mma_16816(s[j], qa[k][0], 0u, qa[k][1], 0u, b0, b1);
+          else
+            mma_16816(s[j], qa[k][0], qa[k][1], qa[k][2 % L::kA], qa[k][3 % L::kA], b0, b1);
+        }
+      }
+      const int next = grp + kFewWarps;
+      if (next < past) load_k(next, block_next);
+      // ---- log2 weights: x[u][j][e] of row g + 8u, key 2t + e + 8j ----
+      float x[kNt][2][2];
+#pragma unroll
+      for (int u = 0; u < kNt; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            x[u][j][e] = fmaf(kSplit ? s[j][e] + s[j][e + 2] : s[j][e + 2 * u], fac[u], off[u]);
+      if (!full) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int jj = 2 * t + e + 8 * j, key = key0 + jj;
+            const bool any = seen_any(jj) && (have >> (8 + 2 * j + e) & 1);
+#pragma unroll
+            for (int u = 0; u < kNt; ++u) {
+              const int p = it.p0 + row_tok(g + 8 * u);
+              if (!(any && key <= p && (a.window == 0 || key > p - a.window || key < a.first)))
+                x[u][j][e] = -inf;
+            }
+          }
+      }
+      // the maxima may lag, as long as no weight is past 2^(kLift + kLag)
+      float most = -inf;
+#pragma unroll
+      for (int u = 0; u < kNt; ++u)
+        most = fmaxf(most, fmaxf(fmaxf(x[u][0][0], x[u][0][1]), fmaxf(x[u][1][0], x[u][1][1])));
+      bool stay = most <= kLift + kLag;
+#pragma unroll
+      for (int u = 0; u < kNt; ++u) stay = stay && live[u];
+      if (!__all_sync(0xffffffffu, stay)) {
+#pragma unroll
+        for (int u = 0; u < kNt; ++u) {
+          float top = fmaxf(fmaxf(x[u][0][0], x[u][0][1]), fmaxf(x[u][1][0], x[u][1][1]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const bool none = top == -inf;
+          const float by = none ? 0.0f : fminf(kLift - top, live[u] ? 0.0f : inf);
+          const float sh = ex2(live[u] ? by : 0.0f);
+          live[u] = live[u] || !none;
+          off[u] += by;
+          sum[u] *= sh;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[u][j][e] += by;
+          const float sh0 = __shfl_sync(0xffffffffu, sh, 8 * t), sh1 = __shfl_sync(0xffffffffu, sh, 8 * t + 4);
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            o[i][u][0] *= sh0;
+            o[i][u][1] *= sh1;
+            o[i][u][2] *= sh0;
+            o[i][u][3] *= sh1;
+          }
+        }
+      }
+      uint32_t pb[kNt][2], pl[2] = {0, 0};
+#pragma unroll
+      for (int u = 0; u < kNt; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float p0 = ex2(x[u][j][0]), p1_ = ex2(x[u][j][1]);
+          sum[u] += p0 + p1_;
+          const __half2 h = __floats2half2_rn(p0, p1_);
+          pb[u][j] = half2_bits(h);
+          if (kSplit) pl[j] = half2_bits(__floats2half2_rn(p0 - __low2float(h), p1_ - __high2float(h)));
+        }
+      // ---- O^T ----
+      uint32_t sc[4];
+      bool plain = true;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sc[j] = few_scale_fast(vsb[j]);
+        plain = plain && few_ordinary(vsb[j]);
+      }
+      if (!__all_sync(0xffffffffu, plain)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bool lost = false;
+          sc[j] = few_scale(vsb[j], lost);
+          if (lost && seen_any(2 * t + (j & 1) + 8 * (j >> 1))) m.redo = 1;
+        }
+      }
+      const uint32_t sc01 = __byte_perm(sc[0], sc[1], 0x5410), sc23 = __byte_perm(sc[2], sc[3], 0x5410);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = e2m1x2_to_f16(vc[j].w[i / 4], i & 3);
+        const uint32_t a0 = hmul2_u(__byte_perm(h[0], h[1], 0x5410), sc01);
+        const uint32_t a1 = hmul2_u(__byte_perm(h[0], h[1], 0x7632), sc01);
+        const uint32_t a2 = hmul2_u(__byte_perm(h[2], h[3], 0x5410), sc23);
+        const uint32_t a3 = hmul2_u(__byte_perm(h[2], h[3], 0x7632), sc23);
+#pragma unroll
+        for (int u = 0; u < kNt; ++u) mma_16816(o[i][u], a0, a1, a2, a3, pb[u][0], pb[u][1]);
+        if (kSplit) mma_16816(o[i][0], a0, a1, a2, a3, pl[0], pl[1]);
+      }
+      if (next < past) load_v(next, block_next);
+      block_next = block_of(next + kFewWarps);
+    }
+
+    // ---------------- the CTA's warps joined, the rows out or to a partial slot ----------------
+#pragma unroll
+    for (int u = 0; u < kNt; ++u) {
+      sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
+      sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
+      if (t == 0) {
+        m.top[warp][g + 8 * u] = live[u] ? kLift - off[u] : -inf;
+        m.sum[warp][g + 8 * u] = sum[u];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kNt; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 2 * t + e + 8 * u;
+        float top = -inf;
+#pragma unroll
+        for (int k = 0; k < kFewWarps; ++k) top = fmaxf(top, m.top[k][row]);
+        const float mine = m.top[warp][row];
+        const float f = mine == -inf ? 0.0f : ex2(mine - top);
+        float* to = merge + (warp * kRn + row) * kD + g * (kD / 8);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+          *reinterpret_cast<float2*>(to + 2 * i) = make_float2(o[i][u][e] * f, o[i][u][e + 2] * f);
+      }
+    const bool item_first = c.at + w.lead >= begin, item_last = c.at + w.lead + it.tiles <= end;
+    const bool whole = item_first && item_last;
+    if (tid < rows) {
+      const int row = tid;
+      const int part = 2 * blockIdx.x + slot1;
+      const int h = h0 + row_head(row), tok = it.t0 + row_tok(row);
+      float top = -inf, l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kFewWarps; ++k) top = fmaxf(top, m.top[k][row]);
+#pragma unroll
+      for (int k = 0; k < kFewWarps; ++k) l += m.top[k][row] == -inf ? 0.0f : m.sum[k][row] * ex2(m.top[k][row] - top);
+      const int redo = m.redo;
+      float os = 1.0f / 16.0f;  // the f16 values are 16 times the cache's
+      if (whole) {
+        float z = l;
+        if (a.sink) {
+          const float sk = a.sink[h] * kLog2e;
+          const float to = fmaxf(top, sk), base = to == -inf ? 0.0f : to;
+          const float sh = top == -inf ? 0.0f : ex2(top - base);
+          os *= sh;
+          z = l * sh + ex2(sk - base + kLift);
+        }
+        os = z == 0.0f ? 0.0f : os / z;
+        m.out_row[row] = tok * a.out_token_stride + h * a.out_head_stride;
+      } else {
+        w.part_ml[(long long)part * kRn + row] = make_float2(top, l);
+        m.out_row[row] = ((long long)part * kRn + row) * kD;
+        if (row == 0) w.part_redo[part] = redo;
+      }
+      m.out_scale[row] = os;
+      if (item_first) {
+        const int parts = whole ? 1 : cut.cta_of(c.at + w.lead + it.tiles - 1) - (int)blockIdx.x + 1;
+        w.meta[(long long)tok * a.heads + h] = make_int4(blockIdx.x, parts, slot1 | row << 1, redo);
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * (kD / 4); i += kFewThreads) {
+      const int row = i / (kD / 4), col = i % (kD / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < kFewWarps; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(merge + (k * kRn + row) * kD + col);
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
+      }
+      const long long to = m.out_row[row] + col;
+      const float by = m.out_scale[row];
+      if (!whole)
+        kv_store4(w.part_o + to, v, by);
+      else if (kSplit)
+        kv_store4(static_cast<float*>(a.out) + to, v, by);
+      else if (a.dtype == WH_DTYPE_BF16)
+        kv_store4(static_cast<__nv_bfloat16*>(a.out) + to, v, by);
+      else
+        kv_store4(static_cast<__half*>(a.out) + to, v, by);
+    }
+    slot1 = 1;
+    left -= n;
+    if (left > 0) c.next(a, w);
+    __syncthreads();
+  }
+  pdl_launch_dependents();
+}
+
+template <int kD, int kNt, bool kSplit>
+static cudaError_t launch_attend_few(const KvAttnArgs& a, const KvWork& w, cudaStream_t s, bool pdl) {
+  using L = KvFew<kD, kNt, kSplit>;
+  const cudaError_t e = ensure_smem(kv_attend_few_kernel<kD, kNt, kSplit>, L::kBytes);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kv_attend_few_kernel<kD, kNt, kSplit>, dim3(w.ctas), kFewThreads, L::kBytes, s, pdl, a, w);
+}
+
+}  // namespace wh

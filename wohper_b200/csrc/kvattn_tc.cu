@@ -100,12 +100,7 @@ struct KvTc {
     uint64_t k_full[kTcRing], k_empty[kTcRing], v_full[kTcRing], v_empty[kTcRing];
     uint64_t s_full[2], p_full[2], p_empty[2];
     uint64_t q_full[kTcFrag], q_empty, o_empty, all_done;
-    long long part[2][32];
-    long long total, begin, end;  // units of the line, the CTA's piece of it
-    long long first_tile, last_tile;
-    KvItem item;               // the item at the piece's start, and where in it
-    int2 tq;
-    int r, len, i, kvh, ht, j, into;
+    KvPlace at;
     uint32_t tmem;
   };
 };
@@ -251,152 +246,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
   }
   pdl_wait_prior();
 
-  // ---- this CTA's piece of the line: a scan of the requests' units and tiles ----
-  {
-    constexpr int kWarps = kTcThreads / 32;
-    // a request's length and tokens, its units and tiles
-    struct Req {
-      int len;
-      int2 tq;
-      long long units, tiles;
-    };
-    auto request = [&](int r) {
-      Req q{0, make_int2(0, 0), 0, 0};
-      if (r >= a.requests) return q;
-      q.len = a.kv_lens[r];
-      q.tq = kv_queries(a, r);
-      int items = 0;
-      for (int i = 0; i * w.tt < q.tq.y; ++i, ++items) q.tiles += kv_item(a, w, q.len, q.tq, i).tiles;
-      q.units = (q.tiles + (long long)items * w.lead) * (a.c.kv_heads * w.ht);
-      q.tiles *= a.c.kv_heads * w.ht;
-      if (q.tq.y > 0 && kv_clip(a, q.len) != q.len) flag(a.status, WH_DEV_BADARG);
-      return q;
-    };
-    // x becomes the inclusive sums over the CTA's threads; returns the sum of all
-    auto scan = [&](long long (&x)[2], long long (&all)[2]) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long p = __shfl_up_sync(0xffffffffu, x[k], o);
-          if (lane >= o) x[k] += p;
-        }
-        if (lane == 31) m.part[k][warp] = x[k];
-      }
-      tc::fence_before_sync();
-      __syncthreads();
-      tc::fence_after_sync();
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        long long y = lane < kWarps ? m.part[k][lane] : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long p = __shfl_up_sync(0xffffffffu, y, o);
-          if (lane >= o) y += p;
-        }
-        all[k] = __shfl_sync(0xffffffffu, y, 31);
-        const long long before = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
-        if (warp > 0) x[k] += before;
-      }
-    };
-    // Unit x of the line is unit `off` of request r, whose tiles follow `tiles`
-    // earlier ones: the first tile at or after x, and (where) the item it is in.
-    auto find = [&](int r, const Req& q, long long off, long long tiles, bool where) {
-      const int per = a.c.kv_heads * w.ht;  // items of the same tokens
-      int i = 0;
-      KvItem it = kv_item(a, w, q.len, q.tq, 0);
-      while (off >= (long long)(it.tiles + w.lead) * per) {
-        off -= (long long)(it.tiles + w.lead) * per;
-        tiles += (long long)it.tiles * per;
-        it = kv_item(a, w, q.len, q.tq, ++i);
-      }
-      const int one = it.tiles + w.lead;
-      const int u = off <= 0x7fffffffLL ? (int)off / one : (int)(off / one);
-      const int in = (int)(off - (long long)u * one);
-      const int j = max(0, in - w.lead);
-      if (where) {
-        m.item = it;
-        m.tq = q.tq;
-        m.r = r;
-        m.len = q.len;
-        m.i = i;
-        m.kvh = u / w.ht;
-        m.ht = u % w.ht;
-        m.j = j;
-        m.into = in;
-      }
-      return tiles + (long long)u * it.tiles + j;
-    };
-    Req q = request(tid);
-    long long x[2] = {q.units, q.tiles};
-    for (int r = tid + kTcThreads; r < a.requests; r += kTcThreads) {
-      const Req p = request(r);
-      x[0] += p.units;
-      x[1] += p.tiles;
-    }
-    long long all[2];
-    scan(x, all);
-    const KvCut cut(w, all[0]);
-    if (tid == 0) {
-      const bool in = (int)blockIdx.x < cut.ctas;
-      m.total = all[0];
-      m.begin = in ? cut.start(blockIdx.x) : 0;
-      m.end = in ? cut.start(blockIdx.x + 1) : 0;
-    }
-    if ((int)blockIdx.x < cut.ctas) {
-      const long long b = cut.start(blockIdx.x), e = cut.start(blockIdx.x + 1);
-      if (tid == 0 && e == all[0]) m.last_tile = all[1];
-      long long base[2] = {0, 0};
-      for (int r0 = 0; r0 < a.requests && base[0] <= e; r0 += kTcThreads) {
-        if (a.requests > kTcThreads) {  // several requests a thread: again, in their order
-          q = request(r0 + tid);
-          x[0] = q.units;
-          x[1] = q.tiles;
-          __syncthreads();
-          scan(x, all);
-          x[0] += base[0];
-          x[1] += base[1];
-          base[0] += all[0];
-          base[1] += all[1];
-        } else {
-          base[0] = e + 1;
-        }
-        const long long u0 = x[0] - q.units, t0 = x[1] - q.tiles;
-        if (u0 <= b && b < x[0]) m.first_tile = find(r0 + tid, q, b - u0, t0, true);
-        if (u0 <= e && e < x[0]) m.last_tile = find(r0 + tid, q, e - u0, t0, false);
-      }
-    }
-  }
-  __syncthreads();
+  tc::fence_before_sync();
+  kv_place<kTcThreads>(a, w, m.at);
+  tc::fence_after_sync();
   const uint32_t tmem = m.tmem;
-  const int ntiles = m.end > m.begin ? (int)(m.last_tile - m.first_tile) : 0;
+  const int ntiles = m.at.ntiles();
 
   if (warp == kTcAddr) {
     // ---------------- addresses ----------------
     if (ntiles > 0) {
-      int r = m.r, len = m.len, i = m.i, kvh = m.kvh, ht = m.ht, j = m.j;
-      int2 tq = m.tq;
-      KvItem it = m.item;
-      long long at = m.begin - m.into;  // where the item begins
-      // the item after this one
-      auto next_item = [&]() {
-        at += it.tiles + w.lead;
-        j = 0;
-        if (++ht < w.ht) return;
-        ht = 0;
-        if (++kvh < a.c.kv_heads) return;
-        kvh = 0;
-        ++i;
-        if (i * w.tt >= tq.y) {
-          i = 0;
-          do {
-            ++r;
-            tq = kv_queries(a, r);
-          } while (tq.y == 0);
-          len = a.kv_lens[r];
-        }
-        it = kv_item(a, w, len, tq, i);
-      };
+      KvWalk c(m.at);
       bool frag_first = true;
       int slot1 = 0;
       int key[2], blk[2];
@@ -405,23 +264,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int v = jj * kKvTile + lane + 32 * k;
-          key[k] = v >= x.seen ? -1 : v < x.head ? v : x.start + (v - x.head);
+          key[k] = v >= x.seen ? -1 : kv_key(x.head, x.start, v);
           blk[k] = key[k] < 0 ? -1 : a.block_table[(long long)rr * a.max_blocks + key[k] / a.c.page];
         }
       };
-      look_up(r, it, j);
+      look_up(c.r, c.it, c.j);
       for (int n = 0; n < ntiles; ++n) {
         const int slot = n % kTcInfo;
         if (n >= kTcInfo && !warp_wait(&m.info_empty[slot], ((n / kTcInfo) - 1) & 1, a.status)) break;
         // this tile's rows; the next tile's look-up starts before they are written down
-        const int r_ = r, j_ = j, kvh_ = kvh, ht_ = ht;
-        const long long at_ = at + w.lead;  // its tiles
-        const KvItem x = it;
+        const int r_ = c.r, j_ = c.j, kvh_ = c.kvh, ht_ = c.ht;
+        const long long at_ = c.at + w.lead;  // its tiles
+        const KvItem x = c.it;
         const int ck[2] = {key[0], key[1]}, cb[2] = {blk[0], blk[1]};
-        const bool frag_last = j + 1 == it.tiles || n + 1 == ntiles;
+        const bool frag_last = c.j + 1 == c.it.tiles || n + 1 == ntiles;
         if (n + 1 < ntiles) {
-          if (++j == it.tiles) next_item();
-          look_up(r, it, j);
+          if (++c.j == c.it.tiles) c.next(a, w);
+          look_up(c.r, c.it, c.j);
         }
         KvTileInfo& f = m.info[slot];
         bool all = true;
@@ -453,8 +312,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           f.start = x.start;
           f.u0 = j_ * kKvTile;
           f.flags = (frag_first ? kFragFirst : 0) | (frag_last ? kFragLast : 0) |
-                    (all ? 0 : kTileMasked) | (at_ >= m.begin ? kItemFirst : 0) |
-                    (at_ + x.tiles <= m.end ? kItemLast : 0) | slot1;
+                    (all ? 0 : kTileMasked) | (at_ >= m.at.begin ? kItemFirst : 0) |
+                    (at_ + x.tiles <= m.at.end ? kItemLast : 0) | slot1;
         }
         frag_first = frag_last;
         if (frag_last) slot1 = kSlot1;
@@ -717,7 +576,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
     Raw raw[kAhead];
     // the first item's queries while the first rows are looked up
     bool ok = true;
-    if (ntiles > 0) ok = begin_item(m.item.t0, m.item.nt, m.kvh, m.ht);
+    if (ntiles > 0) ok = begin_item(m.at.item.t0, m.at.item.nt, m.at.kvh, m.at.ht);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (ok && u < ntiles) ok = load(u, raw[u]);
@@ -790,7 +649,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int u = f.u0 + key0 + 8 * k;
-          const int i = u < f.head ? u : f.start + (u - f.head);
+          const int i = kv_key(f.head, f.start, u);
           const bool real = f.row[key0 + 8 * k].x >= 0;
 #pragma unroll
           for (int e = 0; e < kMax; ++e) {
@@ -929,7 +788,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           m.out_scale[row] = os;
           if (flags & kItemFirst) {  // where the item's parts lie
             const int parts =
-                whole ? 1 : KvCut(w, m.total).cta_of(f.first + f.tiles - 1) - (int)blockIdx.x + 1;
+                whole ? 1 : KvCut(w, m.at.total).cta_of(f.first + f.tiles - 1) - (int)blockIdx.x + 1;
             w.meta[(long long)t * a.heads + h] =
                 make_int4(blockIdx.x, parts, (flags & kSlot1 ? 1 : 0) | row << 1, redo);
           }
