@@ -92,14 +92,6 @@ __device__ __forceinline__ uint32_t few_scale(uint32_t b, bool& lost) {
   }
   return (k >= -14 ? uint32_t(k + 15) << 10 : 1u << (k + 24)) * 0x10001u;
 }
-__device__ __forceinline__ uint32_t e2m1x2_to_f16(uint32_t w, int byte) {
-  uint32_t h;
-  asm("{ .reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %1; cvt.rn.f16x2.e2m1x2 %0, a; }"
-      : "=r"(h)
-      : "r"(w >> (8 * byte)));
-  return h;
-}
-
 template <int kD, int kNt, bool kSplit>
 __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
     kv_attend_few_kernel(KvAttnArgs a, KvWork w) {
@@ -204,70 +196,86 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
     const int past = min((c.j + n) * (kKvTile / kFewKeys), (it.seen + kFewKeys - 1) / kFewKeys);
     int grp = c.j * (kKvTile / kFewKeys) + warp;
 
-    // where the row that the group's key j lies in begins; false where nothing is there
-    auto locate = [&](int key0, int block0, int j, long long& co, long long& so) {
-      const int key = key0 + j;
-      int block = block0, row = j;
-      if (even) {
-        row += key0 % a.c.page;
-      } else {
-        block = key < len ? table[key / a.c.page] : -1;
-        row = key % a.c.page;
-        if (key < len && (block < 0 || block >= a.c.blocks)) flag(a.status, WH_DEV_BADARG);
-        if (block >= a.c.blocks) block = -1;
-      }
-      const long long r = (long long)c.kvh * a.c.page + row;
-      co = block * a.c.block_stride + r * (kD / 2);
-      so = block * a.c.scale_block_stride + r * (kD / 32);
-      return block >= 0;
-    };
+    // A group's block (even pages).  A key that is not there reads block 0 and counts as
+    // not seen.
     auto block_of = [&](int gi) {
       if (!even || gi >= past) return -1;
       const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
-      int b = key0 < len ? table[key0 / a.c.page] : -1;
+      int b = key0 < len ? table[kv_page_of(a.c, key0)] : -1;
       if (key0 < len && (b < 0 || b >= a.c.blocks)) {
         flag(a.status, WH_DEV_BADARG);
         b = -1;
       }
       return b;
     };
+    // uneven pages: block and row of one key
+    auto locate = [&](int key, long long& co, long long& so) {
+      const int pg = kv_page_of(a.c, key);
+      int b = key < len ? table[pg] : -1;
+      if (key < len && (b < 0 || b >= a.c.blocks)) {
+        flag(a.status, WH_DEV_BADARG);
+        b = -1;
+      }
+      const int row = key - pg * a.c.page;
+      co = max(b, 0) * a.c.block_stride + (long long)row * (kD / 2);
+      so = max(b, 0) * a.c.scale_block_stride + (long long)row * (kD / 32);
+      return b >= 0;
+    };
+    constexpr int kB = kD > 128 ? 2 : 1;  // scale bytes of a key that a lane needs
+    // this lane's columns in the head's first row
+    const long long head_codes = (long long)c.kvh * a.c.page * (kD / 2), head_scales = (long long)c.kvh * a.c.page * (kD / 32);
+    const uint8_t* kbase = a.c.keys + head_codes + t * L::kKBytes;
+    const uint8_t* ksbase = a.c.key_scales + head_scales + (kD == 64 ? t >> 1 : kD == 128 ? t : 2 * t);
+    const uint8_t* vbase = a.c.values + head_codes + g * L::kVBytes;
+    const uint8_t* vsbase = a.c.value_scales + head_scales + (kD == 64 ? g >> 2 : kD == 128 ? g >> 1 : g);
     KvWords<L::kKBytes> kc[2];
-    uint32_t ksb[2][kD > 128 ? 2 : 1];
+    uint32_t ksb[2][kB];
     KvWords<L::kVBytes> vc[4];
     uint32_t vsb[4];
-    uint32_t have = 0;  // bit j: the keys' loads found a row; bit 8 + j: the values'
+    uint32_t have = 0;  // bit j: key 2t + (j & 1) + 8 (j >> 1) is there
     auto load_k = [&](int gi, int block) {
       const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
-      have &= ~3u;
+      if (even) {
+        const int in = key0 - kv_page_of(a.c, key0) * a.c.page;
+        const uint8_t* kp = kbase + max(block, 0) * a.c.block_stride + (in + g) * (kD / 2);
+        const uint8_t* sp = ksbase + max(block, 0) * a.c.scale_block_stride + (in + g) * (kD / 32);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        long long co, so;
-        if (locate(key0, block, g + 8 * j, co, so)) {
-          have |= 1u << j;
-          kc[j].load(a.c.keys + co + t * L::kKBytes);
+        for (int j = 0; j < 2; ++j) {
+          kc[j].load(kp + 8 * j * (kD / 2));
 #pragma unroll
-          for (int i = 0; i < (kD > 128 ? 2 : 1); ++i)
-            ksb[j][i] = __ldg(a.c.key_scales + so + (kD == 64 ? t >> 1 : kD == 128 ? t : 2 * t + i));
-        } else {
-          kc[j].zero();
+          for (int i = 0; i < kB; ++i) ksb[j][i] = __ldg(sp + 8 * j * (kD / 32) + i);
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < (kD > 128 ? 2 : 1); ++i) ksb[j][i] = 0;
+        for (int j = 0; j < 2; ++j) {
+          long long co, so;
+          locate(key0 + g + 8 * j, co, so);
+          kc[j].load(kbase + co);
+#pragma unroll
+          for (int i = 0; i < kB; ++i) ksb[j][i] = __ldg(ksbase + so + i);
         }
       }
     };
     auto load_v = [&](int gi, int block) {
       const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
-      have &= 3u;
+      if (even) {
+        const int in = key0 - kv_page_of(a.c, key0) * a.c.page + 2 * t;
+        const uint8_t* vp = vbase + max(block, 0) * a.c.block_stride + in * (kD / 2);
+        const uint8_t* sp = vsbase + max(block, 0) * a.c.scale_block_stride + in * (kD / 32);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        long long co, so;
-        if (locate(key0, block, 2 * t + (j & 1) + 8 * (j >> 1), co, so)) {
-          have |= 256u << j;
-          vc[j].load(a.c.values + co + g * L::kVBytes);
-          vsb[j] = __ldg(a.c.value_scales + so + (kD == 64 ? g >> 2 : kD == 128 ? g >> 1 : g));
-        } else {
-          vc[j].zero();
-          vsb[j] = 0;
+        for (int j = 0; j < 4; ++j) {
+          vc[j].load(vp + ((j & 1) + 8 * (j >> 1)) * (kD / 2));
+          vsb[j] = __ldg(sp + ((j & 1) + 8 * (j >> 1)) * (kD / 32));
+        }
+        have = block >= 0 ? 15u : 0u;
+      } else {
+        have = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          long long co, so;
+          if (locate(key0 + 2 * t + (j & 1) + 8 * (j >> 1), co, so)) have |= 1u << j;
+          vc[j].load(vbase + co);
+          vsb[j] = __ldg(vsbase + so);
         }
       }
     };
@@ -284,7 +292,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       const bool full = key0 + kFewKeys - 1 <= min(it.p0, len - 1) &&
                         (u0 < it.head ? key0 + kFewKeys <= it.lo : key0 >= it.from) &&
                         (a.window == 0 || key0 > p1 - a.window || key0 + kFewKeys <= a.first) &&
-                        __all_sync(0xffffffffu, (have & 0xF03u) == 0xF03u);
+                        __all_sync(0xffffffffu, have == 15u);
       // does any query see the group's key j
       auto seen_any = [&](int j) {
         const int key = key0 + j;
@@ -294,7 +302,6 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       float s[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        constexpr int kB = kD > 128 ? 2 : 1;
         uint32_t sc[kB];
         bool plain = true;
 #pragma unroll
@@ -311,15 +318,18 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          const uint32_t word = kc[j].w[k / 2];
+        for (int k = 0; k < kSteps; k += 2) {  // 8 codes: two products' columns
+          const uint4 h = e2m1x8_to_f16(kc[j].w[k / 2]);
+          const uint32_t b[4] = {h.x, h.y, h.z, h.w};
           const uint32_t scale = sc[k * kB / kSteps];
-          const uint32_t b0 = hmul2_u(e2m1x2_to_f16(word, 2 * (k & 1)), scale);
-          const uint32_t b1 = hmul2_u(e2m1x2_to_f16(word, 2 * (k & 1) + 1), scale);
-          if (L::kA == 2)
-            mma_16816(s[j], qa[k][0], 0u, qa[k][1], 0u, b0, b1);
-          else
-            mma_16816(s[j], qa[k][0], qa[k][1], qa[k][2 % L::kA], qa[k][3 % L::kA], b0, b1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t b0 = hmul2_u(b[2 * i], scale), b1 = hmul2_u(b[2 * i + 1], scale);
+            if (L::kA == 2)
+              mma_16816(s[j], qa[k + i][0], 0u, qa[k + i][1], 0u, b0, b1);
+            else
+              mma_16816(s[j], qa[k + i][0], qa[k + i][1], qa[k + i][2 % L::kA], qa[k + i][3 % L::kA], b0, b1);
+          }
         }
       }
       const int next = grp + kFewWarps;
@@ -339,7 +349,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int jj = 2 * t + e + 8 * j, key = key0 + jj;
-            const bool any = seen_any(jj) && (have >> (8 + 2 * j + e) & 1);
+            const bool any = seen_any(jj) && (have >> (2 * j + e) & 1);
 #pragma unroll
             for (int u = 0; u < kNt; ++u) {
               const int p = it.p0 + row_tok(g + 8 * u);
@@ -414,7 +424,10 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       for (int i = 0; i < kSteps; ++i) {
         uint32_t h[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = e2m1x2_to_f16(vc[j].w[i / 4], i & 3);
+        for (int j = 0; j < 4; ++j) {
+          const uint4 x = e2m1x8_to_f16(vc[j].w[i / 4]);  // the compiler keeps what it needs of it
+          h[j] = (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w;
+        }
         const uint32_t a0 = hmul2_u(__byte_perm(h[0], h[1], 0x5410), sc01);
         const uint32_t a1 = hmul2_u(__byte_perm(h[0], h[1], 0x7632), sc01);
         const uint32_t a2 = hmul2_u(__byte_perm(h[2], h[3], 0x5410), sc23);

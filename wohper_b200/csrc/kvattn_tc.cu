@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         for (int k = 0; k < 2; ++k) {
           const int v = jj * kKvTile + lane + 32 * k;
           key[k] = v >= x.seen ? -1 : kv_key(x.head, x.start, v);
-          blk[k] = key[k] < 0 ? -1 : a.block_table[(long long)rr * a.max_blocks + key[k] / a.c.page];
+          blk[k] = key[k] < 0 ? -1 : a.block_table[(long long)rr * a.max_blocks + kv_page_of(a.c, key[k])];
         }
       };
       look_up(c.r, c.it, c.j);
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
             b = -1;
           }
           if (ck[k] < 0) b = -1;
-          const int row = b < 0 ? 0 : kvh_ * a.c.page + ck[k] % a.c.page;
+          const int row = b < 0 ? 0 : kvh_ * a.c.page + (ck[k] - kv_page_of(a.c, ck[k]) * a.c.page);
           all = all && b >= 0 && ck[k] <= x.p0 &&
                 (a.window == 0 || ck[k] > p1 - a.window || ck[k] < a.first);
           f.row[lane + 32 * k] = make_int2(b, row);

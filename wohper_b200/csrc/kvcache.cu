@@ -371,6 +371,9 @@ wh_status kv_cache_check(const wh_kv_cache* c, KvCacheDev* out) {
   out->values = c->values ? c->values : c->keys;
   out->value_scales = c->value_scales ? c->value_scales : c->key_scales;
   out->shared = c->values == nullptr;
+  out->page_shift = -1;
+  for (int k = 0; k <= 20; ++k)
+    if (c->page == 1 << k) out->page_shift = k;
   out->block_stride = c->block_stride ? c->block_stride : dense;
   out->scale_block_stride = c->scale_block_stride ? c->scale_block_stride : dense_s;
   return WH_OK;

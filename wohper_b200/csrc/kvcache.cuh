@@ -12,6 +12,7 @@ namespace wh {
 struct KvCacheDev {
   int blocks, page, kv_heads, head_dim;
   int shared;  // the values are the keys
+  int page_shift;  // log2(page), -1 where page is no power of two
   uint8_t *keys, *key_scales, *values, *value_scales;
   long long block_stride, scale_block_stride;  // bytes
 };
@@ -28,6 +29,11 @@ __device__ __forceinline__ long long kv_code_offset(const KvCacheDev& c, int64_t
 __device__ __forceinline__ long long kv_scale_offset(const KvCacheDev& c, int64_t slot,
                                                      long long row) {
   return (slot / c.page) * c.scale_block_stride + row * (c.head_dim / 32);
+}
+
+// Which of a request's blocks holds row i.
+__device__ __forceinline__ int kv_page_of(const KvCacheDev& c, int i) {
+  return c.page_shift >= 0 ? i >> c.page_shift : i / c.page;
 }
 
 constexpr uint32_t kKvScaleNan = 253;  // scale bytes from here on: the block is not finite
