@@ -23,6 +23,7 @@
 namespace wh {
 
 constexpr int kFewWarps = 8, kFewThreads = kFewWarps * 32;
+constexpr int kFewAhead = 3;  // groups beyond the next that L2 is asked for
 constexpr int kFewKeys = 16;  // rows of the cache a warp takes at a time
 
 template <int kD, int kNt, bool kSplit>
@@ -43,6 +44,9 @@ struct KvFew {
   static constexpr int kBytes = kFewWarps * kRn * kD * 4 + (int)sizeof(Misc);
 };
 
+__device__ __forceinline__ void prefetch_l2(const uint8_t* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory");
+}
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -191,22 +195,37 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 
     const int p1 = it.p0 + it.nt - 1;
     const int len = kv_clip(a, c.len);
-    const int32_t* table = a.block_table + (long long)c.r * a.max_blocks;
-    // groups of 16 rows of the item's list that this warp takes
+    // groups of 16 rows of the item's list: this warp takes grp0, grp0 + 8, ...
     const int past = min((c.j + n) * (kKvTile / kFewKeys), (it.seen + kFewKeys - 1) / kFewKeys);
-    int grp = c.j * (kKvTile / kFewKeys) + warp;
-
-    // A group's block (even pages).  A key that is not there reads block 0 and counts as
-    // not seen.
-    auto block_of = [&](int gi) {
-      if (!even || gi >= past) return -1;
-      const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
-      int b = key0 < len ? table[kv_page_of(a.c, key0)] : -1;
-      if (key0 < len && (b < 0 || b >= a.c.blocks)) {
-        flag(a.status, WH_DEV_BADARG);
-        b = -1;
+    const int grp0 = c.j * (kKvTile / kFewKeys) + warp;
+    const int groups = grp0 < past ? (past - grp0 + kFewWarps - 1) / kFewWarps : 0;
+    auto key0_of = [&](int k) { return kv_key(it.head, it.start, (grp0 + k * kFewWarps) * kFewKeys); };
+    const int32_t* table = a.block_table + (long long)c.r * a.max_blocks;
+    // Even pages: lane i looks up the warp's group first + i, 32 at a time.  A group
+    // that is not there reads block 0 and counts as not seen.
+    long long lane_co = 0, lane_so = 0;  // its rows' codes and scales
+    uint32_t there = 0, whole_seen = 0;  // bit i: it is there; every query sees all of it
+    auto look_up = [&](int first) {
+      const int k = first + lane;
+      bool th = false, all = false;
+      lane_co = lane_so = 0;
+      if (even && k < groups) {
+        const int u0 = (grp0 + k * kFewWarps) * kFewKeys, key0 = key0_of(k);
+        const int pg = kv_page_of(a.c, key0), in = key0 - pg * a.c.page;
+        int b = key0 < len ? table[pg] : -1;
+        if (key0 < len && (b < 0 || b >= a.c.blocks)) {
+          flag(a.status, WH_DEV_BADARG);
+          b = -1;
+        }
+        th = b >= 0;
+        lane_co = max(b, 0) * a.c.block_stride + (long long)in * (kD / 2);
+        lane_so = max(b, 0) * a.c.scale_block_stride + (long long)in * (kD / 32);
+        all = th && key0 + kFewKeys - 1 <= min(it.p0, len - 1) &&
+              (u0 < it.head ? key0 + kFewKeys <= it.lo : key0 >= it.from) &&
+              (a.window == 0 || key0 > p1 - a.window || key0 + kFewKeys <= a.first);
       }
-      return b;
+      there = __ballot_sync(0xffffffffu, th);
+      whole_seen = __ballot_sync(0xffffffffu, all);
     };
     // uneven pages: block and row of one key
     auto locate = [&](int key, long long& co, long long& so) {
@@ -222,7 +241,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       return b >= 0;
     };
     constexpr int kB = kD > 128 ? 2 : 1;  // scale bytes of a key that a lane needs
-    // this lane's columns in the head's first row
+    // this lane's columns in the head's first row (keys: row g, values: row 2t)
     const long long head_codes = (long long)c.kvh * a.c.page * (kD / 2), head_scales = (long long)c.kvh * a.c.page * (kD / 32);
     const uint8_t* kbase = a.c.keys + head_codes + t * L::kKBytes;
     const uint8_t* ksbase = a.c.key_scales + head_scales + (kD == 64 ? t >> 1 : kD == 128 ? t : 2 * t);
@@ -232,67 +251,83 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
     uint32_t ksb[2][kB];
     KvWords<L::kVBytes> vc[4];
     uint32_t vsb[4];
-    uint32_t have = 0;  // bit j: key 2t + (j & 1) + 8 (j >> 1) is there
-    auto load_k = [&](int gi, int block) {
-      const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
+    uint32_t have = 0;  // uneven pages: bit j: key 2t + (j & 1) + 8 (j >> 1) is there
+    // the loads of the warp's group k, which lane i has looked up
+    auto load_k = [&](int k, int i) {
       if (even) {
-        const int in = key0 - kv_page_of(a.c, key0) * a.c.page;
-        const uint8_t* kp = kbase + max(block, 0) * a.c.block_stride + (in + g) * (kD / 2);
-        const uint8_t* sp = ksbase + max(block, 0) * a.c.scale_block_stride + (in + g) * (kD / 32);
+        const uint8_t* kp = kbase + __shfl_sync(0xffffffffu, lane_co, i) + g * (kD / 2);
+        const uint8_t* sp = ksbase + __shfl_sync(0xffffffffu, lane_so, i) + g * (kD / 32);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           kc[j].load(kp + 8 * j * (kD / 2));
 #pragma unroll
-          for (int i = 0; i < kB; ++i) ksb[j][i] = __ldg(sp + 8 * j * (kD / 32) + i);
+          for (int b = 0; b < kB; ++b) ksb[j][b] = __ldg(sp + 8 * j * (kD / 32) + b);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           long long co, so;
-          locate(key0 + g + 8 * j, co, so);
+          locate(key0_of(k) + g + 8 * j, co, so);
           kc[j].load(kbase + co);
 #pragma unroll
-          for (int i = 0; i < kB; ++i) ksb[j][i] = __ldg(ksbase + so + i);
+          for (int b = 0; b < kB; ++b) ksb[j][b] = __ldg(ksbase + so + b);
         }
       }
     };
-    auto load_v = [&](int gi, int block) {
-      const int key0 = kv_key(it.head, it.start, gi * kFewKeys);
+    auto load_v = [&](int k, int i) {
       if (even) {
-        const int in = key0 - kv_page_of(a.c, key0) * a.c.page + 2 * t;
-        const uint8_t* vp = vbase + max(block, 0) * a.c.block_stride + in * (kD / 2);
-        const uint8_t* sp = vsbase + max(block, 0) * a.c.scale_block_stride + in * (kD / 32);
+        const uint8_t* vp = vbase + __shfl_sync(0xffffffffu, lane_co, i) + 2 * t * (kD / 2);
+        const uint8_t* sp = vsbase + __shfl_sync(0xffffffffu, lane_so, i) + 2 * t * (kD / 32);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           vc[j].load(vp + ((j & 1) + 8 * (j >> 1)) * (kD / 2));
           vsb[j] = __ldg(sp + ((j & 1) + 8 * (j >> 1)) * (kD / 32));
         }
-        have = block >= 0 ? 15u : 0u;
       } else {
         have = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           long long co, so;
-          if (locate(key0 + 2 * t + (j & 1) + 8 * (j >> 1), co, so)) have |= 1u << j;
+          if (locate(key0_of(k) + 2 * t + (j & 1) + 8 * (j >> 1), co, so)) have |= 1u << j;
           vc[j].load(vbase + co);
           vsb[j] = __ldg(vsbase + so);
         }
       }
     };
+    // The loads of a group are issued half a step ahead, less than DRAM takes: L2 is
+    // asked for the group kFewAhead after the next (an even page holds it in one piece).
+    const uint8_t* kfetch = a.c.keys + head_codes + lane * 32;
+    const uint8_t* vfetch = a.c.values + head_codes + lane * 32;
+    const uint8_t* sfetch = (lane < 16 ? a.c.key_scales : a.c.value_scales) + head_scales + (lane & 15) * 32;
+    auto fetch = [&](int i) {
+      const long long co = __shfl_sync(0xffffffffu, lane_co, i), so = __shfl_sync(0xffffffffu, lane_so, i);
+#pragma unroll
+      for (int b = 0; b < kFewKeys * kD / 2; b += 1024)
+        if (lane * 32 + b < kFewKeys * kD / 2) {
+          prefetch_l2(kfetch + co + b);
+          if (!a.c.shared) prefetch_l2(vfetch + co + b);
+        }
+      if ((lane & 15) * 32 < kFewKeys * kD / 32) prefetch_l2(sfetch + so);
+    };
 
-    int block = block_of(grp), block_next = block_of(grp + kFewWarps);
-    if (grp < past) {
-      load_k(grp, block);
-      load_v(grp, block);
-    }
-    for (; grp < past; grp += kFewWarps) {
-      const int u0 = grp * kFewKeys;
+    for (int first = 0; first < groups; first += 32 - 1 - kFewAhead) {
+     look_up(first);
+     if (first == 0) {
+       load_k(0, 0);
+       load_v(0, 0);
+#pragma unroll
+       for (int i = 1; i <= kFewAhead; ++i)
+         if (even && i < groups) fetch(i);
+     }
+     const int turn = min(groups - first, 32 - 1 - kFewAhead);
+     for (int i = 0; i < turn; ++i) {
+      const int k = first + i;
+      const bool more = k + 1 < groups;
+      if (even && k + 1 + kFewAhead < groups) fetch(i + 1 + kFewAhead);
+      const int u0 = (grp0 + k * kFewWarps) * kFewKeys;
       const int key0 = kv_key(it.head, it.start, u0);
       // every row of the group is there and seen by every query
-      const bool full = key0 + kFewKeys - 1 <= min(it.p0, len - 1) &&
-                        (u0 < it.head ? key0 + kFewKeys <= it.lo : key0 >= it.from) &&
-                        (a.window == 0 || key0 > p1 - a.window || key0 + kFewKeys <= a.first) &&
-                        __all_sync(0xffffffffu, have == 15u);
+      const bool full = whole_seen >> i & 1;
       // does any query see the group's key j
       auto seen_any = [&](int j) {
         const int key = key0 + j;
@@ -315,25 +350,28 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
           for (int i = 0; i < kB; ++i) sc[i] = few_scale(ksb[j][i], lost);
           if (lost && seen_any(g + 8 * j)) m.redo = 1;
         }
+        // two sums, so that one product need not wait for the one before
+        float s1[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) s[j][e] = s1[e] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kSteps; k += 2) {  // 8 codes: two products' columns
-          const uint4 h = e2m1x8_to_f16(kc[j].w[k / 2]);
+        for (int q = 0; q < kSteps; q += 2) {  // 8 codes: two products' columns
+          const uint4 h = e2m1x8_to_f16(kc[j].w[q / 2]);
           const uint32_t b[4] = {h.x, h.y, h.z, h.w};
-          const uint32_t scale = sc[k * kB / kSteps];
+          const uint32_t scale = sc[q * kB / kSteps];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t b0 = hmul2_u(b[2 * i], scale), b1 = hmul2_u(b[2 * i + 1], scale);
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t b0 = hmul2_u(b[2 * e], scale), b1 = hmul2_u(b[2 * e + 1], scale);
             if (L::kA == 2)
-              mma_16816(s[j], qa[k + i][0], 0u, qa[k + i][1], 0u, b0, b1);
+              mma_16816(e ? s1 : s[j], qa[q + e][0], 0u, qa[q + e][1], 0u, b0, b1);
             else
-              mma_16816(s[j], qa[k + i][0], qa[k + i][1], qa[k + i][2 % L::kA], qa[k + i][3 % L::kA], b0, b1);
+              mma_16816(e ? s1 : s[j], qa[q + e][0], qa[q + e][1], qa[q + e][2 % L::kA], qa[q + e][3 % L::kA], b0, b1);
           }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] += s1[e];
       }
-      const int next = grp + kFewWarps;
-      if (next < past) load_k(next, block_next);
+      if (more) load_k(k + 1, i + 1);
       // ---- log2 weights: x[u][j][e] of row g + 8u, key 2t + e + 8j ----
       float x[kNt][2][2];
 #pragma unroll
@@ -349,7 +387,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int jj = 2 * t + e + 8 * j, key = key0 + jj;
-            const bool any = seen_any(jj) && (have >> (2 * j + e) & 1);
+            const bool any = seen_any(jj) && (even ? there >> i & 1 : have >> (2 * j + e) & 1);
 #pragma unroll
             for (int u = 0; u < kNt; ++u) {
               const int p = it.p0 + row_tok(g + 8 * u);
@@ -421,23 +459,30 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       }
       const uint32_t sc01 = __byte_perm(sc[0], sc[1], 0x5410), sc23 = __byte_perm(sc[2], sc[3], 0x5410);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        uint32_t h[4];
+      for (int i = 0; i < L::kVBytes / 4; ++i) {  // 8 columns: four tiles
+        // a byte of ev / od: the codes of two keys for one even / odd column
+        uint32_t ev[2], od[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 x = e2m1x8_to_f16(vc[j].w[i / 4]);  // the compiler keeps what it needs of it
-          h[j] = (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w;
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t x = vc[2 * k].w[i], y = vc[2 * k + 1].w[i];
+          ev[k] = (x & 0x0F0F0F0Fu) | (y << 4 & 0xF0F0F0F0u);
+          od[k] = (x >> 4 & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u);
         }
-        const uint32_t a0 = hmul2_u(__byte_perm(h[0], h[1], 0x5410), sc01);
-        const uint32_t a1 = hmul2_u(__byte_perm(h[0], h[1], 0x7632), sc01);
-        const uint32_t a2 = hmul2_u(__byte_perm(h[2], h[3], 0x5410), sc23);
-        const uint32_t a3 = hmul2_u(__byte_perm(h[2], h[3], 0x7632), sc23);
+        const uint4 e0 = e2m1x8_to_f16(ev[0]), e1 = e2m1x8_to_f16(ev[1]);
+        const uint4 o0 = e2m1x8_to_f16(od[0]), o1 = e2m1x8_to_f16(od[1]);
+        const uint32_t b0[4] = {e0.x, e0.y, e0.z, e0.w}, b1[4] = {o0.x, o0.y, o0.z, o0.w};
+        const uint32_t b2[4] = {e1.x, e1.y, e1.z, e1.w}, b3[4] = {o1.x, o1.y, o1.z, o1.w};
 #pragma unroll
-        for (int u = 0; u < kNt; ++u) mma_16816(o[i][u], a0, a1, a2, a3, pb[u][0], pb[u][1]);
-        if (kSplit) mma_16816(o[i][0], a0, a1, a2, a3, pl[0], pl[1]);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a0 = hmul2_u(b0[k], sc01), a1 = hmul2_u(b1[k], sc01);
+          const uint32_t a2 = hmul2_u(b2[k], sc23), a3 = hmul2_u(b3[k], sc23);
+#pragma unroll
+          for (int u = 0; u < kNt; ++u) mma_16816(o[4 * i + k][u], a0, a1, a2, a3, pb[u][0], pb[u][1]);
+          if (kSplit) mma_16816(o[4 * i + k][0], a0, a1, a2, a3, pl[0], pl[1]);
+        }
       }
-      if (next < past) load_v(next, block_next);
-      block_next = block_of(next + kFewWarps);
+      if (more) load_v(k + 1, i + 1);
+     }
     }
 
     // ---------------- the CTA's warps joined, the rows out or to a partial slot ----------------
