@@ -245,56 +245,95 @@ __device__ __forceinline__ uint32_t e2m1x2_rn(float lo, float hi) {
   return r;
 }
 
+// How a CTA walks rows: a row is `units` lanes of 8 values (all heads), `side`
+// rows lie side by side in the CTA, and a thread takes kRowsEach of them, whose
+// loads are all issued before the first is used.
+constexpr int kRowCta = 256, kRowsEach = 4;
+struct KvRows {
+  int units, wide, side;  // wide: units that one pass of the CTA covers
+  int ctas;
+};
+static KvRows kv_rows(const KvCacheDev& c, int rows) {
+  KvRows r;
+  r.units = c.kv_heads * (c.head_dim / 8);
+  r.wide = std::min(r.units, kRowCta);
+  r.side = kRowCta / r.wide;
+  r.ctas = (rows + r.side * kRowsEach - 1) / (r.side * kRowsEach);
+  return r;
+}
+struct KvSlot {
+  int block, row;  // block -1: not there
+};
+__device__ __forceinline__ KvSlot kv_slot(const KvCacheDev& c, int64_t slot, uint32_t* status) {
+  if (slot < 0) return {-1, 0};
+  if (slot >= (int64_t)c.blocks * c.page) {
+    flag(status, WH_DEV_BADARG);
+    return {-1, 0};
+  }
+  KvSlot s;
+  s.block = c.page_shift >= 0 ? int(slot >> c.page_shift) : int(slot / c.page);
+  s.row = int(slot - (int64_t)s.block * c.page);
+  return s;
+}
+
 // Four lanes take a block of 32 values, 8 each: wide contiguous loads, the
 // block's maximum by two shuffles, 4 bytes of codes a lane, the scale byte from
-// the first.  Reads size * 32 + writes 17 bytes a block; HBM bound.
+// the first.  Reads 32 values and writes 17 bytes a block.
 template <class T>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvAppendArgs a) {
+__global__ void __launch_bounds__(kRowCta) kv_append_kernel(KvAppendArgs a, KvRows r) {
   pdl_wait_prior();
-  const int which = blockIdx.y;
-  const int parts = a.c.head_dim / 8;  // lanes a row of one head takes (a multiple of 4)
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long total = (long long)a.rows * a.c.kv_heads * parts;
-  if (i >= total) return;  // total and the block size are multiples of 4: whole groups leave
+  const bool values = blockIdx.y;
+  const int side = threadIdx.x / r.wide;
+  if (side >= r.side) return;  // r.wide is a multiple of 4: whole groups leave
   const unsigned group = 0xFu << (threadIdx.x & 28);
-  const int part = int(i % parts);
-  const long long rh = i / parts;
-  const int head = int(rh % a.c.kv_heads);
-  const int row = int(rh / a.c.kv_heads);
-  const int64_t slot = a.slots[row];
-  if (slot < 0) return;
-  if (slot >= (int64_t)a.c.blocks * a.c.page) {
-    flag(a.status, WH_DEV_BADARG);
-    return;
-  }
-  float v[8];
-  kv_load8(reinterpret_cast<const T*>(a.x[which]) + row * a.row_stride[which] +
-               head * a.head_stride[which] + part * 8,
-           v);
-  float m = 0.0f;
-  bool fin = true;
+  const long long row_stride = values ? a.row_stride[1] : a.row_stride[0];
+  const long long head_stride = values ? a.head_stride[1] : a.head_stride[0];
+  const T* x = static_cast<const T*>(values ? a.x[1] : a.x[0]);
+  uint8_t* codes = values ? a.c.values : a.c.keys;
+  uint8_t* scales = values ? a.c.value_scales : a.c.key_scales;
+  const int row0 = blockIdx.x * r.side * kRowsEach + side;
+  KvSlot at[kRowsEach];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    m = fmaxf(m, fabsf(v[j]));
-    fin &= isfinite(v[j]);
+  for (int k = 0; k < kRowsEach; ++k) {
+    const int row = row0 + k * r.side;
+    at[k] = row < a.rows ? kv_slot(a.c, a.slots[row], a.status) : KvSlot{-1, 0};
   }
-  m = fmaxf(m, __shfl_xor_sync(group, m, 1));
-  m = fmaxf(m, __shfl_xor_sync(group, m, 2));
-  fin = __all_sync(group, fin);
-  const int k = e2m1_block_exp(m);
-  const uint32_t byte = !fin ? 255u : m == 0.0f ? 0u : uint32_t(k + 127);
-  const float inv = exp2i(-k);
-  uint32_t w = 0;
-  if (fin) {
+  const int parts = a.c.head_dim / 8;
+  for (int u = threadIdx.x - side * r.wide; u < r.units; u += r.wide) {
+    const int head = u / parts, part = u - head * parts;
+    float v[kRowsEach][8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w |= e2m1x2_rn(__fmul_rn(v[2 * j], inv), __fmul_rn(v[2 * j + 1], inv)) << (8 * j);
+    for (int k = 0; k < kRowsEach; ++k)
+      if (at[k].block >= 0)
+        kv_load8(x + (row0 + k * r.side) * row_stride + head * head_stride + part * 8, v[k]);
+#pragma unroll
+    for (int k = 0; k < kRowsEach; ++k) {
+      if (at[k].block < 0) continue;  // the four lanes alike
+      float m = 0.0f;
+      bool fin = true;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        m = fmaxf(m, fabsf(v[k][j]));
+        fin &= isfinite(v[k][j]);
+      }
+      m = fmaxf(m, __shfl_xor_sync(group, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(group, m, 2));
+      fin = __all_sync(group, fin);
+      const int e = e2m1_block_exp(m);
+      const uint32_t byte = !fin ? 255u : m == 0.0f ? 0u : uint32_t(e + 127);
+      const float inv = exp2i(-e);
+      uint32_t w = 0;
+      if (fin) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w |= e2m1x2_rn(__fmul_rn(v[k][2 * j], inv), __fmul_rn(v[k][2 * j + 1], inv)) << (8 * j);
+      }
+      const long long row = (long long)head * a.c.page + at[k].row;
+      reinterpret_cast<uint32_t*>(codes + at[k].block * a.c.block_stride + row * (a.c.head_dim / 2))[part] = w;
+      if ((part & 3) == 0)
+        scales[at[k].block * a.c.scale_block_stride + row * (a.c.head_dim / 32) + (part >> 2)] = (uint8_t)byte;
+    }
   }
-  const long long at = kv_row(a.c, slot, head);
-  uint8_t* codes = (which ? a.c.values : a.c.keys) + kv_code_offset(a.c, slot, at);
-  uint8_t* scales = (which ? a.c.value_scales : a.c.key_scales) + kv_scale_offset(a.c, slot, at);
-  reinterpret_cast<uint32_t*>(codes)[part] = w;
-  if ((part & 3) == 0) scales[part >> 2] = (uint8_t)byte;
 }
 
 // ---------------------------------------------------------------------------
@@ -309,30 +348,45 @@ struct KvGatherArgs {
 };
 
 // A lane takes 8 values: 4 bytes of codes and the block's scale byte in, one
-// 16-byte store (two for f32) out, all contiguous over a warp.  HBM bound.
+// 16-byte store (two for f32) out, all contiguous over a row.
 template <class T>
-__global__ void __launch_bounds__(256) kv_gather_kernel(KvGatherArgs a) {
+__global__ void __launch_bounds__(kRowCta) kv_gather_kernel(KvGatherArgs a, KvRows r) {
   pdl_wait_prior();
-  const int which = blockIdx.y;
-  const int parts = a.c.head_dim / 8;
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (long long)a.rows * a.c.kv_heads * parts) return;
-  const int part = int(i % parts);
-  const long long rh = i / parts;
-  const int head = int(rh % a.c.kv_heads);
-  const int row = int(rh / a.c.kv_heads);
-  const int64_t slot = a.slots[row];
-  const bool in = slot >= 0 && slot < (int64_t)a.c.blocks * a.c.page;
-  if (slot >= 0 && !in) flag(a.status, WH_DEV_BADARG);
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (in) {
-    const long long at = kv_row(a.c, slot, head);
-    const uint8_t* codes = (which ? a.c.values : a.c.keys) + kv_code_offset(a.c, slot, at);
-    const uint8_t* scales =
-        (which ? a.c.value_scales : a.c.key_scales) + kv_scale_offset(a.c, slot, at);
-    kv_decode8(reinterpret_cast<const uint32_t*>(codes)[part], scales[part >> 2], v);
+  const bool values = blockIdx.y;
+  const int side = threadIdx.x / r.wide;
+  if (side >= r.side) return;
+  const uint8_t* codes = values ? a.c.values : a.c.keys;
+  const uint8_t* scales = values ? a.c.value_scales : a.c.key_scales;
+  T* out = static_cast<T*>(values ? a.out[1] : a.out[0]);
+  const int row0 = blockIdx.x * r.side * kRowsEach + side;
+  KvSlot at[kRowsEach];
+#pragma unroll
+  for (int k = 0; k < kRowsEach; ++k) {
+    const int row = row0 + k * r.side;
+    at[k] = row < a.rows ? kv_slot(a.c, a.slots[row], a.status) : KvSlot{-1, 0};
   }
-  kv_store8(reinterpret_cast<T*>(a.out[which]) + rh * a.c.head_dim + part * 8, v);
+  const int parts = a.c.head_dim / 8;
+  for (int u = threadIdx.x - side * r.wide; u < r.units; u += r.wide) {
+    const int head = u / parts, part = u - head * parts;
+    uint32_t w[kRowsEach], sb[kRowsEach];
+#pragma unroll
+    for (int k = 0; k < kRowsEach; ++k) {
+      w[k] = sb[k] = 0;
+      if (at[k].block >= 0) {
+        const long long row = (long long)head * a.c.page + at[k].row;
+        w[k] = __ldg(reinterpret_cast<const uint32_t*>(codes + at[k].block * a.c.block_stride + row * (a.c.head_dim / 2)) + part);
+        sb[k] = __ldg(scales + at[k].block * a.c.scale_block_stride + row * (a.c.head_dim / 32) + (part >> 2));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRowsEach; ++k) {
+      const int row = row0 + k * r.side;
+      if (row >= a.rows) continue;
+      float v[8];
+      kv_decode8(w[k], sb[k], v);
+      kv_store8(out + ((long long)row * r.units + u) * 8, v);
+    }
+  }
 }
 
 }  // namespace wh
@@ -443,8 +497,7 @@ wh_status wh_kv_append(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots
   if (!kv_rows_aligned(k, k_row_stride, k_head_stride, size) ||
       (v && !kv_rows_aligned(v, v_row_stride, v_head_stride, size)))
     return fail(WH_ERR_INVALID_POINTER, "append: rows must start on 16 bytes");
-  const long long ctas = ((long long)rows * a.c.kv_heads * (a.c.head_dim / 8) + 255) / 256;
-  if (ctas > 0x7fffffffLL) return fail(WH_ERR_UNSUPPORTED, "append: too many rows");
+  const KvRows r = kv_rows(a.c, rows);
   a.slots = slots;
   a.rows = rows;
   a.x[0] = k;
@@ -454,14 +507,14 @@ wh_status wh_kv_append(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots
   a.head_stride[0] = k_head_stride;
   a.head_stride[1] = v_head_stride;
   a.status = c->status;
-  const dim3 grid((unsigned)ctas, v ? 2 : 1);
+  const dim3 grid(r.ctas, v ? 2 : 1);
   const cudaStream_t s = (cudaStream_t)stream;
   if (dtype == WH_DTYPE_F32)
-    WH_CUDA(launch_pdl(kv_append_kernel<float>, grid, 256, 0, s, c->pdl(), a));
+    WH_CUDA(launch_pdl(kv_append_kernel<float>, grid, kRowCta, 0, s, c->pdl(), a, r));
   else if (dtype == WH_DTYPE_BF16)
-    WH_CUDA(launch_pdl(kv_append_kernel<__nv_bfloat16>, grid, 256, 0, s, c->pdl(), a));
+    WH_CUDA(launch_pdl(kv_append_kernel<__nv_bfloat16>, grid, kRowCta, 0, s, c->pdl(), a, r));
   else
-    WH_CUDA(launch_pdl(kv_append_kernel<__half>, grid, 256, 0, s, c->pdl(), a));
+    WH_CUDA(launch_pdl(kv_append_kernel<__half>, grid, kRowCta, 0, s, c->pdl(), a, r));
   return WH_OK;
 }
 
@@ -478,21 +531,20 @@ wh_status wh_kv_gather(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots
     return fail(WH_ERR_INVALID_POINTER, "gather: slots, k (v only where the cache has values)");
   if (!aligned(k, 16) || !aligned(v, 16))
     return fail(WH_ERR_INVALID_POINTER, "gather: outputs must be 16-byte aligned");
-  const long long ctas = ((long long)rows * a.c.kv_heads * (a.c.head_dim / 8) + 255) / 256;
-  if (ctas > 0x7fffffffLL) return fail(WH_ERR_UNSUPPORTED, "gather: too many rows");
+  const KvRows r = kv_rows(a.c, rows);
   a.slots = slots;
   a.rows = rows;
   a.out[0] = k;
   a.out[1] = v;
   a.status = c->status;
-  const dim3 grid((unsigned)ctas, v ? 2 : 1);
+  const dim3 grid(r.ctas, v ? 2 : 1);
   const cudaStream_t s = (cudaStream_t)stream;
   if (dtype == WH_DTYPE_F32)
-    WH_CUDA(launch_pdl(kv_gather_kernel<float>, grid, 256, 0, s, c->pdl(), a));
+    WH_CUDA(launch_pdl(kv_gather_kernel<float>, grid, kRowCta, 0, s, c->pdl(), a, r));
   else if (dtype == WH_DTYPE_BF16)
-    WH_CUDA(launch_pdl(kv_gather_kernel<__nv_bfloat16>, grid, 256, 0, s, c->pdl(), a));
+    WH_CUDA(launch_pdl(kv_gather_kernel<__nv_bfloat16>, grid, kRowCta, 0, s, c->pdl(), a, r));
   else
-    WH_CUDA(launch_pdl(kv_gather_kernel<__half>, grid, 256, 0, s, c->pdl(), a));
+    WH_CUDA(launch_pdl(kv_gather_kernel<__half>, grid, kRowCta, 0, s, c->pdl(), a, r));
   return WH_OK;
 }
 
