@@ -246,19 +246,19 @@ __device__ __forceinline__ uint32_t e2m1x2_rn(float lo, float hi) {
 }
 
 // How a CTA walks rows: a row is `units` lanes of 8 values (all heads), `side`
-// rows lie side by side in the CTA, and a thread takes kRowsEach of them, whose
+// rows lie side by side in the CTA, and a thread takes `kEach` of them, whose
 // loads are all issued before the first is used.
-constexpr int kRowCta = 256, kRowsEach = 4;
+constexpr int kRowCta = 256;
 struct KvRows {
   int units, wide, side;  // wide: units that one pass of the CTA covers
   int ctas;
 };
-static KvRows kv_rows(const KvCacheDev& c, int rows) {
+static KvRows kv_rows(const KvCacheDev& c, int rows, int each) {
   KvRows r;
   r.units = c.kv_heads * (c.head_dim / 8);
   r.wide = std::min(r.units, kRowCta);
   r.side = kRowCta / r.wide;
-  r.ctas = (rows + r.side * kRowsEach - 1) / (r.side * kRowsEach);
+  r.ctas = (rows + r.side * each - 1) / (r.side * each);
   return r;
 }
 struct KvSlot {
@@ -279,8 +279,10 @@ __device__ __forceinline__ KvSlot kv_slot(const KvCacheDev& c, int64_t slot, uin
 // Four lanes take a block of 32 values, 8 each: wide contiguous loads, the
 // block's maximum by two shuffles, 4 bytes of codes a lane, the scale byte from
 // the first.  Reads 32 values and writes 17 bytes a block.
+constexpr int kAppendEach = 2;
 template <class T>
-__global__ void __launch_bounds__(kRowCta) kv_append_kernel(KvAppendArgs a, KvRows r) {
+__global__ void __launch_bounds__(kRowCta, 5) kv_append_kernel(KvAppendArgs a, KvRows r) {
+  constexpr int kEach = kAppendEach;
   pdl_wait_prior();
   const bool values = blockIdx.y;
   const int side = threadIdx.x / r.wide;
@@ -291,30 +293,31 @@ __global__ void __launch_bounds__(kRowCta) kv_append_kernel(KvAppendArgs a, KvRo
   const T* x = static_cast<const T*>(values ? a.x[1] : a.x[0]);
   uint8_t* codes = values ? a.c.values : a.c.keys;
   uint8_t* scales = values ? a.c.value_scales : a.c.key_scales;
-  const int row0 = blockIdx.x * r.side * kRowsEach + side;
-  KvSlot at[kRowsEach];
-#pragma unroll
-  for (int k = 0; k < kRowsEach; ++k) {
-    const int row = row0 + k * r.side;
-    at[k] = row < a.rows ? kv_slot(a.c, a.slots[row], a.status) : KvSlot{-1, 0};
-  }
+  const int row0 = blockIdx.x * r.side * kEach + side;
   const int parts = a.c.head_dim / 8;
   for (int u = threadIdx.x - side * r.wide; u < r.units; u += r.wide) {
     const int head = u / parts, part = u - head * parts;
-    float v[kRowsEach][8];
+    // the rows' values and slots are asked for together
+    KvRaw8<T> raw[kEach];
+    int64_t slot[kEach];
 #pragma unroll
-    for (int k = 0; k < kRowsEach; ++k)
-      if (at[k].block >= 0)
-        kv_load8(x + (row0 + k * r.side) * row_stride + head * head_stride + part * 8, v[k]);
+    for (int k = 0; k < kEach; ++k) {
+      const int row = min(row0 + k * r.side, a.rows - 1);
+      slot[k] = row0 + k * r.side < a.rows ? a.slots[row] : -1;
+      raw[k].load(x + row * row_stride + head * head_stride + part * 8);
+    }
 #pragma unroll
-    for (int k = 0; k < kRowsEach; ++k) {
-      if (at[k].block < 0) continue;  // the four lanes alike
+    for (int k = 0; k < kEach; ++k) {
+      const KvSlot at = kv_slot(a.c, slot[k], a.status);
+      if (at.block < 0) continue;  // the four lanes alike
+      float v[8];
+      raw[k].widen(v);
       float m = 0.0f;
       bool fin = true;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        m = fmaxf(m, fabsf(v[k][j]));
-        fin &= isfinite(v[k][j]);
+        m = fmaxf(m, fabsf(v[j]));
+        fin &= isfinite(v[j]);
       }
       m = fmaxf(m, __shfl_xor_sync(group, m, 1));
       m = fmaxf(m, __shfl_xor_sync(group, m, 2));
@@ -326,12 +329,12 @@ __global__ void __launch_bounds__(kRowCta) kv_append_kernel(KvAppendArgs a, KvRo
       if (fin) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          w |= e2m1x2_rn(__fmul_rn(v[k][2 * j], inv), __fmul_rn(v[k][2 * j + 1], inv)) << (8 * j);
+          w |= e2m1x2_rn(__fmul_rn(v[2 * j], inv), __fmul_rn(v[2 * j + 1], inv)) << (8 * j);
       }
-      const long long row = (long long)head * a.c.page + at[k].row;
-      reinterpret_cast<uint32_t*>(codes + at[k].block * a.c.block_stride + row * (a.c.head_dim / 2))[part] = w;
+      const long long row = (long long)head * a.c.page + at.row;
+      reinterpret_cast<uint32_t*>(codes + at.block * a.c.block_stride + row * (a.c.head_dim / 2))[part] = w;
       if ((part & 3) == 0)
-        scales[at[k].block * a.c.scale_block_stride + row * (a.c.head_dim / 32) + (part >> 2)] = (uint8_t)byte;
+        scales[at.block * a.c.scale_block_stride + row * (a.c.head_dim / 32) + (part >> 2)] = (uint8_t)byte;
     }
   }
 }
@@ -349,8 +352,10 @@ struct KvGatherArgs {
 
 // A lane takes 8 values: 4 bytes of codes and the block's scale byte in, one
 // 16-byte store (two for f32) out, all contiguous over a row.
+constexpr int kGatherEach = 4;
 template <class T>
 __global__ void __launch_bounds__(kRowCta) kv_gather_kernel(KvGatherArgs a, KvRows r) {
+  constexpr int kEach = kGatherEach;
   pdl_wait_prior();
   const bool values = blockIdx.y;
   const int side = threadIdx.x / r.wide;
@@ -358,19 +363,19 @@ __global__ void __launch_bounds__(kRowCta) kv_gather_kernel(KvGatherArgs a, KvRo
   const uint8_t* codes = values ? a.c.values : a.c.keys;
   const uint8_t* scales = values ? a.c.value_scales : a.c.key_scales;
   T* out = static_cast<T*>(values ? a.out[1] : a.out[0]);
-  const int row0 = blockIdx.x * r.side * kRowsEach + side;
-  KvSlot at[kRowsEach];
+  const int row0 = blockIdx.x * r.side * kEach + side;
+  KvSlot at[kEach];
 #pragma unroll
-  for (int k = 0; k < kRowsEach; ++k) {
+  for (int k = 0; k < kEach; ++k) {
     const int row = row0 + k * r.side;
     at[k] = row < a.rows ? kv_slot(a.c, a.slots[row], a.status) : KvSlot{-1, 0};
   }
   const int parts = a.c.head_dim / 8;
   for (int u = threadIdx.x - side * r.wide; u < r.units; u += r.wide) {
     const int head = u / parts, part = u - head * parts;
-    uint32_t w[kRowsEach], sb[kRowsEach];
+    uint32_t w[kEach], sb[kEach];
 #pragma unroll
-    for (int k = 0; k < kRowsEach; ++k) {
+    for (int k = 0; k < kEach; ++k) {
       w[k] = sb[k] = 0;
       if (at[k].block >= 0) {
         const long long row = (long long)head * a.c.page + at[k].row;
@@ -379,7 +384,7 @@ __global__ void __launch_bounds__(kRowCta) kv_gather_kernel(KvGatherArgs a, KvRo
       }
     }
 #pragma unroll
-    for (int k = 0; k < kRowsEach; ++k) {
+    for (int k = 0; k < kEach; ++k) {
       const int row = row0 + k * r.side;
       if (row >= a.rows) continue;
       float v[8];
@@ -497,7 +502,7 @@ wh_status wh_kv_append(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots
   if (!kv_rows_aligned(k, k_row_stride, k_head_stride, size) ||
       (v && !kv_rows_aligned(v, v_row_stride, v_head_stride, size)))
     return fail(WH_ERR_INVALID_POINTER, "append: rows must start on 16 bytes");
-  const KvRows r = kv_rows(a.c, rows);
+  const KvRows r = kv_rows(a.c, rows, kAppendEach);
   a.slots = slots;
   a.rows = rows;
   a.x[0] = k;
@@ -531,7 +536,7 @@ wh_status wh_kv_gather(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots
     return fail(WH_ERR_INVALID_POINTER, "gather: slots, k (v only where the cache has values)");
   if (!aligned(k, 16) || !aligned(v, 16))
     return fail(WH_ERR_INVALID_POINTER, "gather: outputs must be 16-byte aligned");
-  const KvRows r = kv_rows(a.c, rows);
+  const KvRows r = kv_rows(a.c, rows, kGatherEach);
   a.slots = slots;
   a.rows = rows;
   a.out[0] = k;

@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace wh {
@@ -16,20 +18,6 @@ struct KvCacheDev {
   uint8_t *keys, *key_scales, *values, *value_scales;
   long long block_stride, scale_block_stride;  // bytes
 };
-
-// Slot s holds row s % page of block s / page; a head's rows are contiguous in
-// their block.  kv_row: the row's index among its block's rows.
-__device__ __forceinline__ long long kv_row(const KvCacheDev& c, int64_t slot, int head) {
-  return (long long)head * c.page + (long long)(slot % c.page);
-}
-__device__ __forceinline__ long long kv_code_offset(const KvCacheDev& c, int64_t slot,
-                                                    long long row) {
-  return (slot / c.page) * c.block_stride + row * (c.head_dim / 2);
-}
-__device__ __forceinline__ long long kv_scale_offset(const KvCacheDev& c, int64_t slot,
-                                                     long long row) {
-  return (slot / c.page) * c.scale_block_stride + row * (c.head_dim / 32);
-}
 
 // Which of a request's blocks holds row i.
 __device__ __forceinline__ int kv_page_of(const KvCacheDev& c, int i) {
@@ -59,30 +47,39 @@ __device__ __forceinline__ void kv_decode8(uint32_t w, uint32_t scale_byte, floa
   }
 }
 
-// 8 consecutive elements, 16-byte aligned
-__device__ __forceinline__ void kv_load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void kv_load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 8 consecutive elements, 16-byte aligned, as they lie in memory
+template <class T>
+struct KvRaw8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[2 * j] = __uint_as_float(w[j] << 16);
-    v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
-__device__ __forceinline__ void kv_load8(const __half* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = h2_to_f2(w[j]);
-    v[2 * j] = f.x;
-    v[2 * j + 1] = f.y;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (std::is_same<T, float>::value) {
+          v[(4 * i + j) & 7] = __uint_as_float(x[j]);
+        } else if (std::is_same<T, __nv_bfloat16>::value) {
+          v[2 * j] = __uint_as_float(x[j] << 16);
+          v[2 * j + 1] = __uint_as_float(x[j] & 0xFFFF0000u);
+        } else {
+          const float2 f = h2_to_f2(x[j]);
+          v[2 * j] = f.x;
+          v[2 * j + 1] = f.y;
+        }
+      }
+    }
   }
+};
+template <class T>
+__device__ __forceinline__ void kv_load8(const T* p, float (&v)[8]) {
+  KvRaw8<T> r;
+  r.load(p);
+  r.widen(v);
 }
 __device__ __forceinline__ void kv_store8(float* p, const float (&v)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
