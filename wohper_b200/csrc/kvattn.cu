@@ -170,10 +170,13 @@ __global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(KvAttnArgs a
 // all columns; few rows (long contexts, many parts): a CTA each and 128 columns.
 // Bound by the latency of four dependent loads (row, parts' maxima, sums, store).
 // ---------------------------------------------------------------------------
+constexpr int kJoinParts = 512;  // most CTAs that a line is cut into
 template <class T, int kV, int kWpr>
 __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWork w) {
   __shared__ KvRowSmem sm;
   __shared__ int redo_row[4];
+  __shared__ float red[4];
+  extern __shared__ float2 part[];  // [rows][kJoinParts]: maximum (then weight), sum
   constexpr int kRows = kRowThreads / 32 / kWpr;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = warp % kWpr;
@@ -191,46 +194,66 @@ __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWo
   auto slot_of = [&](int p) { return 2 * (mt.x + p) + (p == 0 ? mt.z & 1 : 0); };
   const float inf = __int_as_float(0x7f800000);
   int redo = bad ? 0 : mt.w;
-  const bool join = !bad && parts > 1;
-  float top = -inf, base = 0.0f, z = 0.0f;
-  if (join) {
-    for (int p = lane; p < parts; p += 32) {
+  bool join = !bad && parts > 1;
+  // the parts' maxima and sums, kept beside; the row's maximum
+  float2* ml = &part[warp / kWpr * kJoinParts];
+  float top = -inf;
+  if (join)
+    for (int p = sub * 32 + lane; p < parts; p += 32 * kWpr) {
+      const float2 x = w.part_ml[(long long)slot_of(p) * w.rn + row];
       redo |= w.part_redo[slot_of(p)];
-      top = fmaxf(top, w.part_ml[(long long)slot_of(p) * w.rn + row].x);
+      ml[p] = x;
+      top = fmaxf(top, x.x);
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    redo = __any_sync(0xffffffffu, redo);
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  redo = __any_sync(0xffffffffu, redo);
+  if (kWpr > 1) {  // one row a CTA
+    if (lane == 0) red[warp] = top;
+    redo = __syncthreads_or(redo);
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  } else {
+    __syncwarp();
   }
+  join = join && !redo;
+  const float sk = a.sink && join ? a.sink[h] * kLog2e : -inf;
+  const float to = fmaxf(top, sk), base = to == -inf ? 0.0f : to;
+  // their weights; the row's sum
+  float z = 0.0f;
+  if (join)
+    for (int p = sub * 32 + lane; p < parts; p += 32 * kWpr) {
+      const float2 x = ml[p];
+      const float f = x.x == -inf ? 0.0f : exp2f(x.x - base);
+      z += x.y * f;
+      ml[p].x = f;
+    }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  if (kWpr > 1) {
+    __syncthreads();
+    if (lane == 0) red[warp] = z;
+    __syncthreads();
+    z = (red[0] + red[1]) + (red[2] + red[3]);
+  } else {
+    __syncwarp();
+  }
+  if (a.sink && join) z += exp2f(sk - base + kLift);
   float4 acc[kV];
 #pragma unroll
   for (int v = 0; v < kV; ++v) acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const int D = a.c.head_dim, dim = blockIdx.y * 128 + lane * 4;
-  if (join && !redo) {
-    const float sk = a.sink ? a.sink[h] * kLog2e : -inf;
-    const float to = fmaxf(top, sk);
-    base = to == -inf ? 0.0f : to;
-    for (int p = lane; p < parts; p += 32) {
-      const float2 ml = w.part_ml[(long long)slot_of(p) * w.rn + row];
-      z += ml.x == -inf ? 0.0f : ml.y * exp2f(ml.x - base);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    if (a.sink) z += exp2f(sk - base + kLift);
-    if (dim < D) {
+  if (join && dim < D) {
 #pragma unroll(kV == 1 ? 8 : 8 / kV)
-      for (int p = sub; p < parts; p += kWpr) {
-        const long long at = (long long)slot_of(p) * w.rn + row;
-        const float m = w.part_ml[at].x;
-        const float f = m == -inf ? 0.0f : exp2f(m - base);
+    for (int p = sub; p < parts; p += kWpr) {
+      const float f = ml[p].x;
+      const float* at = w.part_o + ((long long)slot_of(p) * w.rn + row) * D + dim;
 #pragma unroll
-        for (int v = 0; v < kV; ++v) {
-          const float4 o = *reinterpret_cast<const float4*>(w.part_o + at * D + dim + v * 128);
-          acc[v].x = fmaf(f, o.x, acc[v].x);
-          acc[v].y = fmaf(f, o.y, acc[v].y);
-          acc[v].z = fmaf(f, o.z, acc[v].z);
-          acc[v].w = fmaf(f, o.w, acc[v].w);
-        }
+      for (int v = 0; v < kV; ++v) {
+        const float4 o = *reinterpret_cast<const float4*>(at + v * 128);
+        acc[v].x = fmaf(f, o.x, acc[v].x);
+        acc[v].y = fmaf(f, o.y, acc[v].y);
+        acc[v].z = fmaf(f, o.z, acc[v].z);
+        acc[v].w = fmaf(f, o.w, acc[v].w);
       }
     }
   }
@@ -247,7 +270,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWo
       acc[0].w += o.w;
     }
   }
-  if (join && !redo && sub == 0 && dim < D) {
+  if (join && sub == 0 && dim < D) {
     const float inv = z == 0.0f ? 0.0f : 1.0f / z;
     T* out = reinterpret_cast<T*>(a.out) + t * a.out_token_stride + h * a.out_head_stride + dim;
 #pragma unroll
@@ -306,7 +329,7 @@ KvHow kv_how(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads,
     w.lead = d == 512 ? 4 : 8;
     w.align = 1;
   }
-  w.min_units = w.lead + 2;
+  w.ctas = std::min(w.ctas, kJoinParts);
   w.tt = std::max(1, w.rn / group);
   w.ht = (group + w.rn - 1) / w.rn;
   return p;
@@ -355,12 +378,13 @@ cudaError_t kv_launch(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool 
                                    : kv_launch_tc<64>(a, p, s, pdl);
   if (e != cudaSuccess) return e;
   if (rows <= 4u * p.w.ctas)
-    return launch_pdl(kv_join_kernel<T, 1, 4>, dim3(rows, std::max(1, d / 128)), kRowThreads, 0, s,
-                      pdl, a, p.w);
+    return launch_pdl(kv_join_kernel<T, 1, 4>, dim3(rows, std::max(1, d / 128)), kRowThreads,
+                      kJoinParts * sizeof(float2), s, pdl, a, p.w);
   const dim3 grid((rows + 3) / 4);
-  return d == 512   ? launch_pdl(kv_join_kernel<T, 4, 1>, grid, kRowThreads, 0, s, pdl, a, p.w)
-         : d == 256 ? launch_pdl(kv_join_kernel<T, 2, 1>, grid, kRowThreads, 0, s, pdl, a, p.w)
-                    : launch_pdl(kv_join_kernel<T, 1, 1>, grid, kRowThreads, 0, s, pdl, a, p.w);
+  const size_t smem = 4 * kJoinParts * sizeof(float2);
+  return d == 512   ? launch_pdl(kv_join_kernel<T, 4, 1>, grid, kRowThreads, smem, s, pdl, a, p.w)
+         : d == 256 ? launch_pdl(kv_join_kernel<T, 2, 1>, grid, kRowThreads, smem, s, pdl, a, p.w)
+                    : launch_pdl(kv_join_kernel<T, 1, 1>, grid, kRowThreads, smem, s, pdl, a, p.w);
 }
 
 }  // namespace

@@ -77,7 +77,7 @@ struct KvWork {
   int ht;    // items that one token's heads of one kv head take
   int lead;  // units ahead of an item's tiles
   int align;  // rows that an item's list begins at multiples of (a power of two)
-  int ctas, min_units;
+  int ctas;
   int4* meta;       // [tokens][heads]: first CTA, CTAs, its slot and row, redo
   float* part_o;    // [2 * ctas][rn][head_dim]
   float2* part_ml;  // [2 * ctas][rn]: maximum (base 2), sum
@@ -120,7 +120,7 @@ struct KvCut {
   __device__ __forceinline__ KvCut(const KvWork& w, long long units) : total(units) {
     if (units <= 0x7fffffffLL) {
       const int u = (int)units;
-      ctas = min(w.ctas, u / w.min_units + (u % w.min_units != 0));
+      ctas = min(w.ctas, u);
       each = u / max(ctas, 1);
       more = u - (int)each * ctas;
     } else {
@@ -173,31 +173,6 @@ __device__ __forceinline__ void kv_place(const KvAttnArgs& a, const KvWork& w, K
     if (q.tq.y > 0 && kv_clip(a, q.len) != q.len) flag(a.status, WH_DEV_BADARG);
     return q;
   };
-  // x becomes the inclusive sums over the CTA's threads; returns the sum of all
-  auto scan = [&](long long (&x)[2], long long (&all)[2]) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long p = __shfl_up_sync(0xffffffffu, x[k], o);
-        if (lane >= o) x[k] += p;
-      }
-      if (lane == 31) m.part[k][warp] = x[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      long long y = lane < kWarps ? m.part[k][lane] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long p = __shfl_up_sync(0xffffffffu, y, o);
-        if (lane >= o) y += p;
-      }
-      all[k] = __shfl_sync(0xffffffffu, y, 31);
-      const long long before = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
-      if (warp > 0) x[k] += before;
-    }
-  };
   // Unit x of the line is unit `off` of request r, whose tiles follow `tiles`
   // earlier ones: the first tile at or after x, and (where) the item it is in.
   auto find = [&](int r, const Req& q, long long off, long long tiles, bool where) {
@@ -226,44 +201,84 @@ __device__ __forceinline__ void kv_place(const KvAttnArgs& a, const KvWork& w, K
     }
     return tiles + (long long)u * it.tiles + j;
   };
-  Req q = request(tid);
-  long long x[2] = {q.units, q.tiles};
-  for (int r = tid + kThreads; r < a.requests; r += kThreads) {
-    const Req p = request(r);
-    x[0] += p.units;
-    x[1] += p.tiles;
-  }
-  long long all[2];
-  scan(x, all);
-  const KvCut cut(w, all[0]);
-  if (tid == 0) {
-    const bool in = (int)blockIdx.x < cut.ctas;
-    m.total = all[0];
-    m.begin = in ? cut.start(blockIdx.x) : 0;
-    m.end = in ? cut.start(blockIdx.x + 1) : 0;
-  }
-  if ((int)blockIdx.x < cut.ctas) {
-    const long long b = cut.start(blockIdx.x), e = cut.start(blockIdx.x + 1);
-    if (tid == 0 && e == all[0]) m.last_tile = all[1];
-    long long base[2] = {0, 0};
-    for (int r0 = 0; r0 < a.requests && base[0] <= e; r0 += kThreads) {
-      if (a.requests > kThreads) {  // several requests a thread: again, in their order
-        q = request(r0 + tid);
-        x[0] = q.units;
-        x[1] = q.tiles;
-        __syncthreads();
-        scan(x, all);
-        x[0] += base[0];
-        x[1] += base[1];
-        base[0] += all[0];
-        base[1] += all[1];
-      } else {
-        base[0] = e + 1;
-      }
-      const long long u0 = x[0] - q.units, t0 = x[1] - q.tiles;
-      if (u0 <= b && b < x[0]) m.first_tile = find(r0 + tid, q, b - u0, t0, true);
-      if (u0 <= e && e < x[0]) m.last_tile = find(r0 + tid, q, e - u0, t0, false);
+  // Inclusive sums over kThreads requests at a time; with more requests than that
+  // the line's length first.  Loops are kept rolled: this code runs once.
+  long long total[2] = {0, 0}, base[2] = {0, 0};
+  if (a.requests > kThreads) {
+    for (int r = tid; r < a.requests; r += kThreads) {
+      const Req p = request(r);
+      total[0] += p.units;
+      total[1] += p.tiles;
     }
+#pragma unroll 1
+    for (int o = 16; o; o >>= 1) {
+      total[0] += __shfl_xor_sync(0xffffffffu, total[0], o);
+      total[1] += __shfl_xor_sync(0xffffffffu, total[1], o);
+    }
+    if (lane == 0) {
+      m.part[0][warp] = total[0];
+      m.part[1][warp] = total[1];
+    }
+    __syncthreads();
+    total[0] = total[1] = 0;
+    for (int k = 0; k < kWarps; ++k) {
+      total[0] += m.part[0][k];
+      total[1] += m.part[1][k];
+    }
+    __syncthreads();
+  }
+#pragma unroll 1
+  for (int r0 = 0; r0 < a.requests; r0 += kThreads) {
+    const Req q = request(r0 + tid);
+    long long x[2] = {q.units, q.tiles};
+    if (r0 + warp * 32 < a.requests) {
+#pragma unroll 1
+      for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const long long p = __shfl_up_sync(0xffffffffu, x[k], o);
+          if (lane >= o) x[k] += p;
+        }
+      }
+      if (lane == 31) {
+        m.part[0][warp] = x[0];
+        m.part[1][warp] = x[1];
+      }
+    }
+    __syncthreads();
+    long long before[2] = {base[0], base[1]};
+#pragma unroll 1
+    for (int k = 0; k < kWarps && r0 + k * 32 < a.requests; ++k) {
+      if (k < warp) {
+        before[0] += m.part[0][k];
+        before[1] += m.part[1][k];
+      }
+      base[0] += m.part[0][k];
+      base[1] += m.part[1][k];
+    }
+    if (a.requests <= kThreads) {
+      total[0] = base[0];
+      total[1] = base[1];
+    }
+    const KvCut cut(w, total[0]);
+    const bool in = (int)blockIdx.x < cut.ctas;
+    const long long b = in ? cut.start(blockIdx.x) : 0, e = in ? cut.start(blockIdx.x + 1) : 0;
+    if (tid == 0 && r0 == 0) {
+      m.total = total[0];
+      m.begin = b;
+      m.end = e;
+      if (e == total[0]) m.last_tile = total[1];
+    }
+    const long long u0 = before[0] + x[0] - q.units, t0 = before[1] + x[1] - q.tiles;
+#pragma unroll 1
+    for (int k = 0; in && k < 2; ++k) {
+      const long long at = k ? e : b;
+      if (u0 > at || at >= u0 + q.units) continue;
+      const long long tile = find(r0 + tid, q, at - u0, t0, k == 0);
+      (k ? m.last_tile : m.first_tile) = tile;
+    }
+    if (base[0] > e) break;  // uniform
+    __syncthreads();
   }
   __syncthreads();
 }

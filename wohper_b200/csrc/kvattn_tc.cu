@@ -810,7 +810,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
             }
             const int live = rows - r0;
             const uint32_t col = tmem_w + L::kTmemO + (r0 - half * kRh) * (kSplit ? 2 : 1);
-#pragma unroll
+#pragma unroll 1
             for (int blk = 0; blk < L::kBlocks; ++blk) {
               float v[8];
               if (kSplit) {
