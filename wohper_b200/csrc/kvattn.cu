@@ -295,10 +295,14 @@ __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWo
 namespace {
 
 // Which kernel takes the call and how it cuts the queries.
-//  - few: at most 16 query rows (8 of f32) to a kv head and request, rows of at
-//    most 256: decoded in registers, bound by the cache's bytes;
-//  - tc: other rows of 64, 128, 256 and 512;
-//  - otherwise one CTA a query row.
+//  - few: a pass over the cache for every 16 query rows (8 of f32) of a kv head,
+//    nearly bound by its bytes;
+//  - tc: one pass for 64 rows (32 of f32), bound by the tile pipeline;
+//  - row: a CTA a query row, for rows of other widths.
+// Measured on 8 requests of 4096 rows, 8 kv heads, us (few / tc), rows to a kv head:
+//   64 wide,  bf16: 16 21/62, 32 31/63;    f32: 16 27/52, 32 45/53
+//   128 wide, bf16: 16 31/65, 32 47/66, 48 64/67, 64 81/67;  f32: 16 39/60, 32 67/62
+//   256 wide, bf16: 16 66/81, 32 101/81;   f32: 16 68/81, 32 118/81
 // A call's tokens are taken as evenly spread over its requests, the one thing
 // the host knows; an item with fewer rows than it has room for is still right.
 enum class KvWay { few, tc, row };
@@ -316,9 +320,10 @@ KvHow kv_how(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads,
   p.split = dtype == WH_DTYPE_F32;
   const long long each = (long long)group * ((tokens + requests - 1) / requests);
   KvWork& w = p.w;
-  if (d <= 256 && each <= (p.split ? 8 : 16)) {
+  const int most = d == 256 ? 20 : (d == 128 ? 48 : 64) / (p.split ? 2 : 1);
+  if (d <= 256 && each <= most) {
     p.way = KvWay::few;
-    w.rn = each <= 8 ? 8 : 16;
+    w.rn = p.split || each <= 8 ? 8 : 16;
     w.ctas = c->num_sms * (d * w.rn <= 8 * 128 ? 2 : 1);
     w.lead = 8;
     w.align = kFewKeys;
@@ -326,7 +331,7 @@ KvHow kv_how(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads,
     p.way = KvWay::tc;
     w.rn = p.split ? kTcCols / 2 : kTcCols;
     w.ctas = c->num_sms;
-    w.lead = d == 512 ? 4 : 8;
+    w.lead = 4;
     w.align = 1;
   }
   w.ctas = std::min(w.ctas, kJoinParts);

@@ -580,6 +580,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 template <int kD, int kNt, bool kSplit>
 static cudaError_t launch_attend_few(const KvAttnArgs& a, const KvWork& w, cudaStream_t s, bool pdl) {
   using L = KvFew<kD, kNt, kSplit>;
+  if (w.rn != L::kRn) return cudaErrorInvalidValue;
   const cudaError_t e = ensure_smem(kv_attend_few_kernel<kD, kNt, kSplit>, L::kBytes);
   if (e != cudaSuccess) return e;
   return launch_pdl(kv_attend_few_kernel<kD, kNt, kSplit>, dim3(w.ctas), kFewThreads, L::kBytes, s, pdl, a, w);

@@ -858,6 +858,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
 template <int kD, bool kSplit, bool kSep>
 static cudaError_t launch_attend_tc(const KvAttnArgs& a, const KvWork& w, cudaStream_t s, bool pdl) {
   const size_t smem = KvTcSmem<kD, kSplit, kSep>::kBytes;
+  if (w.rn != KvTc<kD, kSplit>::kRn) return cudaErrorInvalidValue;
   const cudaError_t e = ensure_smem(kv_attend_tc_kernel<kD, kSplit, kSep>, smem);
   if (e != cudaSuccess) return e;
   return launch_pdl(kv_attend_tc_kernel<kD, kSplit, kSep>, dim3(w.ctas), kTcThreads, smem, s, pdl, a, w);
