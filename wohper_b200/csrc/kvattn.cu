@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(KvAttnArgs a
 // all columns; few rows (long contexts, many parts): a CTA each and 128 columns.
 // Bound by the latency of four dependent loads (row, parts' maxima, sums, store).
 // ---------------------------------------------------------------------------
-constexpr int kJoinParts = 512;  // most CTAs that a line is cut into
+constexpr int kJoinParts = 640;  // most CTAs that a line is cut into
 template <class T, int kV, int kWpr>
 __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWork w) {
   __shared__ KvRowSmem sm;
@@ -324,7 +324,7 @@ KvHow kv_how(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads,
   if (d <= 256 && each <= most) {
     p.way = KvWay::few;
     w.rn = p.split || each <= 8 ? 8 : 16;
-    w.ctas = c->num_sms * (d * w.rn <= 8 * 128 ? 2 : 1);
+    w.ctas = c->num_sms * (d * w.rn <= 8 * 128 ? 4 : 2);
     w.lead = 8;
     w.align = kFewKeys;
   } else {

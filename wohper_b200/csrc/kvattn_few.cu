@@ -22,7 +22,7 @@
 
 namespace wh {
 
-constexpr int kFewWarps = 8, kFewThreads = kFewWarps * 32;
+constexpr int kFewWarps = 4, kFewThreads = kFewWarps * 32;
 constexpr int kFewAhead = 3;  // groups beyond the next that L2 is asked for
 constexpr int kFewKeys = 16;  // rows of the cache a warp takes at a time
 
@@ -33,7 +33,7 @@ struct KvFew {
   static constexpr int kSteps = kD / 16;   // products of S along D; 16-column tiles of O^T
   static constexpr int kA = kSplit || kNt == 2 ? 4 : 2;  // registers of A that are not zero
   static constexpr int kKBytes = kD / 8, kVBytes = kD / 16;  // of a row's codes a lane has
-  static constexpr int kCtas = kD * kNt <= 128 ? 2 : 1;      // resident CTAs aimed at
+  static constexpr int kCtas = kD * kNt <= 128 ? 4 : 2;      // resident CTAs aimed at
   struct Misc {
     KvPlace at;
     float top[kFewWarps][kRn], sum[kFewWarps][kRn];
