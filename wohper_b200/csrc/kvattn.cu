@@ -324,7 +324,7 @@ KvHow kv_how(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads,
   if (d <= 256 && each <= most) {
     p.way = KvWay::few;
     w.rn = p.split || each <= 8 ? 8 : 16;
-    w.ctas = c->num_sms * (d * w.rn <= 8 * 128 ? 4 : 2);
+    w.ctas = c->num_sms * (d * w.rn <= 8 * 128 ? 4 : d * w.rn == 8 * 256 ? 3 : 2);
     w.lead = 8;
     w.align = kFewKeys;
   } else {

@@ -33,8 +33,10 @@ struct KvFew {
   static constexpr int kSteps = kD / 16;   // products of S along D; 16-column tiles of O^T
   static constexpr int kA = kSplit || kNt == 2 ? 4 : 2;  // registers of A that are not zero
   static constexpr int kKBytes = kD / 8, kVBytes = kD / 16;  // of a row's codes a lane has
-  static constexpr int kCtas = kD * kNt <= 128 ? 4 : 2;      // resident CTAs aimed at
+  static constexpr int kCtas = kD * kNt <= 128 ? 4 : kD * kNt == 256 ? 3 : 2;      // resident CTAs aimed at
   struct Misc {
+    alignas(16) uint32_t q[kSteps][32][kA];  // A's registers of each product, a lane's together
+    float fac[kRn];              // accumulator -> log2 score
     KvPlace at;
     float top[kFewWarps][kRn], sum[kFewWarps][kRn];
     float out_scale[kRn];
@@ -129,56 +131,62 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
     if (tid == 0) m.redo = 0;
     __syncthreads();
 
-    // the queries as A: lane (g, t) holds columns [t D/4, (t+1) D/4) of row g (and g + 8)
-    uint32_t qa[kSteps][L::kA];
+    // The queries as A: lane (g, t) holds columns [t D/4, (t+1) D/4) of row g (and g + 8).
+    // One warp makes them, all read them from shared memory: they would take a
+    // fifth of the registers.
+    if (warp == 0) {
+#pragma unroll 1
+      for (int u = 0; u < kNt; ++u) {
+        const int row = g + 8 * u;
+        const bool real = row < rows;
+        float v[kD / 4];
+        const long long off = real ? (it.t0 + row_tok(row)) * a.q_token_stride + (h0 + row_head(row)) * a.q_head_stride + t * (kD / 4)
+                                   : 0;
+#pragma unroll
+        for (int e = 0; e < kD / 32; ++e) {
+          float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+          if (real) {
+            if (kSplit)
+              kv_load8(static_cast<const float*>(a.q) + off + 8 * e, x);
+            else if (a.dtype == WH_DTYPE_BF16)
+              kv_load8(static_cast<const __nv_bfloat16*>(a.q) + off + 8 * e, x);
+            else
+              kv_load8(static_cast<const __half*>(a.q) + off + 8 * e, x);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[8 * e + i] = x[i];
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < kD / 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const bool fin = top < 0x7f800000u;
+        if (!fin) m.redo = 1;
+        const int ex = max(int(top >> 23) - 127, -100);
+        const float mul = fin ? exp2i(14 - ex) : 0.0f;
+        if (t == 0) m.fac[row] = a.scale * kLog2e * exp2i(max(ex - 18, -126));
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {  // A's registers 2k (row g) and 2k + 1 (row g + 8)
+            const float x = fin ? v[4 * s + 2 * k] * mul : 0.0f, y = fin ? v[4 * s + 2 * k + 1] * mul : 0.0f;
+            const __half2 hi = __floats2half2_rn(x, y);
+            if (L::kA == 2) {
+              m.q[s][lane][k] = half2_bits(hi);
+            } else if (kSplit) {
+              m.q[s][lane][(2 * k) % L::kA] = half2_bits(hi);
+              m.q[s][lane][(2 * k + 1) % L::kA] = half2_bits(__floats2half2_rn(x - __low2float(hi), y - __high2float(hi)));
+            } else {
+              m.q[s][lane][(2 * k + u) % L::kA] = half2_bits(hi);
+            }
+          }
+      }
+    }
+    __syncthreads();
     float fac[kNt];
 #pragma unroll
-    for (int u = 0; u < kNt; ++u) {
-      const int row = g + 8 * u;
-      const bool real = row < rows;
-      float v[kD / 4];
-      const long long off = real ? (it.t0 + row_tok(row)) * a.q_token_stride + (h0 + row_head(row)) * a.q_head_stride + t * (kD / 4)
-                                 : 0;
-#pragma unroll
-      for (int e = 0; e < kD / 32; ++e) {
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (real) {
-          if (kSplit)
-            kv_load8(static_cast<const float*>(a.q) + off + 8 * e, x);
-          else if (a.dtype == WH_DTYPE_BF16)
-            kv_load8(static_cast<const __nv_bfloat16*>(a.q) + off + 8 * e, x);
-          else
-            kv_load8(static_cast<const __half*>(a.q) + off + 8 * e, x);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * e + i] = x[i];
-      }
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < kD / 4; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const bool fin = top < 0x7f800000u;
-      if (!fin) m.redo = 1;
-      const int ex = max(int(top >> 23) - 127, -100);
-      const float mul = fin ? exp2i(14 - ex) : 0.0f;
-      fac[u] = a.scale * kLog2e * exp2i(max(ex - 18, -126));
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {  // A's registers 2k (row g) and 2k + 1 (row g + 8)
-          const float x = fin ? v[4 * s + 2 * k] * mul : 0.0f, y = fin ? v[4 * s + 2 * k + 1] * mul : 0.0f;
-          const __half2 hi = __floats2half2_rn(x, y);
-          if (L::kA == 2) {
-            qa[s][k] = half2_bits(hi);
-          } else if (kSplit) {
-            qa[s][(2 * k) % L::kA] = half2_bits(hi);
-            qa[s][(2 * k + 1) % L::kA] = half2_bits(__floats2half2_rn(x - __low2float(hi), y - __high2float(hi)));
-          } else {
-            qa[s][(2 * k + u) % L::kA] = half2_bits(hi);
-          }
-        }
-    }
+    for (int u = 0; u < kNt; ++u) fac[u] = m.fac[g + 8 * u];
 
     float o[kSteps][kNt][4];  // tile i: columns g D/8 + 2i (0, 1) and + 2i + 1 (2, 3), rows 2t, 2t + 1
     float off[kNt], sum[kNt];
@@ -335,41 +343,55 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       };
       // ---- scores ----
       float s[2][4];
+      uint32_t ksc[2][kB];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint32_t sc[kB];
         bool plain = true;
 #pragma unroll
-        for (int i = 0; i < kB; ++i) {
-          sc[i] = few_scale_fast(ksb[j][i]);
-          plain = plain && few_ordinary(ksb[j][i]);
+        for (int e = 0; e < kB; ++e) {
+          ksc[j][e] = few_scale_fast(ksb[j][e]);
+          plain = plain && few_ordinary(ksb[j][e]);
         }
         if (!__all_sync(0xffffffffu, plain)) {
           bool lost = false;
 #pragma unroll
-          for (int i = 0; i < kB; ++i) sc[i] = few_scale(ksb[j][i], lost);
+          for (int e = 0; e < kB; ++e) ksc[j][e] = few_scale(ksb[j][e], lost);
           if (lost && seen_any(g + 8 * j)) m.redo = 1;
         }
-        // two sums, so that one product need not wait for the one before
-        float s1[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = s1[e] = 0.0f;
+        for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
+      }
+      // the two key tiles in turn, so that a product need not wait for the one before
 #pragma unroll
-        for (int q = 0; q < kSteps; q += 2) {  // 8 codes: two products' columns
+      for (int q = 0; q < kSteps; q += 2) {  // 8 codes: two products' columns
+        uint32_t b[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
           const uint4 h = e2m1x8_to_f16(kc[j].w[q / 2]);
-          const uint32_t b[4] = {h.x, h.y, h.z, h.w};
-          const uint32_t scale = sc[q * kB / kSteps];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t b0 = hmul2_u(b[2 * e], scale), b1 = hmul2_u(b[2 * e + 1], scale);
-            if (L::kA == 2)
-              mma_16816(e ? s1 : s[j], qa[q + e][0], 0u, qa[q + e][1], 0u, b0, b1);
-            else
-              mma_16816(e ? s1 : s[j], qa[q + e][0], qa[q + e][1], qa[q + e][2 % L::kA], qa[q + e][3 % L::kA], b0, b1);
-          }
+          const uint32_t scale = ksc[j][q * kB / kSteps];
+          b[j][0] = hmul2_u(h.x, scale);
+          b[j][1] = hmul2_u(h.y, scale);
+          b[j][2] = hmul2_u(h.z, scale);
+          b[j][3] = hmul2_u(h.w, scale);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] += s1[e];
+        for (int e = 0; e < 2; ++e) {
+          uint32_t qa[4] = {0, 0, 0, 0};
+          if (L::kA == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(m.q[q + e][lane]);
+            qa[0] = x.x;
+            qa[2] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(m.q[q + e][lane]);
+            qa[0] = x.x;
+            qa[1] = x.y;
+            qa[2] = x.z;
+            qa[3] = x.w;
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            mma_16816(s[j], qa[0], qa[1], qa[2], qa[3], b[j][2 * e], b[j][2 * e + 1]);
+        }
       }
       if (more) load_k(k + 1, i + 1);
       // ---- log2 weights: x[u][j][e] of row g + 8u, key 2t + e + 8j ----
