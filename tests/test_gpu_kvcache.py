@@ -172,6 +172,15 @@ def test_attention_many_requests(ctx, W, layout):
     c.check(W, ctx)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_attention_more_requests_than_a_cta_has_threads(ctx, W, dtype):
+    rng = np.random.default_rng(4)
+    lens, qs = rng.integers(0, 90, 1900).tolist(), rng.integers(0, 2, 1900).tolist()
+    lens[1500] = 700
+    c = Case(24, 9, 1, 512, False, lens, qs, 32, dtype)
+    c.check(W, ctx, window=200, first=2)
+
+
 @pytest.mark.parametrize("layout", [LATENT, (8, 2, 128, True), (32, 8, 128, True)], ids=str)
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
 def test_attention_long_context(ctx, W, layout, dtype):
