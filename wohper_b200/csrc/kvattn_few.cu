@@ -12,9 +12,12 @@
 //                                 [g D/8, (g+1) D/8) of keys 2t, 2t+1, 2t+8, 2t+9;
 //                                 P^T is B, which is how S leaves its product
 // (the order of the columns within a product is free, so every lane's columns are
-// contiguous in memory).  A decode costs about 1.3 instructions a code, the same
-// as the rest of a step together.  Every warp keeps its own maxima, sums and O^T;
+// contiguous in memory).  Every warp keeps its own maxima, sums and O^T;
 // the CTA joins them when an item ends.
+//
+// Measured: 16 requests x 16384 rows, 8 kv heads x 128, 4 bf16 query rows each: 71
+// us with the join, 2.6 TB/s of codes, 56 % of the issue slots, about 410 warp
+// instructions for 16 rows of keys and values.
 //
 // f16 tiles, scales, query halves (kSplit: rows 8-15 of A are the low halves) and
 // rows to be computed again are as in kvattn_tc.cu.  kNt: groups of 8 query rows.
