@@ -40,9 +40,10 @@ namespace wh {
 constexpr int kTcSoft = 8, kTcDec = 16;
 constexpr int kTcMma = kTcSoft + kTcDec, kTcAddr = kTcMma + 1;
 constexpr int kTcThreads = (kTcAddr + 1) * 32;
-// Registers: 72 a thread at launch (26 warps); the decode warps give 8 up, the
-// softmax warps take 16: 8 x 88 + 16 x 64 + 2 x 72 = 26 x 72.
-constexpr int kTcSoftRegs = 88, kTcDecRegs = 64, kTcRegs = 72;
+// Registers: 72 a thread at launch (26 warps); the decode warps give 16 up, the
+// softmax warps take 32: 8 x 104 + 16 x 56 + 2 x 72 = 26 x 72.  More tiles in
+// flight a decode warp (kAhead 2) spilled: 61 against 67 us at 32 x 8192 x 512 bf16.
+constexpr int kTcSoftRegs = 104, kTcDecRegs = 56, kTcRegs = 72;
 static_assert(kTcSoft * kTcSoftRegs + kTcDec * kTcDecRegs <= (kTcSoft + kTcDec) * kTcRegs, "registers");
 static_assert(kTcSoft % 4 == 0 && kTcDec % 4 == 0, "whole warpgroups");
 constexpr int kTcInfo = 8;   // tiles the address warp may run ahead
@@ -83,7 +84,7 @@ struct KvTc {
   static constexpr int kUnits = kD >= 128 ? kD / 128 : 1;
   static constexpr int kPer = kUnits > 1 ? kUnits / 2 : 1;
   static constexpr int kFillers = kUnits > 1 ? kTcDec : kTcDec / 2;  // warps that fill a tile
-  static constexpr int kAhead = kPer > 1 ? 2 : 4;  // tiles whose codes a decode warp has in flight
+  static constexpr int kAhead = 1;  // tiles whose codes a decode warp has in flight: more spilled and lost
   static constexpr int kNh = kN / 2;                        // columns of a softmax half
   static constexpr int kRh = kRn / 2;                       // query rows of a softmax half
   static constexpr int kMax = kNh / 4 / (kSplit ? 2 : 1);   // query rows a softmax thread holds
