@@ -301,9 +301,9 @@ namespace {
 //  - tc: one pass for 64 rows (32 of f32), bound by the tile pipeline;
 //  - row: a CTA a query row, for rows of other widths.
 // Measured on 8 requests of 4096 rows, 8 kv heads, us (few / tc), rows to a kv head:
-//   64 wide,  bf16: 16 21/62, 32 31/63;    f32: 16 27/52, 32 45/53
-//   128 wide, bf16: 16 31/65, 32 47/66, 48 64/67, 64 81/67;  f32: 16 39/60, 32 67/62
-//   256 wide, bf16: 16 66/81, 32 101/81;   f32: 16 68/81, 32 118/81
+//   64 wide,  bf16: 16 21/47, 32 31/48;                f32: 16 27/44, 24 37/45, 32 47/45
+//   128 wide, bf16: 16 26/47, 32 40/49, 48 54/48;      f32: 16 36/44, 32 62/45
+//   256 wide, bf16: 16 50/65, 32 74/66;                f32: 16 60/66, 32 99/66
 // A call's tokens are taken as evenly spread over its requests, the one thing
 // the host knows; an item with fewer rows than it has room for is still right.
 enum class KvWay { few, tc, row };
@@ -321,7 +321,7 @@ KvHow kv_how(const wh_ctx* c, int head_dim, int kv_heads, int tokens, int heads,
   p.split = dtype == WH_DTYPE_F32;
   const long long each = (long long)group * ((tokens + requests - 1) / requests);
   KvWork& w = p.w;
-  const int most = d == 256 ? 20 : (d == 128 ? 48 : 64) / (p.split ? 2 : 1);
+  const int most = p.split ? (d == 256 ? 16 : d == 128 ? 20 : 24) : (d == 256 ? 24 : d == 128 ? 40 : 48);
   if (d <= 256 && each <= most) {
     p.way = KvWay::few;
     w.rn = p.split || each <= 8 ? 8 : 16;
