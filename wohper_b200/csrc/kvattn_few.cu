@@ -331,14 +331,14 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
          if (even && i < groups) fetch(i);
      }
      const int turn = min(groups - first, 32 - 1 - kFewAhead);
-     for (int i = 0; i < turn; ++i) {
-      const int k = first + i;
+     for (int at = 0; at < turn; ++at) {
+      const int k = first + at;
       const bool more = k + 1 < groups;
-      if (even && k + 1 + kFewAhead < groups) fetch(i + 1 + kFewAhead);
+      if (even && k + 1 + kFewAhead < groups) fetch(at + 1 + kFewAhead);
       const int u0 = (grp0 + k * kFewWarps) * kFewKeys;
       const int key0 = kv_key(it.head, it.start, u0);
       // every row of the group is there and seen by every query
-      const bool full = whole_seen >> i & 1;
+      const bool full = whole_seen >> at & 1;
       // does any query see the group's key j
       auto seen_any = [&](int j) {
         const int key = key0 + j;
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
             mma_16816(s[j], qa[0], qa[1], qa[2], qa[3], b[j][2 * e], b[j][2 * e + 1]);
         }
       }
-      if (more) load_k(k + 1, i + 1);
+      if (more) load_k(k + 1, at + 1);
       // ---- log2 weights: x[u][j][e] of row g + 8u, key 2t + e + 8j ----
       float x[kNt][2][2];
 #pragma unroll
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int jj = 2 * t + e + 8 * j, key = key0 + jj;
-            const bool any = seen_any(jj) && (even ? there >> i & 1 : have >> (2 * j + e) & 1);
+            const bool any = seen_any(jj) && (even ? there >> at & 1 : have >> (2 * j + e) & 1);
 #pragma unroll
             for (int u = 0; u < kNt; ++u) {
               const int p = it.p0 + row_tok(g + 8 * u);
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
           if (kSplit) mma_16816(o[4 * i + k][0], a0, a1, a2, a3, pl[0], pl[1]);
         }
       }
-      if (more) load_v(k + 1, i + 1);
+      if (more) load_v(k + 1, at + 1);
      }
     }
 

@@ -27,10 +27,10 @@
 // queries of 512).  The MMA warp takes whichever product is ready, the second
 // one first, since it frees a tile.
 //
-// Measured, 512 wide: a tile takes about 4.3 k cycles, decode 1.0-1.4 k, scores
-// 1.15 k and sums 0.9 k (both bound by the operands' shared-memory reads),
-// softmax 1.7-2.5 k, two tiles in flight; 32 requests x 8192 rows, 64 bf16 heads:
-// 67 us with the join, 26 % of the tensor pipe.  M = 128 keys a product would
+// Measured, 512 wide: decode 1.0-1.4 k cycles a tile, scores 1.15 k and sums 0.9 k
+// (both bound by the operands' shared-memory reads), softmax 1.7-2.5 k, two tiles
+// in flight: about 4 k cycles a tile; 32 requests x 8192 rows, 64 bf16 heads: 61 us
+// with the join, 32 x 4096 of f32 55 us.  M = 128 keys a product would
 // read 14 % fewer operand bytes but leave room for one tile only.
 #include "kvattn.cuh"
 #include "tc.cuh"
