@@ -341,6 +341,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       return __all_sync(0xffffffffu, mbar_test_wait(bar, phase)) != 0;
     };
     int ns = 0, np = 0;     // next tile of the first, of the second product
+    int begun = 0;          // fragments whose first product has begun
     int frags = 0;          // fragments whose second product has begun
     int fl_even = 0, fl_odd = 0;
     uint64_t since = 0;
@@ -376,8 +377,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       if (!did && ns < ntiles && ns < np + 2) {
         const int slot = ns % kTcInfo, ks = ns % kStages, b = ns & 1;
         if (ready(&m.info_full[slot], (ns / kTcInfo) & 1) &&
-            ready(&m.k_full[ks], (ns / kStages) & 1)) {
+            ready(&m.k_full[ks], (ns / kStages) & 1) &&
+            // A new fragment's queries are all there.  k_full does not say so where
+            // half of the decode warps fill the keys (heads up to 128 wide); that
+            // every warp has arrived also keeps q_empty within a phase of them.
+            (!(m.info[slot].flags & kFragFirst) ||
+             ready(&m.q_full[begun % kTcFrag], (begun / kTcFrag) & 1))) {
           const int fl = m.info[slot].flags;
+          begun += fl & kFragFirst;
           (b ? fl_odd : fl_even) = fl;
           tc::fence_after_sync();
           const uint64_t dk_ = dk + (uint32_t(ks) * L::kTileBytes >> 4);
