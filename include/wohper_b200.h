@@ -627,11 +627,13 @@ size_t wh_kv_attention_scratch_bytes(const wh_ctx* ctx, const wh_kv_cache* cache
  * window, or i < first).  sink (nullable) [heads]: a logit that takes part in
  * each softmax and has no value.  A query that sees no row gives zeros.
  *   out [tokens][heads][head_dim] of q's dtype; strides in elements, rows of q
- * and out 16-byte aligned and contiguous.  Rows of tokens from cu_q[requests]
- * on are not written.  Sums, maxima and normalisers are f32; f32 queries give
- * f32 accuracy.  Not-finite rows reach only the queries that see them.
- * Block ids outside the pool and lengths beyond max_blocks * page are recorded
- * as WH_ERR_DEVICE_ARG; such rows count as not seen. */
+ * and out 16-byte aligned and contiguous.  out may be q itself (same address and
+ * strides); it may not overlap q or another input in another way.  Rows of
+ * tokens from cu_q[requests] on are not written.  Sums, maxima and normalisers
+ * are f32; f32 queries give f32 accuracy.  Not-finite rows reach only the
+ * queries that see them.  Block ids outside the pool and lengths beyond
+ * max_blocks * page are recorded as WH_ERR_DEVICE_ARG; such rows count as not
+ * seen. */
 wh_status wh_kv_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void* q, int dtype,
                           int tokens, int heads, long long q_token_stride,
                           long long q_head_stride, int requests, const int32_t* cu_q,

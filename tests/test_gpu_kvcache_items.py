@@ -30,3 +30,29 @@ def test_every_item_is_scored_with_its_own_queries(ctx, W, heads, d, dtype, sep)
         again = W.kv_attention(ctx, *args)
         np.testing.assert_array_equal(again.double().cpu().numpy(), got)
     ctx.sync()
+
+
+@pytest.mark.parametrize("layout", [(64, 1, 512, False), (28, 4, 128, True), (64, 1, 128, True), (16, 2, 256, True),
+                                    (6, 2, 96, True)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_out_may_be_q(ctx, W, layout, dtype):  # noqa: F811
+    # many items that lie in one CTA, some computed again: a query that is not finite, a
+    # scale byte that f16 does not hold; and one long request that is split
+    lens = [40] * 300 + [3000]
+
+    def spoil(c):
+        c.q[::7, 0, 3] = float("nan")
+        for r in range(0, 300, 5):
+            for s in c.scales:
+                s[c.table[r, 1], :, 2, 0] = 90
+
+    c = Case(32, *layout, lens, [1] * 301, 16, dtype, spoil=spoil)
+    args = (dev(c.cu), dev(np.array(lens, np.int32)), dev(c.table))
+    cache = c.cache(W)
+    want = W.kv_attention(ctx, cache, c.q, *args)
+    q = c.q.clone()
+    got = W.kv_attention(ctx, cache, q, *args, out=q)
+    ctx.sync()
+    assert got is q
+    np.testing.assert_array_equal(got.double().cpu().numpy(), want.double().cpu().numpy())
+    assert torch.isfinite(want[:, 1:]).all() and not torch.isfinite(want[::7, 0]).any()

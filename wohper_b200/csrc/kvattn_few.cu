@@ -538,6 +538,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       }
     const bool item_first = c.at + w.lead >= begin, item_last = c.at + w.lead + it.tiles <= end;
     const bool whole = item_first && item_last;
+    const int redo = m.redo;
     if (tid < rows) {
       const int row = tid;
       const int part = 2 * blockIdx.x + slot1;
@@ -547,7 +548,6 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       for (int k = 0; k < kFewWarps; ++k) top = fmaxf(top, m.top[k][row]);
 #pragma unroll
       for (int k = 0; k < kFewWarps; ++k) l += m.top[k][row] == -inf ? 0.0f : m.sum[k][row] * ex2(m.top[k][row] - top);
-      const int redo = m.redo;
       float os = 1.0f / 16.0f;  // the f16 values are 16 times the cache's
       if (whole) {
         float z = l;
@@ -572,7 +572,9 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       }
     }
     __syncthreads();
-    for (int i = tid; i < rows * (kD / 4); i += kFewThreads) {
+    // rows to be computed again are left alone: out may be q, which that still reads
+    const int stored = whole && redo ? 0 : rows;
+    for (int i = tid; i < stored * (kD / 4); i += kFewThreads) {
       const int row = i / (kD / 4), col = i % (kD / 4) * 4;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll

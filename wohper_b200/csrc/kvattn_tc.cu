@@ -772,11 +772,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         tc::fence_after_sync();
         if (!bar_and(bar, 128, ok)) break;
         const bool whole = (flags & kItemFirst) && (flags & kItemLast);
+        const int redo = m.redo[frag % kTcRedo];
         const int rows = w.ht > 1 ? min(kRn, a.group - f.ht * kRn) : f.nt * a.group;
         const int row = half * kRh + quad * 32 + lane;
         if (quad * 32 + lane < kRh && row >= rows) m.out_row[row] = 0;
         if (quad * 32 + lane < kRh && row < rows) {
-          const int redo = m.redo[frag % kTcRedo];
           const int part = 2 * blockIdx.x + (flags & kSlot1 ? 1 : 0);
           const int h = f.kvh * a.group + f.ht * kRn + m.row_head[row];
           const int t = f.t0 + m.row_tok[row];
@@ -846,14 +846,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
             }
           }
         };
-        if (!whole)
+        // rows to be computed again are left alone: out may be q, which that still reads
+        if (!whole) {
           write(w.part_o);
-        else if (kSplit)
-          write(static_cast<float*>(a.out));
-        else if (a.dtype == WH_DTYPE_BF16)
-          write(static_cast<__nv_bfloat16*>(a.out));
-        else
-          write(static_cast<__half*>(a.out));
+        } else if (!redo) {
+          if (kSplit)
+            write(static_cast<float*>(a.out));
+          else if (a.dtype == WH_DTYPE_BF16)
+            write(static_cast<__nv_bfloat16*>(a.out));
+          else
+            write(static_cast<__half*>(a.out));
+        }
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.o_empty);

@@ -283,7 +283,8 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     (cu_q None: one each) and kv_lens[r] rows, the new ones included; the last
     query sits at position kv_lens[r] - 1.  A query at p sees rows i <= p and,
     with a window, only i > p - window or i < first.  sink: f32 [heads] or None.
-    scale defaults to head_dim ** -0.5.  Returns out, like q."""
+    scale defaults to head_dim ** -0.5.  Returns out, like q; out may be q itself,
+    but may not overlap it in another way."""
     dev = cache.keys.device
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         _fail(_INVALID_SHAPE, "q: [tokens, heads, head_dim]")
