@@ -7,7 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from tests.test_gpu_kvcache import BF16, F32, Case, ctx, dev, W  # noqa: F401 (fixtures)
+from tests.test_gpu_kvcache import BF16, F32, Case, ctx, dev, tolerance, W  # noqa: F401 (fixtures)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -56,3 +56,33 @@ def test_out_may_be_q(ctx, W, layout, dtype):  # noqa: F811
     assert got is q
     np.testing.assert_array_equal(got.double().cpu().numpy(), want.double().cpu().numpy())
     assert torch.isfinite(want[:, 1:]).all() and not torch.isfinite(want[::7, 0]).any()
+
+
+@pytest.mark.parametrize("layout", [(64, 1, 512, False), (28, 4, 128, True), (64, 1, 128, True), (64, 1, 64, False),
+                                    (16, 2, 256, True), (6, 2, 96, True)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("sink", [False, True], ids=["", "sink"])
+def test_rows_of_bad_blocks_count_as_not_seen(ctx, W, layout, dtype, sink):  # noqa: F811
+    # runs of bad pages (16 rows) at the front, in the middle, at the end and everywhere,
+    # so that a CTA's first tiles hold no row, over items of one CTA and of several
+    lens, page = [200, 100, 64] + [3000] * 14 + [70], 16
+    c = Case(33, *layout, lens, [1] * len(lens), page, dtype)
+    bad = [[0, 1, 2, 3, 4], [6], [0, 1, 2, 3]]
+    bad += [sorted(c.rng.choice(187, 90, False)) if r % 3 else list(range(r, r + 100)) for r in range(14)]
+    bad += [[0, 2, 3]]
+    lens_d = dev(np.array(lens, np.int32))
+    table = c.table.copy()
+    for r, b in enumerate(bad):
+        table[r, b] = -1 if r % 2 else c.codes[0].shape[0] + r
+    got = W.kv_attention(ctx, c.cache(W), c.q, dev(c.cu), lens_d, dev(table),
+                         sink=dev(c.sink) if sink else None)
+    with pytest.raises(W.WohperError, match="DeviceArg"):
+        ctx.sync()
+    # the plain form over the pages that are there: one query, which sees all of them
+    for r, b in enumerate(bad):
+        left = np.delete(c.table[r], b)
+        c.table[r], c.table[r, :len(left)] = -1, left
+        c.lens[r] = lens[r] - sum(min(page, lens[r] - page * i) for i in b)
+    want, smax, vmax = c.want(layout[2] ** -0.5, sink=c.sink if sink else None)
+    ratio = np.abs(got.double().cpu().numpy() - want) / np.maximum(tolerance(want, smax, vmax, dtype), 1e-300)
+    assert (ratio <= 1).all(), np.argwhere(ratio.max((1, 2)) > 1).ravel()

@@ -678,7 +678,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
       float most = -inf;
 #pragma unroll
       for (int e = 0; e < kMax; ++e) most = fmaxf(most, fmaxf(s[e][0], s[e][1]));
-      const bool stay = ok && !(flags & kFragFirst) && most <= kLift + kLag;
+      bool stay = ok && !(flags & kFragFirst) && most <= kLift + kLag;
+      // A row that has seen nothing yet (its tiles so far lay in blocks outside the
+      // pool) takes its maximum from the first keys that it sees.
+      if (live != (1u << kMax) - 1) {
+#pragma unroll
+        for (int e = 0; e < kMax; ++e)
+          stay = stay && ((live >> e & 1) || fmaxf(s[e][0], s[e][1]) == -inf);
+      }
       tc::fence_before_sync();
       if (!bar_and(bar, 128, stay)) {
         // the tile's maxima, over the warp's 16 keys, then over the warps
