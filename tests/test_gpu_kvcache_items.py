@@ -86,3 +86,29 @@ def test_rows_of_bad_blocks_count_as_not_seen(ctx, W, layout, dtype, sink):  # n
     want, smax, vmax = c.want(layout[2] ** -0.5, sink=c.sink if sink else None)
     ratio = np.abs(got.double().cpu().numpy() - want) / np.maximum(tolerance(want, smax, vmax, dtype), 1e-300)
     assert (ratio <= 1).all(), np.argwhere(ratio.max((1, 2)) > 1).ravel()
+
+
+@pytest.mark.parametrize("page", [1, 7, 16, 24, 100])
+@pytest.mark.parametrize("layout", [(8, 2, 128, True), (28, 4, 128, True), (8, 2, 64, False), (4, 2, 256, True),
+                                    (64, 1, 512, False), (64, 1, 128, True), (6, 2, 96, True)], ids=str)
+@pytest.mark.parametrize("window,first", [(40, 0), (40, 5), (130, 33)])
+def test_pages_that_no_query_sees_need_no_block(ctx, W, page, layout, window, first):  # noqa: F811
+    # a server gives back the pages behind the window: their entries are -1 (or stale
+    # ids past a pool that shrank), and the step is still an ordinary one
+    lens, qs = [640, 129, 333, 41, 1, 1000], [1, 3, 1, 1, 1, 2]
+    c = Case(34 + page, *layout, lens, qs, page, BF16)
+    table = c.table.copy()
+    for r, (n, q) in enumerate(zip(lens, qs)):
+        seen = [i for i in range(n) if i > n - q - window or i < first]
+        keep = {i // page for i in seen}
+        for p in range(table.shape[1]):
+            if p not in keep:
+                table[r, p] = -1 if (r + p) % 2 else 1 << 30
+    c.table, full = table, c.table
+    lens_d = dev(np.array(lens, np.int32))
+    got = W.kv_attention(ctx, c.cache(W), c.q, dev(c.cu), lens_d, dev(c.table), window=window, first=first)
+    ctx.sync()  # nothing recorded
+    want, smax, vmax = c.want(layout[2] ** -0.5, window, first)
+    assert (np.abs(got.double().cpu().numpy() - want) <= tolerance(want, smax, vmax, BF16)).all()
+    again = W.kv_attention(ctx, c.cache(W), c.q, dev(c.cu), lens_d, dev(full), window=window, first=first)
+    assert torch.equal(got, again)

@@ -238,11 +238,18 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       there = __ballot_sync(0xffffffffu, th);
       whole_seen = __ballot_sync(0xffffffffu, all);
     };
-    // uneven pages: block and row of one key
-    auto locate = [&](int key, long long& co, long long& so) {
+    // does any query see the key, which the list has in the group of its row u0
+    auto seen_by_any = [&](int u0, int key) {
+      return key < len && key <= p1 && (u0 < it.head ? key < it.lo : key >= it.from);
+    };
+    // Uneven pages: block and row of key j of the warp's group k.  The group's other keys
+    // may lie in pages that no query sees and the table need not have.
+    auto locate = [&](int k, int j, long long& co, long long& so) {
+      const int key = key0_of(k) + j;
+      const bool seen = seen_by_any((grp0 + k * kFewWarps) * kFewKeys, key);
       const int pg = kv_page_of(a.c, key);
-      int b = key < len ? table[pg] : -1;
-      if (key < len && (b < 0 || b >= a.c.blocks)) {
+      int b = seen ? table[pg] : -1;
+      if (seen && (b < 0 || b >= a.c.blocks)) {
         flag(a.status, WH_DEV_BADARG);
         b = -1;
       }
@@ -278,7 +285,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           long long co, so;
-          locate(key0_of(k) + g + 8 * j, co, so);
+          locate(k, g + 8 * j, co, so);
           kc[j].load(kbase + co);
 #pragma unroll
           for (int b = 0; b < kB; ++b) ksb[j][b] = __ldg(ksbase + so + b);
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           long long co, so;
-          if (locate(key0_of(k) + 2 * t + (j & 1) + 8 * (j >> 1), co, so)) have |= 1u << j;
+          if (locate(k, 2 * t + (j & 1) + 8 * (j >> 1), co, so)) have |= 1u << j;
           vc[j].load(vbase + co);
           vsb[j] = __ldg(vsbase + so);
         }
@@ -339,11 +346,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
       const int key0 = kv_key(it.head, it.start, u0);
       // every row of the group is there and seen by every query
       const bool full = whole_seen >> at & 1;
-      // does any query see the group's key j
-      auto seen_any = [&](int j) {
-        const int key = key0 + j;
-        return key < len && key <= p1 && (u0 < it.head ? key < it.lo : key >= it.from);
-      };
+      auto seen_any = [&](int j) { return seen_by_any(u0, key0 + j); };
       // ---- scores ----
       float s[2][4];
       uint32_t ksc[2][kB];
