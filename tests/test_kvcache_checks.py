@@ -1,0 +1,26 @@
+"""CPU checks of what the paged 4-bit cache refuses before anything reaches the GPU."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+def refused(W, kind, why, fn, *a, **kw):
+    with pytest.raises(W.WohperError) as e:
+        fn(*a, **kw)
+    assert e.value.kind == kind and why in str(e.value), e.value
+
+
+def test_a_pool_whose_blocks_lie_on_one_another_is_refused():
+    # a stride of 0 between several blocks is not a dense pool
+    import wohper_b200 as W
+
+    k = torch.zeros(1, 2, 5, 32, dtype=torch.uint8)
+    s = torch.zeros(1, 2, 5, 2, dtype=torch.uint8)
+    many = torch.zeros(3, 2, 5, 2, dtype=torch.uint8)
+    W.PagedKvCache(k, s)
+    W.PagedKvCache(k.expand(1, -1, -1, -1), s)
+    refused(W, "InvalidShape", "stride", W.PagedKvCache, k.expand(3, -1, -1, -1), many)
+    refused(W, "InvalidShape", "stride", W.PagedKvCache, torch.zeros(3, 2, 5, 32, dtype=torch.uint8),
+            s.expand(3, -1, -1, -1))

@@ -117,6 +117,9 @@ class PagedKvCache:
             _fail(_INVALID_SHAPE, "keys and values: one block stride")
         if b == 1:  # a stride means nothing where there is a single block
             step = scale_step = 0
+        elif step < h * p * half or scale_step < h * p * (half // 16):
+            # 0 (an expanded tensor) would read as a dense pool
+            _fail(_INVALID_SHAPE, "keys, scales: a block stride below a block's size")
         self._spec = KvCacheSpec(b, p, h, 2 * half, k.data_ptr(), ks.data_ptr(), _ptr(v), _ptr(vs),
                                  step, scale_step)
         self._ref = C.byref(self._spec)
