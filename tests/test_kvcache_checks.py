@@ -24,3 +24,15 @@ def test_a_pool_whose_blocks_lie_on_one_another_is_refused():
     refused(W, "InvalidShape", "stride", W.PagedKvCache, k.expand(3, -1, -1, -1), many)
     refused(W, "InvalidShape", "stride", W.PagedKvCache, torch.zeros(3, 2, 5, 32, dtype=torch.uint8),
             s.expand(3, -1, -1, -1))
+
+
+@pytest.mark.parametrize("name", ["keys", "key_scales", "values", "value_scales"])
+def test_a_pool_keeps_its_tensors(name):
+    # the calls use the addresses of construction: another tensor is another cache
+    import wohper_b200 as W
+
+    c = W.PagedKvCache.empty(2, 4, 1, 64, True, device="cpu")
+    old = getattr(c, name)
+    with pytest.raises(AttributeError):
+        setattr(c, name, torch.zeros_like(old))
+    assert getattr(c, name) is old

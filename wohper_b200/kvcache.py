@@ -78,13 +78,14 @@ def _on(stream):
 _HERE = contextlib.nullcontext()
 
 
-@dataclass
+@dataclass(frozen=True)
 class PagedKvCache:
     """A pool of blocks: uint8 CUDA tensors keys [blocks, kv_heads, page,
     head_dim / 2] and key_scales [blocks, kv_heads, page, head_dim / 32]; values
     and value_scales alike, or None where the values are the keys (a latent
     cache).  The outermost stride may be wider than dense (a layer's slice of a
-    pool that holds several); it must be the same for keys and values."""
+    pool that holds several); it must be the same for keys and values.  A cache
+    keeps the tensors that it was made of: other tensors are another cache."""
     keys: object
     key_scales: object
     values: Optional[object] = None
@@ -120,9 +121,10 @@ class PagedKvCache:
         elif step < h * p * half or scale_step < h * p * (half // 16):
             # 0 (an expanded tensor) would read as a dense pool
             _fail(_INVALID_SHAPE, "keys, scales: a block stride below a block's size")
-        self._spec = KvCacheSpec(b, p, h, 2 * half, k.data_ptr(), ks.data_ptr(), _ptr(v), _ptr(vs),
-                                 step, scale_step)
-        self._ref = C.byref(self._spec)
+        spec = KvCacheSpec(b, p, h, 2 * half, k.data_ptr(), ks.data_ptr(), _ptr(v), _ptr(vs), step,
+                           scale_step)
+        object.__setattr__(self, "_spec", spec)
+        object.__setattr__(self, "_ref", C.byref(spec))
 
     @classmethod
     def empty(cls, blocks: int, page: int, kv_heads: int, head_dim: int,
