@@ -556,7 +556,9 @@ wh_status wh_lm_head_topk_batch(wh_ctx* ctx, const uint16_t* weight, long long r
  * kv head.  A row of head_dim values is head_dim/2 bytes of E2M1 codes (OCP
  * values 0 0.5 1 1.5 2 3 4 6, low nibble = even column) and head_dim/32 UE8M0
  * scale bytes b: 2^(b-127), 0 for b = 0, and a block of 32 with b >= 253 reads
- * as NaN.  Slot s (0 <= s < blocks * page) is row s % page of block s / page. */
+ * as NaN.  Slot s (0 <= s < blocks * page) is row s % page of block s / page.
+ *   All pointers of the wh_kv_* calls are of the context's device, which has to be
+ * the current one (WH_ERR_CUDA otherwise). */
 typedef struct wh_kv_cache {
   int blocks, page, kv_heads, head_dim; /* head_dim: a multiple of 32, at most 512 */
   uint8_t* keys;         /* [blocks][kv_heads][page][head_dim/2], 16-byte aligned */

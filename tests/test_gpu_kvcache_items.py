@@ -112,3 +112,19 @@ def test_pages_that_no_query_sees_need_no_block(ctx, W, page, layout, window, fi
     assert (np.abs(got.double().cpu().numpy() - want) <= tolerance(want, smax, vmax, BF16)).all()
     again = W.kv_attention(ctx, c.cache(W), c.q, dev(c.cu), lens_d, dev(full), window=window, first=first)
     assert torch.equal(got, again)
+
+
+def test_a_context_of_another_gpu_is_refused(ctx, W):  # noqa: F811
+    class Other:
+        device, handle = ctx.device + 1, ctx.handle
+
+    cache = W.PagedKvCache.empty(4, 16, 1, 64)
+    slots, lens = torch.arange(2, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    table, q = torch.zeros(2, 2, dtype=torch.int32, device="cuda"), torch.zeros(2, 3, 64, device="cuda")
+    for call in (lambda: W.kv_append(Other, cache, slots, q[:, :1].contiguous()), lambda: W.kv_gather(Other, cache, slots),
+                 lambda: W.kv_attention(Other, cache, q, None, lens, table),
+                 lambda: W.kv_plan(Other, 16, lens, lens, table, slots.int(), lens[:1], 2)):
+        with pytest.raises(W.WohperError) as e:
+            call()
+        assert e.value.kind == "InvalidPointer"
+    ctx.sync()

@@ -413,7 +413,7 @@ wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, in
                           float scale, int window, int first, const float* sink, void* out,
                           long long out_token_stride, long long out_head_stride, void* scratch,
                           size_t scratch_bytes, wh_stream_t stream) {
-  if (!c) return fail(WH_ERR_INVALID_POINTER, "ctx is null");
+  if (wh_status st = kv_device_check(c)) return st;
   KvAttnArgs a{};
   if (wh_status st = kv_cache_check(cache, &a.c)) return st;
   int size;

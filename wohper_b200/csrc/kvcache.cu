@@ -442,6 +442,15 @@ wh_status kv_cache_check(const wh_kv_cache* c, KvCacheDev* out) {
   return WH_OK;
 }
 
+// The kernels launch on the current device, which has to be the context's.
+wh_status kv_device_check(const wh_ctx* c) {
+  if (!c) return fail(WH_ERR_INVALID_POINTER, "ctx is null");
+  int cur = -1;
+  WH_CUDA(cudaGetDevice(&cur));
+  if (cur != c->device) return fail(WH_ERR_CUDA, "the context's device is not the current device");
+  return WH_OK;
+}
+
 bool kv_dtype_size(int dtype, int* size) {
   *size = dtype == WH_DTYPE_F32 ? 4 : 2;
   return dtype == WH_DTYPE_F32 || dtype == WH_DTYPE_BF16 || dtype == WH_DTYPE_F16;
@@ -464,7 +473,7 @@ wh_status wh_kv_plan(wh_ctx* c, int requests, int page, int max_blocks, int toke
                      const int32_t* free_top, int32_t* free_top_out, int32_t* kv_lens_out,
                      int32_t* cu_q, int64_t* slots, int32_t* positions, int32_t* token_requests,
                      void* scratch, size_t scratch_bytes, wh_stream_t stream) {
-  if (!c) return fail(WH_ERR_INVALID_POINTER, "ctx is null");
+  if (wh_status st = kv_device_check(c)) return st;
   if (requests < 1 || page < 1 || max_blocks < 1)
     return fail(WH_ERR_EMPTY_SHAPE, "plan: requests, page, max_blocks");
   if (tokens < 0 || capacity < 0) return fail(WH_ERR_INVALID_SHAPE, "plan: tokens, capacity");
@@ -494,7 +503,7 @@ wh_status wh_kv_append(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots
                        const void* k, const void* v, int dtype, long long k_row_stride,
                        long long k_head_stride, long long v_row_stride, long long v_head_stride,
                        wh_stream_t stream) {
-  if (!c) return fail(WH_ERR_INVALID_POINTER, "ctx is null");
+  if (wh_status st = kv_device_check(c)) return st;
   KvAppendArgs a{};
   if (wh_status st = kv_cache_check(cache, &a.c)) return st;
   int size;
@@ -529,7 +538,7 @@ wh_status wh_kv_append(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots
 
 wh_status wh_kv_gather(wh_ctx* c, const wh_kv_cache* cache, const int64_t* slots, int rows,
                        void* k, void* v, int dtype, wh_stream_t stream) {
-  if (!c) return fail(WH_ERR_INVALID_POINTER, "ctx is null");
+  if (wh_status st = kv_device_check(c)) return st;
   KvGatherArgs a{};
   if (wh_status st = kv_cache_check(cache, &a.c)) return st;
   int size;

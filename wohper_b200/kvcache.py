@@ -63,6 +63,12 @@ def _dense(t, dtype, n, device, what: str) -> None:
     _fail(_INVALID_SHAPE, f"{what}: {n} dense elements")
 
 
+def _on_gpu(ctx: Context, device, what: str) -> None:
+    """Raises unless `device` is the context's GPU."""
+    if device.type != "cuda" or device.index != ctx.device:
+        _fail(_INVALID_POINTER, f"{what}: on {device}, not on the context's cuda:{ctx.device}")
+
+
 def _handle(stream, device) -> int:
     """The cudaStream_t of stream, or of the current stream (in one call of torch's)."""
     if stream is not None:
@@ -183,6 +189,7 @@ def kv_plan(ctx: Context, page: int, kv_lens, q_lens, block_table, free_blocks, 
     larger fixed one (a captured graph).  A step that does not fit changes
     nothing, gives no tokens, and ctx.sync() raises DeviceArg."""
     n, dev = kv_lens.numel(), kv_lens.device
+    _on_gpu(ctx, dev, "kv_lens")
     i32 = torch.int32
     _dense(kv_lens, i32, n, dev, "kv_lens")
     _dense(q_lens, i32, n, dev, "q_lens")
@@ -232,6 +239,7 @@ def kv_append(ctx: Context, cache: PagedKvCache, slots, keys, values=None, strea
     """Quantises keys (and values) [rows, kv_heads, head_dim], f32, bf16 or f16,
     into the cache's slots (int64 [rows]; negative: skipped)."""
     rows, dev = slots.numel(), cache.keys.device
+    _on_gpu(ctx, dev, "cache")
     _dense(slots, torch.int64, rows, dev, "slots")
     if (values is None) != (cache.values is None):
         _fail(_INVALID_POINTER, "values exactly when the cache has values")
@@ -251,6 +259,7 @@ def kv_gather(ctx: Context, cache: PagedKvCache, slots, dtype=None, stream=None)
     [rows, kv_heads, head_dim] of dtype (float32 by default); values is None for
     a cache whose values are its keys."""
     rows, dev = slots.numel(), cache.keys.device
+    _on_gpu(ctx, dev, "cache")
     _dense(slots, torch.int64, rows, dev, "slots")
     dtype = torch.float32 if dtype is None else dtype
     code = _dtype_code(dtype)
@@ -291,6 +300,7 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     scale defaults to head_dim ** -0.5.  Returns out, like q; out may be q itself,
     but may not overlap it in another way."""
     dev = cache.keys.device
+    _on_gpu(ctx, dev, "cache")
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         _fail(_INVALID_SHAPE, "q: [tokens, heads, head_dim]")
     code = _dtype_code(q.dtype)
