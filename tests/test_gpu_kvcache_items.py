@@ -128,3 +128,19 @@ def test_a_context_of_another_gpu_is_refused(ctx, W):  # noqa: F811
             call()
         assert e.value.kind == "InvalidPointer"
     ctx.sync()
+
+
+def test_a_scratch_that_is_not_dense_memory_of_the_gpu_is_refused(ctx, W):  # noqa: F811
+    cache = W.PagedKvCache.empty(4, 16, 2, 128, True)
+    lens, table = torch.ones(2, dtype=torch.int32, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 4, 128, device="cuda")
+    n = 1 << 24  # more than the call needs
+    for kind, scratch in (("InvalidPointer", torch.empty(n, dtype=torch.uint8)),
+                          ("InvalidShape", torch.empty(1, dtype=torch.uint8, device="cuda").expand(n)),
+                          ("InvalidShape", torch.empty(2 * n, dtype=torch.uint8, device="cuda")[::2])):
+        with pytest.raises(W.WohperError) as e:
+            W.kv_attention(ctx, cache, q, None, lens, table, scratch=scratch)
+        assert e.value.kind == kind
+    ok = torch.empty(n // 4, 4, dtype=torch.uint8, device="cuda")
+    assert W.kv_attention(ctx, cache, q, None, lens, table, scratch=ok).shape == q.shape
+    ctx.sync()

@@ -322,6 +322,8 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
         if scratch is None:
             scratch = torch.empty(_scratch_bytes(ctx, cache, tokens, heads, n, code),
                                   dtype=torch.uint8, device=dev)
+        else:
+            _dense(scratch, scratch.dtype, scratch.numel(), dev, "scratch")
     if out.shape != q.shape or out.dtype is not q.dtype or out.device != dev:
         _fail(_INVALID_SHAPE, "out: like q")
     q0, q1, q2 = q.stride()
