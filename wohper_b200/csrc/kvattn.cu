@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWo
   const int4 mt = mine ? w.meta[id] : make_int4(0, 1, 0, 0);
   const int parts = mt.y, row = mt.z >> 1;
   // a meta that the tensor-core kernel did not write: it gave up on a wait
-  const bool bad = mt.x < 0 || parts < 1 || mt.x + parts > w.ctas || row < 0 || row >= w.rn;
+  const bool bad = mt.x < 0 || parts < 1 || parts > w.ctas || mt.x > w.ctas - parts || row < 0 || row >= w.rn;
   if (bad) flag(a.status, WH_DEV_BADARG);
   auto slot_of = [&](int p) { return 2 * (mt.x + p) + (p == 0 ? mt.z & 1 : 0); };
   const float inf = __int_as_float(0x7f800000);
