@@ -605,8 +605,9 @@ wh_status wh_kv_plan(wh_ctx* ctx, int requests, int page, int max_blocks, int to
  * least power of two 2^k in [2^-126, 2^125] with max|x| <= 6 * 2^k (scale byte
  * 0 for an all-zero block, 255 where a value is not finite), codes rounded to
  * nearest, ties to even, saturated.  slots < 0 are skipped, slots past the pool
- * are skipped and recorded as WH_ERR_DEVICE_ARG; two rows with one slot leave
- * either.  v: the values' rows (NULL exactly when the cache's values are). */
+ * are skipped and recorded as WH_ERR_DEVICE_ARG.  Two rows with one slot leave
+ * its row undefined (codes of one may stand beside scales of the other).
+ * v: the values' rows (NULL exactly when the cache's values are). */
 wh_status wh_kv_append(wh_ctx* ctx, const wh_kv_cache* cache, const int64_t* slots, int rows,
                        const void* k, const void* v, int dtype, long long k_row_stride,
                        long long k_head_stride, long long v_row_stride, long long v_head_stride,

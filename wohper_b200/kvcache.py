@@ -237,7 +237,8 @@ def _row_strides(x, cache: PagedKvCache, rows: int, what: str):
 
 def kv_append(ctx: Context, cache: PagedKvCache, slots, keys, values=None, stream=None) -> None:
     """Quantises keys (and values) [rows, kv_heads, head_dim], f32, bf16 or f16,
-    into the cache's slots (int64 [rows]; negative: skipped)."""
+    into the cache's slots (int64 [rows]; negative: skipped; twice the same: its row
+    is undefined)."""
     rows, dev = slots.numel(), cache.keys.device
     _on_gpu(ctx, dev, "cache")
     _dense(slots, torch.int64, rows, dev, "slots")
