@@ -504,9 +504,18 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
         for (int k = 0; k < 4; ++k) {
           const uint32_t a0 = hmul2_u(b0[k], sc01), a1 = hmul2_u(b1[k], sc01);
           const uint32_t a2 = hmul2_u(b2[k], sc23), a3 = hmul2_u(b3[k], sc23);
+          if (kSplit) {
+            // A product of its own, added with rounding to nearest: a sum that runs through
+            // the tensor core loses half of its last place with each product, always downwards.
+            float z[4] = {0, 0, 0, 0};
+            mma_16816(z, a0, a1, a2, a3, pl[0], pl[1]);
+            mma_16816(z, a0, a1, a2, a3, pb[0][0], pb[0][1]);
 #pragma unroll
-          for (int u = 0; u < kNt; ++u) mma_16816(o[4 * i + k][u], a0, a1, a2, a3, pb[u][0], pb[u][1]);
-          if (kSplit) mma_16816(o[4 * i + k][0], a0, a1, a2, a3, pl[0], pl[1]);
+            for (int e = 0; e < 4; ++e) o[4 * i + k][0][e] += z[e];
+          } else {
+#pragma unroll
+            for (int u = 0; u < kNt; ++u) mma_16816(o[4 * i + k][u], a0, a1, a2, a3, pb[u][0], pb[u][1]);
+          }
         }
       }
       if (more) load_v(k + 1, at + 1);
