@@ -3,11 +3,13 @@ tiles: its error must not grow with the length.
 
 The tensor cores drop what lies below an f32 sum's last bit, so a sum that runs through
 many products shrinks: by half of the last place, 2^-24.5 of it, for each product of 16
-rows.  Bound on the signed error sum(err * sign(o)) / sum(|o|) with few query rows to a kv head:
-a score is a sum of head_dim / 16 products, which moves a weight by that many times
-2^-24.5 of the score; a group of 16 rows is one product of the weights' upper halves and
-one of the lower, added to f32 sums that round to nearest: 2^-24.5 * (2 + head_dim / 16 * S),
-S the largest |score|.
+rows.  Bounds on the signed error sum(err * sign(o)) / sum(|o|):
+ - few query rows: a score is a sum of head_dim / 16 products, which moves a weight by
+   that many times 2^-24.5 of the score; a group of 16 rows is one product of the weights'
+   upper halves and one of the lower, added to f32 sums that round to nearest:
+   2^-24.5 * (2 + head_dim / 16 * S), S the largest |score|;
+ - the tensor-core kernel: besides that, 4 products a tile over at most 32 tiles before
+   the sums are put aside: 2^-24.5 * (4 * 32 + head_dim / 16 * S).
 The scores are kept below 1, and the number of outputs (10^5 and more) leaves nothing of
 the errors without a sign."""
 from __future__ import annotations
@@ -51,9 +53,11 @@ def exact(cache, q, table, r):
     return (torch.softmax(s, -1) @ v).view(heads, d), float(s.abs().max())
 
 
-@pytest.mark.parametrize("layout,requests,rows", [((8, 8, 128, True), 64, 32768), ((32, 8, 64, False), 64, 32768),
-                                                  ((16, 2, 256, False), 64, 65536)], ids=str)
-def test_f32_sums_do_not_shrink_with_the_length(layout, requests, rows):
+@pytest.mark.parametrize("name,layout,requests,rows", [
+    ("few", (8, 8, 128, True), 64, 32768), ("few", (32, 8, 64, False), 64, 32768), ("few", (16, 2, 256, False), 64, 65536),
+    ("tc", (64, 1, 512, False), 48, 49152), ("tc", (64, 1, 128, True), 48, 49152), ("tc", (64, 2, 64, False), 64, 32768)],
+    ids=str)
+def test_f32_sums_do_not_shrink_with_the_length(name, layout, requests, rows):
     import wohper_b200 as W
 
     ctx = W.Context(0)
@@ -68,6 +72,6 @@ def test_f32_sums_do_not_shrink_with_the_length(layout, requests, rows):
         top += float(want.abs().sum())
         largest = max(largest, s)
     assert largest < 1
-    products = layout[2] / 16 * largest + 2
+    products = layout[2] / 16 * largest + (4 * 32 if name == "tc" else 2)
     assert abs(err / top) <= 2.0**-24.5 * products, (err / top, 2.0**-24.5 * products)
     ctx.close()

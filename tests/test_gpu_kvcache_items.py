@@ -7,6 +7,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from tests import kv_reference as R
 from tests.test_gpu_kvcache import BF16, F32, Case, ctx, dev, tolerance, W  # noqa: F401 (fixtures)
 
 torch = pytest.importorskip("torch")
@@ -144,3 +145,37 @@ def test_a_scratch_that_is_not_dense_memory_of_the_gpu_is_refused(ctx, W):  # no
     ok = torch.empty(n // 4, 4, dtype=torch.uint8, device="cuda")
     assert W.kv_attention(ctx, cache, q, None, lens, table, scratch=ok).shape == q.shape
     ctx.sync()
+
+
+@pytest.mark.parametrize("layout", [(26, 1, 64, False), (22, 1, 128, True), (3, 1, 512, False)], ids=str)
+@pytest.mark.parametrize("sink", [False, True], ids=["", "sink"])
+def test_items_of_more_tiles_than_a_sum_runs_through(ctx, W, layout, sink):  # noqa: F811
+    # 160 items of up to 47 tiles and two long ones: some in one CTA, some in several, sums
+    # put aside after 32 tiles; rows to be computed again because of the first, the last or a
+    # middle tile; a largest score that comes early, late, or not at all
+    lens = ([3000, 2049, 2048, 2900] * 40) + [9000, 12000]
+
+    def spoil(c):
+        for r, p in ((3, 0), (8, 100), (13, 180), (160, 0), (161, 700)):
+            c.scales[0][c.table[r, p], :, 2, 0] = 90
+        c.q[20, 1, 3] = float("inf")
+        for r, i in ((30, 5), (31, 2040), (32, 2999), (161, 11000)):
+            row = c.q[r, 0].float().cpu().numpy()
+            cc, ss = R.quantise(row * 2)
+            c.codes[0][c.table[r, i // 16], :, i % 16], c.scales[0][c.table[r, i // 16], :, i % 16] = cc, ss
+
+    c = Case(35, *layout, lens, [1] * len(lens), 16, F32, spoil=spoil)
+    args = (c.cache(W), c.q, dev(c.cu), dev(np.array(lens, np.int32)), dev(c.table))
+    kw = dict(sink=dev(c.sink) if sink else None)
+    got = W.kv_attention(ctx, *args, **kw)
+    for _ in range(3):
+        assert torch.equal(got.nan_to_num(), W.kv_attention(ctx, *args, **kw).nan_to_num())
+    q = c.q.clone()
+    W.kv_attention(ctx, args[0], q, *args[2:], **kw, out=q)
+    ctx.sync()
+    assert torch.equal(got.nan_to_num(), q.nan_to_num()) and torch.isnan(got[20, 1]).all()
+    c.q[20, 1] = 1.0  # its own row is not compared
+    want, smax, vmax = c.want(layout[2] ** -0.5, sink=c.sink if sink else None)
+    ratio = np.abs(got.double().cpu().numpy() - want) / np.maximum(tolerance(want, smax, vmax, F32), 1e-300)
+    ratio[20, 1] = 0
+    assert (ratio <= 1).all(), np.argwhere(~(ratio.max((1, 2)) <= 1)).ravel()

@@ -56,12 +56,14 @@ constexpr float kLift = 9.0f;  // weights are held as 2^(s - m + kLift) <= 2^15
 constexpr int kKvBias = 123;   // scale byte b stands for 2^(b - kKvBias) in the f16 tiles
 
 enum : int {
-  kFragFirst = 1,   // the CTA's first tile of this item
-  kFragLast = 2,    // the CTA's last tile of this item
+  kFragFirst = 1,   // the first tile of a fragment: a CTA's tiles of an item, at most kFold
+  kFragLast = 2,    // its last tile
   kTileMasked = 4,  // some row of the tile is not seen by every query
   kItemFirst = 8,   // the item's first tile is in this CTA
   kItemLast = 16,   // the item's last tile is in this CTA
-  kSlot1 = 32,      // partial slot 1 (the fragment does not begin the CTA's range)
+  kSlot1 = 32,      // partial slot 1 (the item does not begin the CTA's range)
+  kFragCut = 64,    // with kFragLast: the CTA goes on with the item in the next fragment
+  kFragCont = 128,  // the item's partial slot holds the sums of earlier fragments
 };
 
 struct KvTileInfo {
@@ -84,6 +86,13 @@ struct KvTc {
   static constexpr int kUnits = kD >= 128 ? kD / 128 : 1;
   static constexpr int kPer = kUnits > 1 ? kUnits / 2 : 1;
   static constexpr int kFillers = kUnits > 1 ? kTcDec : kTcDec / 2;  // warps that fill a tile
+  // Most tiles of a fragment (0: any number).  A sum that runs through the tensor core
+  // loses up to 2e-7 of itself with each tile, always downwards (values of one sign: 2.4e-4
+  // after 1300 tiles).  After 32 tiles f32 sums are added, in f32, to what the partial slot
+  // holds: at most 1.3e-6 whatever the length, for 11 % of the time at 32 x 32768 x 512 (331 us).
+  // 16-bit calls, where the code for it alone costs 2 %, keep on: the loss passes f16's
+  // own rounding after about 10^3 tiles a CTA (64 requests x 10^5 rows), bf16's after 10^4.
+  static constexpr int kFold = kSplit ? 32 : 0;
   static constexpr int kAhead = 1;  // tiles whose codes a decode warp has in flight: more spilled and lost
   static constexpr int kNh = kN / 2;                        // columns of a softmax half
   static constexpr int kRh = kRn / 2;                       // query rows of a softmax half
@@ -264,7 +273,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
     if (ntiles > 0) {
       KvWalk c(m.at);
       bool frag_first = true;
-      int slot1 = 0;
+      int slot1 = 0, cont = 0;
+      int run = 0;  // tiles of the fragment
       int key[2], blk[2];
       // this lane's two rows of tile jj: position (-1 past the last one seen) and block
       auto look_up = [&](int rr, const KvItem& x, int jj) {
@@ -284,7 +294,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         const long long at_ = c.at + w.lead;  // its tiles
         const KvItem x = c.it;
         const int ck[2] = {key[0], key[1]}, cb[2] = {blk[0], blk[1]};
-        const bool frag_last = c.j + 1 == c.it.tiles || n + 1 == ntiles;
+        const bool item_end = c.j + 1 == c.it.tiles || n + 1 == ntiles;  // of this CTA
+        const bool frag_last = item_end || (L::kFold && ++run == L::kFold);
         if (n + 1 < ntiles) {
           if (++c.j == c.it.tiles) c.next(a, w);
           look_up(c.r, c.it, c.j);
@@ -320,10 +331,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           f.u0 = j_ * kKvTile;
           f.flags = (frag_first ? kFragFirst : 0) | (frag_last ? kFragLast : 0) |
                     (all ? 0 : kTileMasked) | (at_ >= m.at.begin ? kItemFirst : 0) |
-                    (at_ + x.tiles <= m.at.end ? kItemLast : 0) | slot1;
+                    (at_ + x.tiles <= m.at.end ? kItemLast : 0) | slot1 | cont |
+                    (frag_last && !item_end ? kFragCut : 0);
         }
         frag_first = frag_last;
-        if (frag_last) slot1 = kSlot1;
+        if (frag_last) {
+          run = 0;
+          cont = item_end ? 0 : kFragCont;
+          if (item_end) slot1 = kSlot1;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.info_full[slot]);
       }
@@ -623,6 +639,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
     float fac[kMax], off[kMax], sum[kMax];
     uint32_t live = 0;  // bit e: the row has seen a key
     int frag = -1;
+    int redo = 0;  // the item's rows are to be computed again
     bool ok = true;
     for (int n = 0; n < ntiles; ++n) {
       const int slot = n % kTcInfo, b = n & 1;
@@ -778,18 +795,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         ok = product_done(n);
         tc::fence_after_sync();
         if (!bar_and(bar, 128, ok)) break;
-        const bool whole = (flags & kItemFirst) && (flags & kItemLast);
-        const int redo = m.redo[frag % kTcRedo];
+        const bool cut = L::kFold && (flags & kFragCut), cont = L::kFold && (flags & kFragCont);
+        const bool whole = (flags & kItemFirst) && (flags & kItemLast) && !cut;
+        redo = (cont ? redo : 0) | m.redo[frag % kTcRedo];
         const int rows = w.ht > 1 ? min(kRn, a.group - f.ht * kRn) : f.nt * a.group;
         const int row = half * kRh + quad * 32 + lane;
         if (quad * 32 + lane < kRh && row >= rows) m.out_row[row] = 0;
+        const int part = 2 * blockIdx.x + (flags & kSlot1 ? 1 : 0);
         if (quad * 32 + lane < kRh && row < rows) {
-          const int part = 2 * blockIdx.x + (flags & kSlot1 ? 1 : 0);
           const int h = f.kvh * a.group + f.ht * kRn + m.row_head[row];
           const int t = f.t0 + m.row_tok[row];
-          const float l = (m.red[1][0][row] + m.red[1][1][row]) + (m.red[1][2][row] + m.red[1][3][row]);
-          const float top = m.top[row];
+          float l = (m.red[1][0][row] + m.red[1][1][row]) + (m.red[1][2][row] + m.red[1][3][row]);
+          float top = m.top[row];
           float os = 1.0f / 16.0f;  // the tiles hold 16 times the values
+          float keep = 0.0f;        // by what the earlier fragments' sums are multiplied
+          if (cont) {  // this thread wrote them
+            const float2 x = w.part_ml[(long long)part * kRn + row];
+            const float to = fmaxf(top, x.x), base = to == -inf ? 0.0f : to;
+            const float now = top == -inf ? 0.0f : ex2(top - base);
+            keep = x.x == -inf ? 0.0f : ex2(x.x - base);
+            os *= now;
+            l = l * now + x.y * keep;
+            top = to;
+          }
           if (whole) {
             float z = l;
             if (a.sink) {
@@ -797,9 +825,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
               const float to = fmaxf(top, sk), base = to == -inf ? 0.0f : to;
               const float sh = top == -inf ? 0.0f : ex2(top - base);
               os *= sh;
+              keep *= sh;
               z = l * sh + ex2(sk - base + kLift);
             }
             os = z == 0.0f ? 0.0f : os / z;
+            keep = z == 0.0f ? 0.0f : keep / z;
             m.out_row[row] = t * a.out_token_stride + h * a.out_head_stride;
           } else {
             w.part_ml[(long long)part * kRn + row] = make_float2(top, l);
@@ -807,7 +837,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
             if (row == 0) w.part_redo[part] = redo;
           }
           m.out_scale[row] = os;
-          if (flags & kItemFirst) {  // where the item's parts lie
+          m.shrink[row] = keep;
+          if ((flags & kItemFirst) && !cut) {  // where the item's parts lie
             const int parts =
                 whole ? 1 : KvCut(w, m.at.total).cta_of(f.first + f.tiles - 1) - (int)blockIdx.x + 1;
             w.meta[(long long)t * a.heads + h] =
@@ -817,6 +848,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         if (!bar_and(bar, 128, ok)) break;
         const int dim = quad * 32 + lane;
         // eight rows at a time, a 128-row block of O^T after the other
+        auto sums = [&](int r0, int blk, float (&v)[8]) {
+          const uint32_t at = tmem_w + L::kTmemO + (r0 - half * kRh) * (kSplit ? 2 : 1) + blk * kN;
+          if (kSplit) {
+            uint32_t o[16];
+            tc::ld_32x32b_x16(at, o);
+            tc::wait_ld_of(o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[2 * e]) + __uint_as_float(o[2 * e + 1]);
+          } else {
+            uint32_t o[8];
+            tc::ld_32x32b_x8(at, o);
+            tc::wait_ld_of(o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[e]);
+          }
+        };
         auto write = [&](auto* out) {
           if (kD < 128 && quad * 32 >= kD) return;
 #pragma unroll 1
@@ -830,31 +877,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
               by[e] = m.out_scale[r0 + e];
             }
             const int live = rows - r0;
-            const uint32_t col = tmem_w + L::kTmemO + (r0 - half * kRh) * (kSplit ? 2 : 1);
 #pragma unroll 1
             for (int blk = 0; blk < L::kBlocks; ++blk) {
               float v[8];
-              if (kSplit) {
-                uint32_t o[16];
-                tc::ld_32x32b_x16(col + blk * kN, o);
-                tc::wait_ld_of(o);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[2 * e]) + __uint_as_float(o[2 * e + 1]);
-              } else {
-                uint32_t o[8];
-                tc::ld_32x32b_x8(col + blk * kN, o);
-                tc::wait_ld_of(o);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[e]);
-              }
+              sums(r0, blk, v);
 #pragma unroll
               for (int e = 0; e < 8; ++e)
                 if (e < live) kv_put(out + to[e] + blk * 128, v[e] * by[e]);
             }
           }
         };
+        // The same with what this thread has left in the partial slot, which goes on from
+        // there (f32 queries: so does the output).
+        auto add = [&](float* out) {
+          if (kD < 128 && quad * 32 >= kD) return;
+#pragma unroll 1
+          for (int r0 = half * kRh; r0 < half * kRh + kRh; r0 += 8) {
+            if (r0 >= rows) break;
+            const float* at = w.part_o + ((long long)part * kRn + r0) * kD + dim;
+            const int live = rows - r0;
+            float old[L::kBlocks][8];
+#pragma unroll
+            for (int blk = 0; blk < L::kBlocks; ++blk)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) old[blk][e] = e < live ? at[e * kD + blk * 128] : 0.0f;
+#pragma unroll
+            for (int blk = 0; blk < L::kBlocks; ++blk) {
+              float v[8];
+              sums(r0, blk, v);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (e < live)
+                  out[m.out_row[r0 + e] + dim + blk * 128] =
+                      fmaf(old[blk][e], m.shrink[r0 + e], v[e] * m.out_scale[r0 + e]);
+            }
+          }
+        };
         // rows to be computed again are left alone: out may be q, which that still reads
-        if (!whole) {
+        if (cont) {
+          if (!whole || !redo) add(whole ? static_cast<float*>(a.out) : w.part_o);
+        } else if (!whole) {
           write(w.part_o);
         } else if (!redo) {
           if (kSplit)
