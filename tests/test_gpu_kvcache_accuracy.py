@@ -75,3 +75,40 @@ def test_f32_sums_do_not_shrink_with_the_length(name, layout, requests, rows):
     products = layout[2] / 16 * largest + (4 * 32 if name == "tc" else 2)
     assert abs(err / top) <= 2.0**-24.5 * products, (err / top, 2.0**-24.5 * products)
     ctx.close()
+
+
+@pytest.mark.parametrize("layout", [(8, 2, 128, True), (64, 1, 128, True), (64, 2, 64, True), (40, 1, 512, True),
+                                    (6, 2, 96, True)], ids=str)
+@pytest.mark.parametrize("wide", [20, 26, 30])
+def test_f32_weights_far_below_the_largest_still_count(layout, wide):
+    # One row with a weight of 1 and the value 0 among rows whose weights are all
+    # e^-(0.75 wide) = 2^-21.6, 2^-28.1, 2^-32.5: the output is theirs alone.  A weight is the sum of two
+    # f16, the lower one held 2^11 times larger: at 2^9 times the weight the upper one is
+    # rounded to 2^-24 at the finest and the lower one to 2^-35, so that a weight of
+    # 2^-32.5 is off by at most 2^-36 of 2^-23.5, or 2^-12 of itself; the score's error
+    # (tests/test_gpu_kvcache.py) comes on top.
+    import numpy as np
+
+    import wohper_b200 as W
+    from tests import kv_reference as R
+    from tests.test_gpu_kvcache import F32, Case, dev
+
+    def spoil(c):
+        peak = np.zeros(layout[2])
+        peak[:wide] = 0.75
+        c.scales[0][:] = 0  # keys of zeros, but for one
+        b = c.table[0, 60 // 16]
+        c.codes[0][b, :, 60 % 16], c.scales[0][b, :, 60 % 16] = R.quantise(peak)
+        c.codes[1] &= 0x77
+        c.scales[1][b, :, 60 % 16] = 0
+        c.q = torch.ones_like(c.q)
+
+    ctx = W.Context(0)
+    c = Case(36, *layout, [900], [1], 16, F32, spoil=spoil)
+    got = W.kv_attention(ctx, c.cache(W), c.q, None, dev(np.array(c.lens, np.int32)), dev(c.table), scale=1.0)
+    ctx.sync()
+    want, smax, _ = c.want(1.0)
+    assert (want > 0).all()
+    ratio = np.abs(got.double().cpu().numpy() / want - 1)
+    assert (ratio <= 2.0**-12 + 2.0**-22 * (16 + 8 * smax.max())).all(), ratio.max()
+    ctx.close()

@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
           sum[u] += p0 + p1_;
           const __half2 h = __floats2half2_rn(p0, p1_);
           pb[u][j] = half2_bits(h);
-          if (kSplit) pl[j] = half2_bits(__floats2half2_rn(p0 - __low2float(h), p1_ - __high2float(h)));
+          if (kSplit) pl[j] = half2_bits(__floats2half2_rn((p0 - __low2float(h)) * kLoUp, (p1_ - __high2float(h)) * kLoUp));
         }
       // ---- O^T ----
       uint32_t sc[4];
@@ -509,6 +509,8 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
             // the tensor core loses half of its last place with each product, always downwards.
             float z[4] = {0, 0, 0, 0};
             mma_16816(z, a0, a1, a2, a3, pl[0], pl[1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] *= 1.0f / kLoUp;
             mma_16816(z, a0, a1, a2, a3, pb[0][0], pb[0][1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[4 * i + k][0][e] += z[e];

@@ -17,8 +17,9 @@
 // [2^14, 2^15) by a power of two; 16-bit queries are then one f16 exactly, f32
 // queries are the sum of two (kSplit: columns 2i and 2i + 1), which keeps 22
 // bits.  Weights are 2^(s - m + kLift) with a maximum m that may lag by kLag,
-// so at most 2^15: one f16 for 16-bit queries (11 bits), two for f32.  Sums are
-// f32.
+// so at most 2^15: one f16 for 16-bit queries (11 bits), two for f32, the lower
+// one times kLoUp: 22 bits down to 2^-23 of the largest weight, then one fewer
+// for each halving, nothing below 2^-45.  Sums are f32.
 //
 // Warps: 0-7 softmax and epilogue (TMEM lane quadrant warp % 4; warps 4-7 the
 // upper half of the columns), 8-23 decode, 24 MMA, 25 addresses (walks the work
@@ -52,6 +53,7 @@ constexpr int kTcRedo = 8;   // fragments whose redo marks are kept
 constexpr int kTcRing = 4;   // most tiles of keys (and of values) in shared memory
 constexpr int kTcCols = 64;  // columns of the products
 constexpr float kLag = 6.0f;   // log2 units that the running maximum may lag behind
+constexpr float kLoUp = 2048.0f;  // the lower f16 of an f32 weight is held times this: its last bit is 2^-35
 constexpr float kLift = 9.0f;  // weights are held as 2^(s - m + kLift) <= 2^15
 constexpr int kKvBias = 123;   // scale byte b stands for 2^(b - kKvBias) in the f16 tiles
 
@@ -769,7 +771,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           if (kSplit) {
             const float p = s[j][k];
             const __half hi = __float2half_rn(p);
-            bits = half2_bits(__halves2half2(hi, __float2half_rn(p - __half2float(hi))));
+            bits = half2_bits(__halves2half2(hi, __float2half_rn((p - __half2float(hi)) * kLoUp)));
           } else {
             bits = half2_bits(__floats2half2_rn(s[kSplit ? 0 : 2 * j][k], s[kSplit ? 0 : 2 * j + 1][k]));
           }
@@ -855,7 +857,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
             tc::ld_32x32b_x16(at, o);
             tc::wait_ld_of(o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[2 * e]) + __uint_as_float(o[2 * e + 1]);
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(__uint_as_float(o[2 * e + 1]), 1.0f / kLoUp, __uint_as_float(o[2 * e]));
           } else {
             uint32_t o[8];
             tc::ld_32x32b_x8(at, o);
