@@ -632,11 +632,17 @@ size_t wh_kv_attention_scratch_bytes(const wh_ctx* ctx, const wh_kv_cache* cache
  *   out [tokens][heads][head_dim] of q's dtype; strides in elements, rows of q
  * and out 16-byte aligned and contiguous.  out may be q itself (same address and
  * strides); it may not overlap q or another input in another way.  Rows of
- * tokens from cu_q[requests] on are not written.  Sums, maxima and normalisers
- * are f32; f32 queries give f32 accuracy.  Not-finite rows reach only the
+ * tokens from cu_q[requests] on are not written.  Not-finite rows reach only the
  * queries that see them.  Block ids outside the pool and lengths beyond
  * max_blocks * page are recorded as WH_ERR_DEVICE_ARG; such rows count as not
- * seen. */
+ * seen.
+ *   Sums, maxima and normalisers are f32.  Heads 64, 128, 256 and 512 wide are
+ * multiplied in f16 parts, which hold the cache's values exactly.  A 16-bit query
+ * is one part (exact down to 2^-28 of its row's largest element) and its weights
+ * have 11 bits.  An f32 query is two parts, 22 bits (fewer below 2^-16 of its
+ * row's largest element), as are its weights (down to 2^-23 of its row's largest
+ * weight); its outputs are as exact as those of f32 products.  Other widths are
+ * computed in f32 throughout. */
 wh_status wh_kv_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void* q, int dtype,
                           int tokens, int heads, long long q_token_stride,
                           long long q_head_stride, int requests, const int32_t* cu_q,

@@ -91,7 +91,7 @@ struct KvTc {
   // Most tiles of a fragment (0: any number).  A sum that runs through the tensor core
   // loses up to 2e-7 of itself with each tile, always downwards (values of one sign: 2.4e-4
   // after 1300 tiles).  After 32 tiles f32 sums are added, in f32, to what the partial slot
-  // holds: at most 1.3e-6 whatever the length, for 11 % of the time at 32 x 32768 x 512 (331 us).
+  // holds: 1.3e-6 to 2e-6 whatever the length, for 11 % of the time at 32 x 32768 x 512.
   // 16-bit calls, where the code for it alone costs 2 %, keep on: the loss passes f16's
   // own rounding after about 10^3 tiles a CTA (64 requests x 10^5 rows), bf16's after 10^4.
   static constexpr int kFold = kSplit ? 32 : 0;

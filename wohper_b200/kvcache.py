@@ -299,7 +299,10 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     query sits at position kv_lens[r] - 1.  A query at p sees rows i <= p and,
     with a window, only i > p - window or i < first.  sink: f32 [heads] or None.
     scale defaults to head_dim ** -0.5.  Returns out, like q; out may be q itself,
-    but may not overlap it in another way."""
+    but may not overlap it in another way.  Rows of tokens past cu_q[-1] are not
+    written: with out=None they hold whatever the memory held (all of them, after a
+    step that did not fit).  f32 queries give the accuracy of f32 products; weights
+    of 16-bit queries are held in 11 bits."""
     dev = cache.keys.device
     _on_gpu(ctx, dev, "cache")
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
