@@ -71,7 +71,7 @@ enum : int {
 struct KvTileInfo {
   int2 row[kKvTile];  // block (-1: not seen) and row in the block
   long long first;    // where the item's tiles begin on the line
-  int tiles, r, t0, nt, p0, kvh, ht, head, start, u0, flags;
+  int tiles, t0, nt, p0, kvh, ht, head, start, u0, flags;
 };
 
 template <int kD, bool kSplit>
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         const int slot = n % kTcInfo;
         if (n >= kTcInfo && !warp_wait(&m.info_empty[slot], ((n / kTcInfo) - 1) & 1, a.status)) break;
         // this tile's rows; the next tile's look-up starts before they are written down
-        const int r_ = c.r, j_ = c.j, kvh_ = c.kvh, ht_ = c.ht;
+        const int j_ = c.j, kvh_ = c.kvh, ht_ = c.ht;
         const long long at_ = c.at + w.lead;  // its tiles
         const KvItem x = c.it;
         const int ck[2] = {key[0], key[1]}, cb[2] = {blk[0], blk[1]};
@@ -322,7 +322,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         if (lane == 0) {
           f.first = at_;
           f.tiles = x.tiles;
-          f.r = r_;
           f.t0 = x.t0;
           f.nt = x.nt;
           f.p0 = x.p0;
