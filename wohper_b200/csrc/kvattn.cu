@@ -297,15 +297,21 @@ namespace {
 
 // Which kernel takes the call and how it cuts the queries.
 //  - few: a pass over the cache for every 16 query rows (8 of f32) of a kv head,
-//    nearly bound by its bytes;
+//    bound by latency (56 % of the issue slots, 40 % of the memory rate);
 //  - tc: one pass for 64 rows (32 of f32), bound by the tile pipeline;
-//  - row: a CTA a query row, for rows of other widths.
+//  - row: a CTA a query row, for rows of other widths (16 x 4096, 32 heads on 8 x 96,
+//    bf16: 202 us; 128 wide on the few-rows kernel 38).
 // Measured on 8 requests of 4096 rows, 8 kv heads, us (few / tc), rows to a kv head:
-//   64 wide,  bf16: 16 21/47, 32 31/48;                f32: 16 27/44, 24 37/45, 32 47/45
-//   128 wide, bf16: 16 26/47, 32 40/49, 48 54/48;      f32: 16 36/44, 32 62/45
-//   256 wide, bf16: 16 50/65, 32 74/66;                f32: 16 60/66, 32 99/66
+//   64 wide,  bf16: 16 20/47, 32 31/47, 48 39/47;         f32: 16 29/45, 24 40/46, 32 49/46
+//   128 wide, bf16: 16 26/47, 32 42/48, 40 55/48, 48 56/49; f32: 16 39/47, 24 53/47, 32 66/48
+//   256 wide, bf16: 16 50/65, 24 72/65, 32 74/66;         f32: 8 42/64, 16 66/66, 24 90/66
+// The limits lie in the pass above the crossing of such equal requests (128 wide 33-40
+// and f32 17-20 rows, 256 wide 17-24), which costs them up to 7 us here.
 // A call's tokens are taken as evenly spread over its requests, the one thing
-// the host knows; an item with fewer rows than it has room for is still right.
+// the host knows.  An item with fewer rows than it has room for is still right, but
+// where one request has most of the tokens the other requests, or it, get the kernel
+// that suits them less: 31 decodes x 4096 rows 66 us, a prompt of 512 tokens 49, both
+// in one call 184 (32 heads on 8 x 128, bf16).
 enum class KvWay { few, tc, row };
 struct KvHow {
   KvWay way;

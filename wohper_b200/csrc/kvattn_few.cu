@@ -1,8 +1,9 @@
 // kvattn_few.cu -- attention over the paged 4-bit cache for kv heads with few
 // query rows (decoding with grouped heads).
 //
-// With at most 16 rows a cache row gives so little work that the cache's bytes
-// bound the kernel; what must not happen is that decoding them costs more than
+// A pass takes 16 query rows (8 of f32) of a kv head; more rows, up to where the
+// tensor-core kernel is faster, take further passes.  With so few a cache row gives
+// little work; what must not happen is that decoding its codes costs more than
 // reading them.  So nothing passes through shared memory: a warp takes 16 rows
 // of the cache at a time and decodes its codes in registers straight into the
 // operands of mma.m16n8k16:
@@ -16,8 +17,9 @@
 // the CTA joins them when an item ends.
 //
 // Measured: 16 requests x 16384 rows, 8 kv heads x 128, 4 bf16 query rows each: 71
-// us with the join, 2.6 TB/s of codes, 56 % of the issue slots, about 410 warp
-// instructions for 16 rows of keys and values.
+// us with the join (f32: 77), 2.6 TB/s of codes, 56 % of the issue slots, about 410
+// warp instructions for 16 rows of keys and values.  Neither is full: with four warps a
+// scheduler it waits on its own loads and dependent instructions.
 //
 // f16 tiles, scales, query halves (kSplit: rows 8-15 of A are the low halves) and
 // rows to be computed again are as in kvattn_tc.cu.  kNt: groups of 8 query rows.
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
 
     const int p1 = it.p0 + it.nt - 1;
     const int len = kv_clip(a, c.len);
-    // groups of 16 rows of the item's list: this warp takes grp0, grp0 + 8, ...
+    // groups of 16 rows of the item's list: this warp takes grp0, grp0 + kFewWarps, ...
     const int past = min((c.j + n) * (kKvTile / kFewKeys), (it.seen + kFewKeys - 1) / kFewKeys);
     const int grp0 = c.j * (kKvTile / kFewKeys) + warp;
     const int groups = grp0 < past ? (past - grp0 + kFewWarps - 1) / kFewWarps : 0;

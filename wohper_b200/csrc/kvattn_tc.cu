@@ -14,9 +14,9 @@
 // 2^9; kept as 16 times the value, scale bytes 100..136).  Items that meet
 // another byte, a not-finite query or a not-finite block are marked and their
 // rows computed again in f32.  A query row is brought to a largest value in
-// [2^14, 2^15) by a power of two; 16-bit queries are then one f16 exactly, f32
-// queries are the sum of two (kSplit: columns 2i and 2i + 1), which keeps 22
-// bits.  Weights are 2^(s - m + kLift) with a maximum m that may lag by kLag,
+// [2^14, 2^15) by a power of two; 16-bit queries are then one f16 (exact, but for
+// elements below 2^-28 of the largest), f32 queries are the sum of two (kSplit:
+// columns 2i and 2i + 1), which keeps 22 bits down to 2^-16 of the largest.  Weights are 2^(s - m + kLift) with a maximum m that may lag by kLag,
 // so at most 2^15: one f16 for 16-bit queries (11 bits), two for f32, the lower
 // one times kLoUp: 22 bits down to 2^-23 of the largest weight, then one fewer
 // for each halving, nothing below 2^-45.  Sums are f32.
@@ -30,9 +30,11 @@
 //
 // Measured, 512 wide: decode 1.0-1.4 k cycles a tile, scores 1.15 k and sums 0.9 k
 // (both bound by the operands' shared-memory reads), softmax 1.7-2.5 k, two tiles
-// in flight: about 4 k cycles a tile; 32 requests x 8192 rows, 64 bf16 heads: 61 us
-// with the join, 32 x 4096 of f32 55 us.  M = 128 keys a product would
+// in flight: about 4 k cycles a tile; 32 requests x 8192 rows, 64 bf16 heads: 62 us
+// with the join, 32 x 4096 of f32 57 us.  M = 128 keys a product would
 // read 14 % fewer operand bytes but leave room for one tile only.
+// The forms whose values are the keys spill nothing; those with values of their own
+// 4-16 bytes, but for 16-bit queries of 256 columns.
 #include "kvattn.cuh"
 #include "tc.cuh"
 
