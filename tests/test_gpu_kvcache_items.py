@@ -179,3 +179,23 @@ def test_items_of_more_tiles_than_a_sum_runs_through(ctx, W, layout, sink):  # n
     ratio = np.abs(got.double().cpu().numpy() - want) / np.maximum(tolerance(want, smax, vmax, F32), 1e-300)
     ratio[20, 1] = 0
     assert (ratio <= 1).all(), np.argwhere(~(ratio.max((1, 2)) <= 1)).ravel()
+
+
+def test_numbers_past_32_bits_are_refused(ctx, W):  # noqa: F811
+    # the C calls take int: 2^32 + n would arrive as n
+    cache = W.PagedKvCache.empty(4, 16, 1, 64)
+    lens, table = torch.ones(2, dtype=torch.int32, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 3, 64, device="cuda")
+    free = torch.arange(4, dtype=torch.int32, device="cuda")
+    for n in (1 << 31, 1 << 32, (1 << 32) + 16, 1 << 63):
+        for call in (lambda: W.kv_attention(ctx, cache, q, None, lens, table, window=n),
+                     lambda: W.kv_attention(ctx, cache, q, None, lens, table, first=n),
+                     lambda: W.kv_plan(ctx, n, lens, lens, table, free, lens[:1], 2),
+                     lambda: W.kv_plan(ctx, 16, lens, lens, table, free, lens[:1], n)):
+            with pytest.raises(W.WohperError) as e:
+                call()
+            assert e.value.kind == "InvalidShape"
+    most = (1 << 31) - 1
+    a = W.kv_attention(ctx, cache, q, None, lens, table, window=most, first=most)
+    assert torch.equal(a, W.kv_attention(ctx, cache, q, None, lens, table))
+    ctx.sync()

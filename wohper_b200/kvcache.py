@@ -22,6 +22,7 @@ import torch
 from . import Context, WohperError, _check, _ptr, lib
 
 _INVALID_SHAPE, _INVALID_POINTER, _UNSUPPORTED = 2, 9, 10
+_INT_MAX = 0x7FFFFFFF  # ctypes would wrap what the C calls' int does not hold
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -203,8 +204,8 @@ def kv_plan(ctx: Context, page: int, kv_lens, q_lens, block_table, free_blocks, 
         if finished.dtype is not torch.uint8 and finished.dtype is not torch.bool:
             _fail(_UNSUPPORTED, "finished: uint8 or bool")
         _dense(finished, finished.dtype, n, dev, "finished")
-    if tokens < 0:
-        _fail(_INVALID_SHAPE, "tokens < 0")
+    if not 0 <= tokens <= _INT_MAX or not 0 <= page <= _INT_MAX:
+        _fail(_INVALID_SHAPE, f"tokens {tokens}, page {page}")
     with _on(stream):
         # lens | cu_q | top | positions | requests | scratch in one allocation, the slots in another
         ints = kv_lens.new_empty(3 * n + 2 + 2 * tokens)
@@ -320,6 +321,8 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     _dense(block_table, torch.int32, block_table.numel(), dev, "block_table")
     if sink is not None:
         _dense(sink, torch.float32, heads, dev, "sink")
+    if not 0 <= window <= _INT_MAX or not 0 <= first <= _INT_MAX:
+        _fail(_INVALID_SHAPE, f"window {window}, first {first}")
     with _on(stream):
         if out is None:
             out = torch.empty((tokens, heads, d), dtype=q.dtype, device=dev)
