@@ -199,3 +199,18 @@ def test_numbers_past_32_bits_are_refused(ctx, W):  # noqa: F811
     a = W.kv_attention(ctx, cache, q, None, lens, table, window=most, first=most)
     assert torch.equal(a, W.kv_attention(ctx, cache, q, None, lens, table))
     ctx.sync()
+
+
+def test_an_out_whose_rows_share_memory_is_refused(ctx, W):  # noqa: F811
+    cache = W.PagedKvCache.empty(4, 16, 1, 64)
+    lens, table = torch.ones(2, dtype=torch.int32, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 3, 64, device="cuda")
+    for out in (torch.empty(1, 3, 64, device="cuda").expand(2, 3, 64), torch.empty(2, 1, 64, device="cuda").expand(2, 3, 64)):
+        with pytest.raises(W.WohperError) as e:
+            W.kv_attention(ctx, cache, q, None, lens, table, out=out)
+        assert e.value.kind == "InvalidShape"
+    # where there is one token, one head, a stride means nothing; queries may share memory
+    one = torch.empty(1, 1, 64, device="cuda").expand(1, 1, 64)
+    W.kv_attention(ctx, cache, q[:1, :1].contiguous(), None, lens[:1], table[:1], out=one)
+    W.kv_attention(ctx, cache, q[:1].expand(2, 3, 64), None, lens, table)
+    ctx.sync()

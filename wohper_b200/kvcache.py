@@ -337,6 +337,8 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     o0, o1, o2 = out.stride()
     if q2 != 1 or o2 != 1:
         _fail(_INVALID_SHAPE, "q, out: contiguous rows")
+    if (tokens > 1 and o0 == 0) or (heads > 1 and o1 == 0):
+        _fail(_INVALID_SHAPE, "out: rows that share memory")
     if tokens == 1:  # a size-1 dimension's stride is free
         q0 = o0 = 0
     if heads == 1:
