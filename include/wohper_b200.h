@@ -70,6 +70,10 @@ typedef enum wh_status {
   WH_ERR_INVALID_EXPERT = 48   /* the layer has no expert with that id */
 } wh_status;
 
+#define WH_DTYPE_F32 0
+#define WH_DTYPE_BF16 1
+#define WH_DTYPE_F16 2
+
 /* ------------------------------------------------------------------------ */
 /* Context                                                                   */
 /* ------------------------------------------------------------------------ */
@@ -130,6 +134,34 @@ wh_status wh_fp8_gemv(wh_ctx* ctx, const uint8_t* weight, const uint8_t* scale, 
  * to the lower entry, in place. */
 wh_status wh_act_quant_fp8(wh_ctx* ctx, float* values, size_t n, int block_size,
                            wh_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* FP8 E4M3 x UE8M0(128x128) matrix product of many tokens                    */
+/* ------------------------------------------------------------------------ */
+/* Device scratch bytes of wh_fp8_gemm. */
+size_t wh_fp8_gemm_scratch_bytes(int cols, int tokens);
+/* The tensor-core form of wh_fp8_gemv with act_quant_block > 0, for any number
+ * of tokens (no reference counterpart: the reference runs a batch as GEMVs,
+ * src/compute.rs:6384-6577): y[t][r] = sum_c W[r][c] * aq(x[t])[c].
+ *   weight [rows][cols] E4M3 bytes, 16-byte aligned, cols % 16 == 0; scale
+ * [ceil(rows/128)][ceil(cols/128)] UE8M0 bytes b (2^(b-127); 255 is NaN), one
+ * per block of 128 x 128, the last ones ragged.  x [tokens] rows of `dtype`
+ * (WH_DTYPE_*), ldx elements apart, each on a 16-byte boundary; aq is
+ * wh_act_quant_fp8 over blocks of act_quant_block (32, 64 or 128) values of a
+ * row.  y [tokens] rows of rows values of y_dtype, ldy elements apart; may not
+ * overlap an input.
+ *   Operands are those of the GEMV bit for bit, but for what the tensor core
+ * reads otherwise: weight bytes 0x7F / 0xFF are NaN (the GEMV: +-480), a scale
+ * byte 0 is 2^-127 (the GEMV: 0).  A not-finite value of x makes its token's
+ * outputs NaN and no other's.  Sums are f32 in the tensor core's order: for an
+ * f32 y over 1024 columns at a time, which are then added in f32; for a 16-bit
+ * y over all of them.  Results repeat bit for bit.
+ *   All pointers are of the context's device, which has to be the current one
+ * (WH_ERR_CUDA otherwise). */
+wh_status wh_fp8_gemm(wh_ctx* ctx, const uint8_t* weight, const uint8_t* scale, int rows, int cols,
+                      int scale_rows, int scale_cols, const void* x, int dtype, int tokens,
+                      long long ldx, void* y, int y_dtype, long long ldy, int act_quant_block,
+                      void* scratch, size_t scratch_bytes, wh_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* FP4 E2M1 x UE8M0(per 32) matvec and expert forward                         */
@@ -570,10 +602,6 @@ typedef struct wh_kv_cache {
   long long block_stride, scale_block_stride;
 } wh_kv_cache;
 
-#define WH_DTYPE_F32 0
-#define WH_DTYPE_BF16 1
-#define WH_DTYPE_F16 2
-
 /* Device scratch bytes of wh_kv_plan. */
 size_t wh_kv_plan_scratch_bytes(int requests);
 /* The bookkeeping of one serving step, on the device.  Request r has kv_lens[r]
@@ -650,6 +678,76 @@ wh_status wh_kv_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void* q, 
                           float scale, int window, int first, const float* sink, void* out,
                           long long out_token_stride, long long out_head_stride, void* scratch,
                           size_t scratch_bytes, wh_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Trees of drafted tokens over the paged cache                               */
+/* ------------------------------------------------------------------------ */
+/* No reference counterpart.  A step that checks drafts gives request r the
+ * tokens cu_q[r] .. cu_q[r + 1] - 1 (as wh_kv_plan's cu_q), the nodes of a tree:
+ * parents[t] is the index inside the request of token t's parent, smaller than its
+ * own, or -1.  kv_lens[r] counts the n nodes' rows: node j's row is row base + j,
+ * base = kv_lens[r] - n, and its position base + its depth.  The step is
+ *   wh_kv_plan, wh_kv_tree, per layer wh_kv_append and wh_kv_tree_attention,
+ *   wh_kv_accept, per layer wh_kv_commit,
+ * in that order on one stream and without a host synchronisation.  max_nodes is at
+ * most 256. */
+
+/* masks [tokens][ceil(max_nodes/64)]: bit j of token t's is set where node j is t
+ * itself or an ancestor of it; positions [tokens].  Tokens of no request get no
+ * bits and position -1.  Recorded as WH_ERR_DEVICE_ARG: a parent outside [-1, own
+ * index) (taken as -1) and tokens past a request's first max_nodes, rounded up to
+ * a multiple of 64 (no bits, -1). */
+wh_status wh_kv_tree(wh_ctx* ctx, int requests, int tokens, int max_nodes, const int32_t* parents,
+                     const int32_t* cu_q, const int32_t* kv_lens, uint64_t* masks,
+                     int32_t* positions, wh_stream_t stream);
+/* wh_kv_attention with a tree's visibility: the query of a token at position p
+ * sees row i < base when window == 0, or i > p - window, or i < first, and row
+ * base + j when bit j of its mask is set (any mask, not only a tree's).  Positions
+ * count as if between base and kv_lens[r] - 1.  A window has to be at least
+ * max_nodes rounded up to a multiple of 64, so that it holds the tree.  The rest,
+ * its scratch (wh_kv_attention_scratch_bytes) and precision too, is
+ * wh_kv_attention's. */
+wh_status wh_kv_tree_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void* q, int dtype,
+                               int tokens, int heads, long long q_token_stride,
+                               long long q_head_stride, int requests, const int32_t* cu_q,
+                               const int32_t* kv_lens, const int32_t* block_table, int max_blocks,
+                               const uint64_t* masks, int max_nodes, const int32_t* positions,
+                               float scale, int window, int first, const float* sink, void* out,
+                               long long out_token_stride, long long out_head_stride,
+                               void* scratch, size_t scratch_bytes, wh_stream_t stream);
+/* What a step keeps.  drafts[t] is token t's id, targets[t] the id that the model
+ * puts after it (its best, or one sampled).  From node 0, which is always kept, the
+ * path goes on to the child of least index whose draft is its parent's target, as
+ * long as there is one: counts [requests] nodes, path [tokens] their indices at
+ * cu_q[r] + i (-1 past them and for tokens of no request), next_tokens [requests]
+ * the target of the last one.  kv_lens_out [requests] = base + counts; the blocks
+ * past it, which held the other nodes' rows, go on the stack in the order of
+ * requests and pages (block_table keeps its entries, which are no longer the
+ * request's).  A request without nodes gets 0, no path, -1 and its length.
+ *   Recorded as WH_ERR_DEVICE_ARG: a parent outside [-1, own index) (the node is on
+ * no path); a request with more than 256 nodes, a cu_q that does not fit tokens, or
+ * a length below its nodes or past max_blocks * page (treated as one without
+ * nodes); a stack height outside [0, capacity] or that would outgrow it (no request
+ * keeps anything, no block moves, lengths as they were).
+ *   kv_lens_out and free_top_out may not be their inputs. */
+wh_status wh_kv_accept(wh_ctx* ctx, int requests, int page, int max_blocks, int tokens,
+                       const int32_t* parents, const int32_t* drafts, const int32_t* targets,
+                       const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
+                       int32_t* free_blocks, int capacity, const int32_t* free_top,
+                       int32_t* free_top_out, int32_t* kv_lens_out, int32_t* counts,
+                       int32_t* path, int32_t* next_tokens, wh_stream_t stream);
+/* Moves the kept rows to their places: for i < counts[r], row base + path[i] of
+ * request r becomes its row base + i, codes and scales as they are, keys and values;
+ * every row is read before it is overwritten.  kv_lens is the step's (before
+ * wh_kv_accept).  To be called before the blocks that wh_kv_accept gave back are
+ * used again.  A pool that interleaves layers inside a block may be passed as one
+ * cache whose kv heads are the layers' kv heads.  A path that does not grow inside
+ * [i, n), or lengths that do not fit, leave the request as it is; a row in a block
+ * outside the pool is left out; both are recorded as WH_ERR_DEVICE_ARG. */
+wh_status wh_kv_commit(wh_ctx* ctx, const wh_kv_cache* cache, int requests, int tokens,
+                       const int32_t* counts, const int32_t* path, const int32_t* cu_q,
+                       const int32_t* kv_lens, const int32_t* block_table, int max_blocks,
+                       wh_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* ZCBLK01 tensor blocks (host memory; no device work)                        */

@@ -84,6 +84,8 @@ EXPORTS = (
     "wh_v4_attention_scratch_len", "wh_v4_attention", "wh_lm_head_batch_scratch_bytes",
     "wh_lm_head_topk_batch", "wh_kv_plan_scratch_bytes", "wh_kv_plan", "wh_kv_append",
     "wh_kv_gather", "wh_kv_attention_scratch_bytes", "wh_kv_attention",
+    "wh_fp8_gemm_scratch_bytes", "wh_fp8_gemm", "wh_kv_tree", "wh_kv_tree_attention",
+    "wh_kv_accept", "wh_kv_commit",
 )
 
 
@@ -211,6 +213,15 @@ def lib(build_if_missing: bool = True) -> C.CDLL:
         "wh_kv_attention_scratch_bytes": (sz, [vp, vp, i, i, i, i]),
         "wh_kv_attention": (st, [vp, vp, vp, i, i, i, C.c_longlong, C.c_longlong, i, vp, vp, vp,
                                  i, f, i, i, vp, vp, C.c_longlong, C.c_longlong, vp, sz, vp]),
+        "wh_fp8_gemm_scratch_bytes": (sz, [i, i]),
+        "wh_fp8_gemm": (st, [vp, vp, vp, i, i, i, i, vp, i, i, C.c_longlong, vp, i, C.c_longlong, i,
+                             vp, sz, vp]),
+        "wh_kv_tree": (st, [vp, i, i, i, vp, vp, vp, vp, vp, vp]),
+        "wh_kv_tree_attention": (st, [vp, vp, vp, i, i, i, C.c_longlong, C.c_longlong, i, vp, vp,
+                                      vp, i, vp, i, vp, f, i, i, vp, vp, C.c_longlong,
+                                      C.c_longlong, vp, sz, vp]),
+        "wh_kv_accept": (st, [vp, i, i, i, i] + [vp] * 7 + [i] + [vp] * 7),
+        "wh_kv_commit": (st, [vp, vp, i, i, vp, vp, vp, vp, vp, i, vp]),
         "wh_zcblk_parse": (st, [vp, sz, vp]),
         "wh_zcblk_tensor_at": (st, [vp, sz, C.c_uint32, vp]),
         "wh_zcblk_tensor_dim": (st, [vp, sz, vp, C.c_uint32, vp]),
@@ -330,6 +341,20 @@ def gemv_fp8_e4m3_ue8m0_tensorwise(ctx, weight, scale, input, output=None, act_q
                                    stream=None):
     return gemv_fp8_e4m3_ue8m0_rows(ctx, weight, scale, input, 0, weight.shape[0], output,
                                     act_quant_block, stream)
+
+
+def gemm_fp8_e4m3_ue8m0(ctx: Context, weight, scale, x, act_quant_block: int = 64, out_dtype=None,
+                        out=None, scratch=None, stream=None):
+    """The product of many tokens on the tensor cores (wh_fp8_gemm): weight uint8
+    [rows, cols] (E4M3; cols % 16 == 0) and scale uint8 [ceil(rows / 128),
+    ceil(cols / 128)] (UE8M0), both dense; x [tokens, cols] f32, bf16 or f16, whose
+    rows may lie apart (on 16 bytes).  x is quantised to E4M3 per act_quant_block
+    (32, 64 or 128) values of a row, as fp8_act_quant_dequant_in_place does.
+    Returns out [tokens, rows] of out_dtype (by default x's), f32 sums: those of the
+    GEMV in another order.  out may not overlap an input; its rows may lie apart."""
+    from . import fp8
+
+    return fp8.gemm(ctx, weight, scale, x, act_quant_block, out_dtype, out, scratch, stream)
 
 
 def fp8_act_quant_dequant_in_place(ctx, values, block_size: int = 64, stream=None):
@@ -805,6 +830,8 @@ class MoeLayer:
 # first use
 # --------------------------------------------------------------------------
 _KV_NAMES = ("KvPlan", "PagedKvCache", "kv_plan", "kv_append", "kv_gather", "kv_attention")
+# trees of drafted tokens over it (wohper_b200/kvtree.py)
+_TREE_NAMES = ("KvAccept", "KvTree", "kv_tree", "kv_tree_attention", "kv_accept", "kv_commit")
 
 
 def __getattr__(name: str):
@@ -812,5 +839,10 @@ def __getattr__(name: str):
         from . import kvcache
 
         globals().update({n: getattr(kvcache, n) for n in _KV_NAMES})
+        return globals()[name]
+    if name in _TREE_NAMES:
+        from . import kvtree
+
+        globals().update({n: getattr(kvtree, n) for n in _TREE_NAMES})
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -41,16 +41,17 @@ __device__ __forceinline__ float row_reduce_sum(float v, float* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-template <class T>
-__device__ void kv_attend_row(const KvAttnArgs& a, int r, int t, int h, KvRowSmem& sm) {
+template <class T, class Args>
+__device__ void kv_attend_row(const Args& a, int r, int t, int h, KvRowSmem& sm) {
   const int tid = threadIdx.x;
   const int D = a.c.head_dim, parts = D / 8;
   const int kvh = h / a.group;
   const int2 tq = kv_queries(a, r);
-  const int p = max(a.kv_lens[r], 0) - tq.y + (t - tq.x);
+  const int last = max(a.kv_lens[r], 0) - 1;
+  const int p = last + 1 - tq.y + (Args::kTree ? 0 : t - tq.x);  // of a tree: the first node's row
   const int n = kv_clip(a, a.kv_lens[r]);
   if (tid == 0 && n != a.kv_lens[r]) flag(a.status, WH_DEV_BADARG);
-  const KvSpan sp = kv_span(a, p, p, n);
+  const KvSpan sp = kv_span(a, p, Args::kTree ? last : p, n);
   const int seen = sp.head + sp.end - sp.start;
   const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_token_stride + h * a.q_head_stride;
   __syncthreads();
@@ -71,8 +72,10 @@ __device__ void kv_attend_row(const KvAttnArgs& a, int r, int t, int h, KvRowSme
     float s = -inf;
     int block = -1;
     long long row = 0;
-    if (u < seen) {
-      const int i = u < sp.head ? u : sp.start + (u - sp.head);
+    const int i = u < sp.head ? u : sp.start + (u - sp.head);
+    bool there = u < seen;
+    if constexpr (Args::kTree) there = there && kv_tree_sees(a, t, i, p, last);
+    if (there) {
       block = a.block_table[(long long)r * a.max_blocks + i / a.c.page];
       if (block < 0 || block >= a.c.blocks) {
         flag(a.status, WH_DEV_BADARG);
@@ -152,8 +155,8 @@ __device__ void kv_attend_row(const KvAttnArgs& a, int r, int t, int h, KvRowSme
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(KvAttnArgs a) {
+template <class T, class Args>
+__global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(Args a) {
   __shared__ KvRowSmem sm;
   pdl_wait_prior();
   const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
@@ -172,8 +175,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_attend_row_kernel(KvAttnArgs a
 // for 2048 rows in five parts, 8 for 64 rows in 148.
 // ---------------------------------------------------------------------------
 constexpr int kJoinParts = 640;  // most CTAs that a line is cut into
-template <class T, int kV, int kWpr>
-__global__ void __launch_bounds__(kRowThreads) kv_join_kernel(KvAttnArgs a, KvWork w) {
+template <class T, int kV, int kWpr, class Args>
+__global__ void __launch_bounds__(kRowThreads) kv_join_kernel(Args a, KvWork w) {
   __shared__ KvRowSmem sm;
   __shared__ int redo_row[4];
   __shared__ float red[4];
@@ -361,25 +364,25 @@ size_t kv_scratch(KvWork& w, int head_dim, int tokens, int heads, uint8_t* base)
   w.part_redo = reinterpret_cast<int*>(take(sizeof(int) * slots));
   return at;
 }
-template <int kD>
-cudaError_t kv_launch_tc(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool pdl) {
+template <int kD, class Args>
+cudaError_t kv_launch_tc(const Args& a, const KvHow& p, cudaStream_t s, bool pdl) {
   if (a.c.shared)
     return p.split ? launch_attend_tc<kD, true, false>(a, p.w, s, pdl)
                    : launch_attend_tc<kD, false, false>(a, p.w, s, pdl);
   return p.split ? launch_attend_tc<kD, true, true>(a, p.w, s, pdl)
                  : launch_attend_tc<kD, false, true>(a, p.w, s, pdl);
 }
-template <int kD>
-cudaError_t kv_launch_few(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool pdl) {
+template <int kD, class Args>
+cudaError_t kv_launch_few(const Args& a, const KvHow& p, cudaStream_t s, bool pdl) {
   if (p.split) return launch_attend_few<kD, 1, true>(a, p.w, s, pdl);
   return p.w.rn == 8 ? launch_attend_few<kD, 1, false>(a, p.w, s, pdl)
                      : launch_attend_few<kD, 2, false>(a, p.w, s, pdl);
 }
-template <class T>
-cudaError_t kv_launch(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool pdl) {
+template <class T, class Args>
+cudaError_t kv_launch(const Args& a, const KvHow& p, cudaStream_t s, bool pdl) {
   const unsigned rows = (unsigned)((long long)a.tokens * a.heads);
   if (p.way == KvWay::row)
-    return launch_pdl(kv_attend_row_kernel<T>, dim3(rows), kRowThreads, 0, s, pdl, a);
+    return launch_pdl(kv_attend_row_kernel<T, Args>, dim3(rows), kRowThreads, 0, s, pdl, a);
   const int d = a.c.head_dim;
   const cudaError_t e = p.way == KvWay::few ? (d == 256   ? kv_launch_few<256>(a, p, s, pdl)
                                                : d == 128 ? kv_launch_few<128>(a, p, s, pdl)
@@ -390,13 +393,13 @@ cudaError_t kv_launch(const KvAttnArgs& a, const KvHow& p, cudaStream_t s, bool 
                                    : kv_launch_tc<64>(a, p, s, pdl);
   if (e != cudaSuccess) return e;
   if (rows <= 4u * p.w.ctas)
-    return launch_pdl(kv_join_kernel<T, 1, 4>, dim3(rows, std::max(1, d / 128)), kRowThreads,
+    return launch_pdl(kv_join_kernel<T, 1, 4, Args>, dim3(rows, std::max(1, d / 128)), kRowThreads,
                       kJoinParts * sizeof(float2), s, pdl, a, p.w);
   const dim3 grid((rows + 3) / 4);
   const size_t smem = 4 * kJoinParts * sizeof(float2);
-  return d == 512   ? launch_pdl(kv_join_kernel<T, 4, 1>, grid, kRowThreads, smem, s, pdl, a, p.w)
-         : d == 256 ? launch_pdl(kv_join_kernel<T, 2, 1>, grid, kRowThreads, smem, s, pdl, a, p.w)
-                    : launch_pdl(kv_join_kernel<T, 1, 1>, grid, kRowThreads, smem, s, pdl, a, p.w);
+  return d == 512   ? launch_pdl(kv_join_kernel<T, 4, 1, Args>, grid, kRowThreads, smem, s, pdl, a, p.w)
+         : d == 256 ? launch_pdl(kv_join_kernel<T, 2, 1, Args>, grid, kRowThreads, smem, s, pdl, a, p.w)
+                    : launch_pdl(kv_join_kernel<T, 1, 1, Args>, grid, kRowThreads, smem, s, pdl, a, p.w);
 }
 
 }  // namespace
@@ -412,7 +415,12 @@ size_t wh_kv_attention_scratch_bytes(const wh_ctx* c, const wh_kv_cache* cache, 
   return p.way == KvWay::row ? 256 : kv_scratch(p.w, cache->head_dim, tokens, heads, nullptr);
 }
 
-wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, int dtype,
+}  // extern "C"
+
+namespace {
+// The checks and the launch that the two calls share; a comes with what is its own.
+template <class Args>
+wh_status kv_attend_call(Args a, wh_ctx* c, const wh_kv_cache* cache, const void* q, int dtype,
                           int tokens, int heads, long long q_token_stride,
                           long long q_head_stride, int requests, const int32_t* cu_q,
                           const int32_t* kv_lens, const int32_t* block_table, int max_blocks,
@@ -420,7 +428,6 @@ wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, in
                           long long out_token_stride, long long out_head_stride, void* scratch,
                           size_t scratch_bytes, wh_stream_t stream) {
   if (wh_status st = kv_device_check(c)) return st;
-  KvAttnArgs a{};
   if (wh_status st = kv_cache_check(cache, &a.c)) return st;
   int size;
   if (!kv_dtype_size(dtype, &size)) return fail(WH_ERR_UNSUPPORTED, "attention: dtype");
@@ -478,6 +485,47 @@ wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, in
   else
     WH_CUDA(kv_launch<__half>(a, p, s, c->pdl()));
   return WH_OK;
+}
+}  // namespace
+
+extern "C" {
+
+wh_status wh_kv_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, int dtype,
+                          int tokens, int heads, long long q_token_stride,
+                          long long q_head_stride, int requests, const int32_t* cu_q,
+                          const int32_t* kv_lens, const int32_t* block_table, int max_blocks,
+                          float scale, int window, int first, const float* sink, void* out,
+                          long long out_token_stride, long long out_head_stride, void* scratch,
+                          size_t scratch_bytes, wh_stream_t stream) {
+  return kv_attend_call(KvAttnArgs{}, c, cache, q, dtype, tokens, heads, q_token_stride, q_head_stride, requests,
+                        cu_q, kv_lens, block_table, max_blocks, scale, window, first, sink, out,
+                        out_token_stride, out_head_stride, scratch, scratch_bytes, stream);
+}
+
+wh_status wh_kv_tree_attention(wh_ctx* c, const wh_kv_cache* cache, const void* q, int dtype,
+                               int tokens, int heads, long long q_token_stride,
+                               long long q_head_stride, int requests, const int32_t* cu_q,
+                               const int32_t* kv_lens, const int32_t* block_table, int max_blocks,
+                               const uint64_t* masks, int max_nodes, const int32_t* positions,
+                               float scale, int window, int first, const float* sink, void* out,
+                               long long out_token_stride, long long out_head_stride,
+                               void* scratch, size_t scratch_bytes, wh_stream_t stream) {
+  if (!c) return fail(WH_ERR_INVALID_POINTER, "ctx is null");
+  if (max_nodes < 1) return fail(WH_ERR_EMPTY_SHAPE, "tree attention: max_nodes");
+  if (max_nodes > kTreeNodes) return fail(WH_ERR_UNSUPPORTED, "tree attention: max_nodes > 256");
+  const int words = (max_nodes + 63) / 64;
+  // then every ancestor lies inside the window of its descendants
+  if (window > 0 && window < 64 * words)
+    return fail(WH_ERR_UNSUPPORTED, "tree attention: a window shorter than the tree");
+  if (tokens > 0 && (!masks || !positions))
+    return fail(WH_ERR_INVALID_POINTER, "tree attention: null pointer");
+  KvTreeAttnArgs a{};
+  a.masks = reinterpret_cast<const uint32_t*>(masks);
+  a.words = 2 * words;
+  a.positions = positions;
+  return kv_attend_call(a, c, cache, q, dtype, tokens, heads, q_token_stride, q_head_stride, requests,
+                        cu_q, kv_lens, block_table, max_blocks, scale, window, first, sink, out,
+                        out_token_stride, out_head_stride, scratch, scratch_bytes, stream);
 }
 
 }  // extern "C"

@@ -6,6 +6,7 @@
 namespace wh {
 
 struct KvAttnArgs {
+  static constexpr bool kTree = false;
   KvCacheDev c;
   const void* q;
   void* out;
@@ -22,6 +23,26 @@ struct KvAttnArgs {
   const float* sink;
   uint32_t* status;
 };
+
+// The same for a step that checks a tree of drafted tokens: the request's n queries
+// are the tree's nodes and its last n rows theirs, rows base .. base + n - 1.  A
+// node sees the rows before base as a query at its own position does, and row
+// base + j where bit j of its mask is set.
+struct KvTreeAttnArgs : KvAttnArgs {
+  static constexpr bool kTree = true;
+  const uint32_t* masks;  // [tokens][words]
+  int words;
+  const int32_t* positions;
+};
+// Does the query of token tok see row i?  last: the request's last row.
+__device__ __forceinline__ bool kv_tree_sees(const KvTreeAttnArgs& a, int tok, int i, int base, int last) {
+  if (i >= base) {
+    const int j = i - base;
+    return j < 32 * a.words && (__ldg(a.masks + (long long)tok * a.words + (j >> 5)) >> (j & 31) & 1);
+  }
+  if (a.window == 0 || i < a.first) return true;
+  return i > min(max(__ldg(a.positions + tok), base), last) - a.window;
+}
 
 // The queries of request r, clipped to the call's tokens.
 __device__ __forceinline__ int2 kv_queries(const KvAttnArgs& a, int r) {
@@ -86,7 +107,7 @@ struct KvWork {
 
 struct KvItem {
   int t0, nt;  // its tokens
-  int p0;      // position of the first
+  int p0;      // position of the first; of a tree: the first node's row
   int lo, from;           // sees rows [0, lo) and [from, ...)
   int head, start, seen;  // its list: [0, head), [start, start + seen - head), from w.align multiples
   int tiles;
@@ -95,13 +116,14 @@ struct KvItem {
 __device__ __forceinline__ int kv_key(int head, int start, int u) {
   return u < head ? u : start + (u - head);
 }
-__device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, const KvWork& w, int len, int2 tq,
-                                          int i) {
+template <class Args>
+__device__ __forceinline__ KvItem kv_item(const Args& a, const KvWork& w, int len, int2 tq, int i) {
   KvItem it;
   it.t0 = tq.x + i * w.tt;
   it.nt = min(w.tt, tq.y - i * w.tt);
-  it.p0 = max(len, 0) - tq.y + i * w.tt;
-  const KvSpan s = kv_span(a, it.p0, it.p0 + it.nt - 1, kv_clip(a, len));
+  it.p0 = max(len, 0) - tq.y + (Args::kTree ? 0 : i * w.tt);
+  // a tree's positions lie between its first row and its last
+  const KvSpan s = kv_span(a, it.p0, Args::kTree ? max(len, 0) - 1 : it.p0 + it.nt - 1, kv_clip(a, len));
   it.lo = s.head;
   it.from = s.start;
   it.head = (s.head + w.align - 1) & -w.align;
@@ -151,8 +173,8 @@ struct KvPlace {
 };
 // Fills m; every thread of the CTA calls it.  A scan of the requests' units and
 // tiles; the thread whose request holds an end of the piece finds the place.
-template <int kThreads>
-__device__ __forceinline__ void kv_place(const KvAttnArgs& a, const KvWork& w, KvPlace& m) {
+template <int kThreads, class Args>
+__device__ __forceinline__ void kv_place(const Args& a, const KvWork& w, KvPlace& m) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int kWarps = kThreads / 32;
   // a request's length and tokens, its units and tiles
@@ -290,7 +312,8 @@ struct KvWalk {
   long long at;  // where the item begins on the line
   __device__ __forceinline__ explicit KvWalk(const KvPlace& p)
       : r(p.r), len(p.len), i(p.i), kvh(p.kvh), ht(p.ht), j(p.j), tq(p.tq), it(p.item), at(p.begin - p.into) {}
-  __device__ __forceinline__ void next(const KvAttnArgs& a, const KvWork& w) {
+  template <class Args>
+  __device__ __forceinline__ void next(const Args& a, const KvWork& w) {
     at += it.tiles + w.lead;
     j = 0;
     if (++ht < w.ht) return;

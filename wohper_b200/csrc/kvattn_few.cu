@@ -103,9 +103,9 @@ __device__ __forceinline__ uint32_t few_scale(uint32_t b, bool& lost) {
   }
   return (k >= -14 ? uint32_t(k + 15) << 10 : 1u << (k + 24)) * 0x10001u;
 }
-template <int kD, int kNt, bool kSplit>
+template <int kD, int kNt, bool kSplit, class Args>
 __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
-    kv_attend_few_kernel(KvAttnArgs a, KvWork w) {
+    kv_attend_few_kernel(Args a, KvWork w) {
   using L = KvFew<kD, kNt, kSplit>;
   constexpr int kRn = L::kRn, kSteps = L::kSteps;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
         for (int e = 0; e < 4; ++e) o[s][u][e] = 0.0f;
     }
 
-    const int p1 = it.p0 + it.nt - 1;
+    // the last position among the item's queries (at most, of a tree)
+    const int p1 = Args::kTree ? max(c.len, 0) - 1 : it.p0 + it.nt - 1;
     const int len = kv_clip(a, c.len);
     // groups of 16 rows of the item's list: this warp takes grp0, grp0 + kFewWarps, ...
     const int past = min((c.j + n) * (kKvTile / kFewKeys), (it.seen + kFewKeys - 1) / kFewKeys);
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
         th = b >= 0;
         lane_co = max(b, 0) * a.c.block_stride + (long long)in * (kD / 2);
         lane_so = max(b, 0) * a.c.scale_block_stride + (long long)in * (kD / 32);
-        all = th && key0 + kFewKeys - 1 <= min(it.p0, len - 1) &&
+        all = th && key0 + kFewKeys - 1 <= min(Args::kTree ? it.p0 - 1 : it.p0, len - 1) &&
               (u0 < it.head ? key0 + kFewKeys <= it.lo : key0 >= it.from) &&
               (a.window == 0 || key0 > p1 - a.window || key0 + kFewKeys <= a.first);
       }
@@ -420,9 +421,15 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
             const bool any = seen_any(jj) && (even ? there >> at & 1 : have >> (2 * j + e) & 1);
 #pragma unroll
             for (int u = 0; u < kNt; ++u) {
-              const int p = it.p0 + row_tok(g + 8 * u);
-              if (!(any && key <= p && (a.window == 0 || key > p - a.window || key < a.first)))
-                x[u][j][e] = -inf;
+              const int tok = row_tok(g + 8 * u);
+              bool seen = any;
+              if constexpr (Args::kTree) {  // rows past the item's repeat its last token
+                seen = seen && kv_tree_sees(a, it.t0 + min(tok, it.nt - 1), key, it.p0, p1);
+              } else {
+                const int p = it.p0 + tok;
+                seen = seen && key <= p && (a.window == 0 || key > p - a.window || key < a.first);
+              }
+              if (!seen) x[u][j][e] = -inf;
             }
           }
       }
@@ -620,13 +627,13 @@ __global__ void __launch_bounds__(kFewThreads, KvFew<kD, kNt, kSplit>::kCtas)
   pdl_launch_dependents();
 }
 
-template <int kD, int kNt, bool kSplit>
-static cudaError_t launch_attend_few(const KvAttnArgs& a, const KvWork& w, cudaStream_t s, bool pdl) {
+template <int kD, int kNt, bool kSplit, class Args>
+static cudaError_t launch_attend_few(const Args& a, const KvWork& w, cudaStream_t s, bool pdl) {
   using L = KvFew<kD, kNt, kSplit>;
   if (w.rn != L::kRn) return cudaErrorInvalidValue;
-  const cudaError_t e = ensure_smem(kv_attend_few_kernel<kD, kNt, kSplit>, L::kBytes);
+  const cudaError_t e = ensure_smem(kv_attend_few_kernel<kD, kNt, kSplit, Args>, L::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kv_attend_few_kernel<kD, kNt, kSplit>, dim3(w.ctas), kFewThreads, L::kBytes, s, pdl, a, w);
+  return launch_pdl(kv_attend_few_kernel<kD, kNt, kSplit, Args>, dim3(w.ctas), kFewThreads, L::kBytes, s, pdl, a, w);
 }
 
 }  // namespace wh

@@ -74,6 +74,7 @@ struct KvTileInfo {
   int2 row[kKvTile];  // block (-1: not seen) and row in the block
   long long first;    // where the item's tiles begin on the line
   int tiles, t0, nt, p0, kvh, ht, head, start, u0, flags;
+  int last;  // of a tree: the request's last row
 };
 
 template <int kD, bool kSplit>
@@ -218,8 +219,8 @@ __device__ __forceinline__ void kv_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void kv_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void kv_put(__half* p, float v) { *p = __float2half_rn(v); }
 
-template <int kD, bool kSplit, bool kSep>
-__global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs a, KvWork w) {
+template <int kD, bool kSplit, bool kSep, class Args>
+__global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(Args a, KvWork w) {
   using L = KvTc<kD, kSplit>;
   using Misc = typename L::Misc;
   constexpr int kN = kTcCols, kRn = L::kRn, kNh = L::kNh, kRh = L::kRh;
@@ -297,6 +298,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         const int j_ = c.j, kvh_ = c.kvh, ht_ = c.ht;
         const long long at_ = c.at + w.lead;  // its tiles
         const KvItem x = c.it;
+        const int last = Args::kTree ? max(c.len, 0) - 1 : 0;
         const int ck[2] = {key[0], key[1]}, cb[2] = {blk[0], blk[1]};
         const bool item_end = c.j + 1 == c.it.tiles || n + 1 == ntiles;  // of this CTA
         const bool frag_last = item_end || (L::kFold && ++run == L::kFold);
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
         }
         KvTileInfo& f = m.info[slot];
         bool all = true;
-        const int p1 = x.p0 + x.nt - 1;
+        const int p1 = Args::kTree ? last : x.p0 + x.nt - 1;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           int b = cb[k];
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           }
           if (ck[k] < 0) b = -1;
           const int row = b < 0 ? 0 : kvh_ * a.c.page + (ck[k] - kv_page_of(a.c, ck[k]) * a.c.page);
-          all = all && b >= 0 && ck[k] <= x.p0 &&
+          all = all && b >= 0 && (Args::kTree ? ck[k] < x.p0 : ck[k] <= x.p0) &&
                 (a.window == 0 || ck[k] > p1 - a.window || ck[k] < a.first);
           f.row[lane + 32 * k] = make_int2(b, row);
         }
@@ -332,6 +334,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           f.head = x.head;
           f.start = x.start;
           f.u0 = j_ * kKvTile;
+          if (Args::kTree) f.last = last;
           f.flags = (frag_first ? kFragFirst : 0) | (frag_last ? kFragLast : 0) |
                     (all ? 0 : kTileMasked) | (at_ >= m.at.begin ? kItemFirst : 0) |
                     (at_ + x.tiles <= m.at.end ? kItemLast : 0) | slot1 | cont |
@@ -687,8 +690,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
           const bool real = f.row[key0 + 8 * k].x >= 0;
 #pragma unroll
           for (int e = 0; e < kMax; ++e) {
-            const int p = f.p0 + m.row_tok[row_of(e)];
-            const bool seen = real && i <= p && (a.window == 0 || i > p - a.window || i < a.first);
+            const int tok = m.row_tok[row_of(e)];
+            bool seen = real;
+            if constexpr (Args::kTree) {  // rows past the item's repeat its last token
+              seen = seen && kv_tree_sees(a, f.t0 + min(tok, f.nt - 1), i, f.p0, f.last);
+            } else {
+              const int p = f.p0 + tok;
+              seen = seen && i <= p && (a.window == 0 || i > p - a.window || i < a.first);
+            }
             if (!seen) s[e][k] = -inf;
           }
         }
@@ -944,13 +953,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attend_tc_kernel(KvAttnArgs 
   if (warp == kTcMma) tc::tmem_dealloc(tmem, L::kTmemCols);
 }
 
-template <int kD, bool kSplit, bool kSep>
-static cudaError_t launch_attend_tc(const KvAttnArgs& a, const KvWork& w, cudaStream_t s, bool pdl) {
+template <int kD, bool kSplit, bool kSep, class Args>
+static cudaError_t launch_attend_tc(const Args& a, const KvWork& w, cudaStream_t s, bool pdl) {
   const size_t smem = KvTcSmem<kD, kSplit, kSep>::kBytes;
   if (w.rn != KvTc<kD, kSplit>::kRn) return cudaErrorInvalidValue;
-  const cudaError_t e = ensure_smem(kv_attend_tc_kernel<kD, kSplit, kSep>, smem);
+  const cudaError_t e = ensure_smem(kv_attend_tc_kernel<kD, kSplit, kSep, Args>, smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kv_attend_tc_kernel<kD, kSplit, kSep>, dim3(w.ctas), kTcThreads, smem, s, pdl, a, w);
+  return launch_pdl(kv_attend_tc_kernel<kD, kSplit, kSep, Args>, dim3(w.ctas), kTcThreads, smem, s, pdl, a, w);
 }
 
 }  // namespace wh

@@ -304,6 +304,13 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     written: with out=None they hold whatever the memory held (all of them, after a
     step that did not fit).  f32 queries give the accuracy of f32 products; weights
     of 16-bit queries are held in 11 bits."""
+    return _attend(ctx, cache, q, cu_q, kv_lens, block_table, scale, window, first, sink, out,
+                   scratch, stream)
+
+
+def _attend(ctx, cache, q, cu_q, kv_lens, block_table, scale, window, first, sink, out, scratch,
+            stream, masks=None, positions=None):
+    """kv_attention; with masks [tokens, words] and positions [tokens] kv_tree_attention."""
     dev = cache.keys.device
     _on_gpu(ctx, dev, "cache")
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
@@ -321,6 +328,11 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
     _dense(block_table, torch.int32, block_table.numel(), dev, "block_table")
     if sink is not None:
         _dense(sink, torch.float32, heads, dev, "sink")
+    if masks is not None:
+        if masks.dim() != 2 or masks.shape[0] != tokens or not 1 <= masks.shape[1] <= 4:
+            _fail(_INVALID_SHAPE, "masks: [tokens, 1 to 4 words]")
+        _dense(masks, torch.int64, masks.numel(), dev, "masks")
+        _dense(positions, torch.int32, tokens, dev, "positions")
     if not 0 <= window <= _INT_MAX or not 0 <= first <= _INT_MAX:
         _fail(_INVALID_SHAPE, f"window {window}, first {first}")
     with _on(stream):
@@ -343,10 +355,13 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
         q0 = o0 = 0
     if heads == 1:
         q1 = o1 = 0
-    _check(lib().wh_kv_attention(ctx.handle, cache._ref, q.data_ptr(), code, tokens, heads, q0, q1,
-                                 n, _ptr(cu_q), kv_lens.data_ptr(), block_table.data_ptr(),
-                                 block_table.shape[1], d ** -0.5 if scale is None else scale,
-                                 window, first, _ptr(sink), out.data_ptr(), o0, o1,
-                                 scratch.data_ptr(), scratch.numel() * scratch.element_size(),
-                                 _handle(stream, dev)))
+    call, tree = lib().wh_kv_attention, ()
+    if masks is not None:
+        call = lib().wh_kv_tree_attention
+        tree = (masks.data_ptr(), 64 * masks.shape[1], positions.data_ptr())
+    _check(call(ctx.handle, cache._ref, q.data_ptr(), code, tokens, heads, q0, q1, n, _ptr(cu_q),
+                kv_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], *tree,
+                d ** -0.5 if scale is None else scale, window, first, _ptr(sink), out.data_ptr(),
+                o0, o1, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+                _handle(stream, dev)))
     return out
