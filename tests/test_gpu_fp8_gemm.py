@@ -92,6 +92,21 @@ def test_sizes(ctx, W, rows, cols, tokens):
     check(y, real, quantised(x, block), dtype)
 
 
+@pytest.mark.parametrize("rows,cols,tokens", [(100, 20496, 3), (100, 20496, 30), (100, 20496, 140), (19200, 2560, 3),
+                                              (19200, 2560, 30), (19200, 2560, 140), (640, 12288, 3), (640, 12288, 140),
+                                              (1300, 1168, 4500), (2048, 512, 5000), (300, 144, 20000),
+                                              (4096, 256, 8192)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_long_sums(ctx, W, rows, cols, tokens, dtype):
+    # many sums of 1024 columns to a tile, alone in it and shared by a cluster
+    rng = np.random.default_rng(rows)
+    w, s, real = weight(rng, rows, cols)
+    x = inputs(rng, tokens, cols, dtype)
+    y = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x)
+    ctx.sync()
+    check(y, real, quantised(x, 64), dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
 @pytest.mark.parametrize("out_dtype", [F32, BF16, F16], ids=str)
 @pytest.mark.parametrize("tokens", [5, 200])
@@ -249,6 +264,6 @@ def test_refusals_and_no_tokens(ctx, W):
     refused(W, "InvalidShape", ctx, w, s, x, out=torch.empty(4, 131, device="cuda"))
     refused(W, "InvalidShape", ctx, w, s, x, out=torch.empty(130, device="cuda").expand(4, 130))
     refused(W, "Unsupported", ctx, w, s, x, out_dtype=BF16, out=torch.empty(4, 130, device="cuda"))
-    refused(W, "ScratchTooSmall", ctx, w, s, x, scratch=torch.empty(100, dtype=torch.uint8, device="cuda"))
+    refused(W, "ScratchTooSmall", ctx, w, s, x.repeat(3, 1), scratch=torch.empty(100, dtype=torch.uint8, device="cuda"))
     assert W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x[:0]).shape == (0, 130)
     ctx.sync()

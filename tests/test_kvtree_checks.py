@@ -58,10 +58,13 @@ def test_gemm_scratch_holds_codes_and_scale_tiles():
     import wohper_b200 as W
 
     size = W.lib().wh_fp8_gemm_scratch_bytes
-    assert size(0, 4) == size(16, 0) == size(-1, -1) == 0
-    for cols, tokens in ((16, 1), (4096, 1), (1360, 257), (8192, 100000)):
-        tiles = -(-tokens // 256) * 2 * -(-cols // 128)
-        assert size(cols, tokens) >= tokens * cols + tiles * 512
+    # few tokens are quantised by the product itself
+    assert size(0, 9) == size(16, 0) == size(-1, -1) == size(4096, 1) == size(4096, 2) == 0
+    for cols, tokens in ((16, 5), (1360, 257), (8192, 100000)):
+        ktiles = -(-cols // 128)
+        for tile, block in ((16, 512), (32, 512), (64, 512), (128, 512), (224, 1024)):
+            if tile >= 128 or tokens <= tile:
+                assert size(cols, tokens) >= tokens * cols + -(-tokens // tile) * ktiles * block
     assert size(32768, 1 << 20) > 1 << 35  # past 32 bits
 
 

@@ -293,6 +293,9 @@ struct wh_ctx {
   int device = 0;
   int num_sms = 148;
   uint32_t* status = nullptr;    // device word: WH_DEV_* bits
+  // device, 512 times each byte value: the scales of a 128 x 128 block of an FP8 weight,
+  // as the tensor core's scale copies read them
+  uint8_t* sf_rows = nullptr;
   uint32_t* counters = nullptr;  // device, router last-CTA counters (zero at rest)
   int counters_len = 0;
   uint32_t* blk_counters = nullptr;  // device, moe_up act-quant block counters (zero at rest)
@@ -408,20 +411,26 @@ wh_status wh_ctx_create(int device, wh_ctx** out) {
   cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, device);
   cudaError_t e = cudaMalloc(&c->status, sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMemset(c->status, 0, sizeof(uint32_t));
+  if (e == cudaSuccess) e = cudaMalloc(&c->sf_rows, 256 * 512);
+  for (int b = 0; b < 256 && e == cudaSuccess; ++b) e = cudaMemsetAsync(c->sf_rows + b * 512, b, 512);
   if (e != cudaSuccess) {
+    cudaFree(c->status);
+    cudaFree(c->sf_rows);
     delete c;
-    return cuda_fail(e, "status word");
+    return cuda_fail(e, "status word, scale rows");
   }
   set_act_quant_table(act_quant_table_host(), nullptr);
   cudaError_t te = cudaSuccess;
   if (!install_expf_table(&te)) {
     cudaFree(c->status);
+    cudaFree(c->sf_rows);
     delete c;
     return fail(WH_ERR_UNSUPPORTED, "host expf differs outside the device's midpoint gate");
   }
   e = te != cudaSuccess ? te : cudaDeviceSynchronize();
   if (e != cudaSuccess) {
     cudaFree(c->status);
+    cudaFree(c->sf_rows);
     delete c;
     return cuda_fail(e, "act quant table upload");
   }
@@ -435,6 +444,7 @@ void wh_ctx_destroy(wh_ctx* c) {
   for (auto& kv : c->experts) free_expert_set(kv.second);
   for (auto e : c->ev) cudaEventDestroy(e);
   if (c->status) cudaFree(c->status);
+  if (c->sf_rows) cudaFree(c->sf_rows);
   if (c->counters) cudaFree(c->counters);
   if (c->blk_counters) cudaFree(c->blk_counters);
   if (c->work) cudaFree(c->work);

@@ -40,9 +40,10 @@ __device__ __forceinline__ uint64_t desc_sf_block(uint32_t smem_addr) {
   return d;
 }
 // kind::mxf8f6f4 block-scaled instruction descriptor: A and B E4M3, K-major,
-// UE8M0 scales, M = 128, N = n (multiple of 8 up to 256), scale bytes sfa/sfb.
-__host__ __device__ __forceinline__ uint32_t idesc_mxf8(int n, uint32_t sfa, uint32_t sfb) {
-  return (sfb & 3u) << 4 | (uint32_t(n) >> 3) << 17 | 1u << 23 | (128u >> 4) << 24 |
+// UE8M0 scales, M = m (256: a pair of CTAs), N = n (multiple of 8 up to 256), scale
+// bytes sfa/sfb.
+__host__ __device__ __forceinline__ uint32_t idesc_mxf8(int n, uint32_t sfa, uint32_t sfb, int m = 128) {
+  return (sfb & 3u) << 4 | (uint32_t(n) >> 3) << 17 | 1u << 23 | (uint32_t(m) >> 4) << 24 |
          (sfa & 3u) << 29;
 }
 
@@ -173,6 +174,45 @@ __device__ __forceinline__ void wait_ld_of(uint32_t (&v)[kCount]) {
   for (int i = 0; i < kCount; ++i) asm volatile("" : "+r"(v[i])::"memory");
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+
+// ---- pairs of CTAs (cta_group::2) ----
+// The even CTA of the pair issues; A's rows and D's lie half in each CTA, B's rows
+// half in each CTA's shared memory; each CTA's TMEM holds the scales of its own rows
+// of A and of all of B, copied from its own shared memory.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   smem_u32(dst_smem)),
+               "r"(ncols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
+               : "memory");
+}
+__device__ __forceinline__ void cp_sf_block_pair(uint32_t taddr, uint64_t src_desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(src_desc)
+               : "memory");
+}
+__device__ __forceinline__ void mma_mxf8_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                              uint32_t tsfa, uint32_t tsfb, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p; }"
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(tsfa), "r"(tsfb)
+      : "memory");
+}
+// commit that arrives on the barrier at the same place in both CTAs
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
 
 }  // namespace tc
 }  // namespace wh
