@@ -343,20 +343,6 @@ def gemv_fp8_e4m3_ue8m0_tensorwise(ctx, weight, scale, input, output=None, act_q
                                     act_quant_block, stream)
 
 
-def gemm_fp8_e4m3_ue8m0(ctx: Context, weight, scale, x, act_quant_block: int = 64, out_dtype=None,
-                        out=None, scratch=None, stream=None):
-    """The product of many tokens on the tensor cores (wh_fp8_gemm): weight uint8
-    [rows, cols] (E4M3; cols % 16 == 0) and scale uint8 [ceil(rows / 128),
-    ceil(cols / 128)] (UE8M0), both dense; x [tokens, cols] f32, bf16 or f16, whose
-    rows may lie apart (on 16 bytes).  x is quantised to E4M3 per act_quant_block
-    (32, 64 or 128) values of a row, as fp8_act_quant_dequant_in_place does.
-    Returns out [tokens, rows] of out_dtype (by default x's), f32 sums: those of the
-    GEMV in another order.  out may not overlap an input; its rows may lie apart."""
-    from . import fp8
-
-    return fp8.gemm(ctx, weight, scale, x, act_quant_block, out_dtype, out, scratch, stream)
-
-
 def fp8_act_quant_dequant_in_place(ctx, values, block_size: int = 64, stream=None):
     _check(lib().wh_act_quant_fp8(ctx.handle, _ptr(values), values.numel(), block_size,
                                   _stream(stream)))
@@ -839,6 +825,11 @@ def __getattr__(name: str):
         from . import kvcache
 
         globals().update({n: getattr(kvcache, n) for n in _KV_NAMES})
+        return globals()[name]
+    if name == "gemm_fp8_e4m3_ue8m0":  # wohper_b200/fp8.py
+        from . import fp8
+
+        globals()[name] = fp8.gemm_fp8_e4m3_ue8m0
         return globals()[name]
     if name in _TREE_NAMES:
         from . import kvtree

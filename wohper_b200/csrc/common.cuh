@@ -120,6 +120,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t phase, uint32_
   return true;
 }
 
+// The same by a whole warp, whose lanes stay together: the branches depend on votes
+// alone.  After a wait with a loop of each lane's own the compiler does not know the
+// warp to be converged, keeps the operands of the copies and products that follow in
+// ordinary registers, and each of them takes about a hundred cycles to issue.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t phase, uint32_t* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) return true;
+  const uint64_t start = globaltimer();
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, phase))) {
+    if (__any_sync(0xffffffffu, globaltimer() - start > WH_WAIT_NS)) {
+      if ((threadIdx.x & 31) == 0) flag(status, WH_DEV_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+
 // Producer drain before it leaves the kernel: a bounded wait that gives up at
 // once when a wait of this launch sequence has already timed out, so a failed
 // kernel returns after one timeout instead of one per ring stage.  A copy that

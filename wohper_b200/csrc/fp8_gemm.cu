@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     for (int kt = k0; kt < k1; ++kt, ++g, at.next()) {
       const int s = at.s;
       const uint32_t byte = sc.at(kt);
-      if (g >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&m.empty[s], at.phase ^ 1, a.status));
+      if (g >= kStages) ok = mbar_wait_warp(&m.empty[s], at.phase ^ 1, a.status);
       if (!ok) break;
       if (tc::elect_one()) {
         mbar_arrive_expect_tx(&m.full[s], kMmWeight + 512);
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     const uint8_t* sf = a.xsf + (long long)(tile / a.mtiles) * a.ktiles * 512;
     for (int kt = k0; kt < k1; ++kt, ++g, at.next()) {
       const int s = at.s;
-      if (g >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&m.empty[s], at.phase ^ 1, a.status));
+      if (g >= kStages) ok = mbar_wait_warp(&m.empty[s], at.phase ^ 1, a.status);
       if (!ok) break;
       if (tc::elect_one()) {
         mbar_arrive_expect_tx(&m.full[s], L::kTokens + L::kSfb);
@@ -386,14 +386,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     bool ok = true;
     for (int c0 = k0; ok && c0 < k1; c0 += a.fold, ++chunk) {
       const int b = chunk % kAcc;
-      if (chunk >= kAcc) ok = __all_sync(0xffffffffu, mbar_wait(&m.acc_empty[b], ((chunk / kAcc) - 1) & 1, a.status));
+      if (chunk >= kAcc) ok = mbar_wait_warp(&m.acc_empty[b], ((chunk / kAcc) - 1) & 1, a.status);
       if (!ok) break;
       tc::fence_after_sync();
       const uint32_t acc = tmem + b * kN;
       const int c1 = min(k1, c0 + a.fold);
       for (int kt = c0; kt < c1; ++kt, at.next()) {
         const int s = at.s;
-        ok = __all_sync(0xffffffffu, mbar_wait(&m.full[s], at.phase, a.status));
+        ok = mbar_wait_warp(&m.full[s], at.phase, a.status);
         if (!ok) break;
         tc::fence_after_sync();
         if (tc::elect_one()) {
@@ -458,9 +458,9 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         // (A phase is told from the next but one only by one who has seen it end.)
         static_assert(kMmEpi == 2 * L::kStages || !kQuant, "two fills between a warp's own");
         if (ok && g >= 2 * kStages)
-          ok = __all_sync(0xffffffffu, mbar_wait(&m.empty[s], (g / kStages) & 1, a.status));
+          ok = mbar_wait_warp(&m.empty[s], (g / kStages) & 1, a.status);
         if (ok && g >= kStages)
-          ok = __all_sync(0xffffffffu, mbar_wait(&m.empty[s], ((g / kStages) - 1) & 1, a.status));
+          ok = mbar_wait_warp(&m.empty[s], ((g / kStages) - 1) & 1, a.status);
         if (!ok) break;
         for (int p = 0; 2 * p < a.tokens; ++p) {
           const int t = 2 * p + (lane >> 4);
@@ -566,7 +566,7 @@ __device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// mbar_wait on a barrier that the other CTA of the cluster arrives on
+// mbar_wait_warp on a barrier that the other CTA of the cluster arrives on
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t phase) {
   uint32_t ok;
   asm volatile(
@@ -577,12 +577,12 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t ph
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t phase, uint32_t* status) {
-  if (mbar_try_wait_cluster(bar, phase)) return true;
+__device__ __forceinline__ bool mbar_wait_warp_cluster(uint64_t* bar, uint32_t phase, uint32_t* status) {
+  if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, phase))) return true;
   const uint64_t start = globaltimer();
-  while (!mbar_try_wait_cluster(bar, phase)) {
-    if (globaltimer() - start > WH_WAIT_NS) {
-      flag(status, WH_DEV_TIMEOUT);
+  while (!__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, phase))) {
+    if (__any_sync(0xffffffffu, globaltimer() - start > WH_WAIT_NS)) {
+      if ((threadIdx.x & 31) == 0) flag(status, WH_DEV_TIMEOUT);
       return false;
     }
   }
@@ -654,7 +654,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmThreads, 1)
       for (int kt = 0; kt < a.ktiles; ++kt, ++g, at.next()) {
         const int s = at.s;
         const uint32_t byte = sc.at(kt);
-        if (g >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&m.empty[s], at.phase ^ 1, a.status));
+        if (g >= kStages) ok = mbar_wait_warp(&m.empty[s], at.phase ^ 1, a.status);
         if (!ok) break;
         if (tc::elect_one()) {
           // the other CTA's bytes may be counted before they are announced; the phase ends after both
@@ -685,7 +685,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmThreads, 1)
       const int n0 = tile / mpairs * kN;
       for (int kt = 0; kt < a.ktiles; ++kt, ++g, at.next()) {
         const int s = at.s;
-        if (g >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&m.empty[s], at.phase ^ 1, a.status));
+        if (g >= kStages) ok = mbar_wait_warp(&m.empty[s], at.phase ^ 1, a.status);
         if (!ok) break;
         if (tc::elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&m.full[s], 2 * (L::kTokens + L::kSfb));
@@ -709,14 +709,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmThreads, 1)
         for (int c0 = 0; ok && c0 < a.ktiles; c0 += a.fold, ++chunk) {
           const int b = chunk % kAcc;
           if (chunk >= kAcc)
-            ok = __all_sync(0xffffffffu, mbar_wait_cluster(&m.acc_empty[b], ((chunk / kAcc) - 1) & 1, a.status));
+            ok = mbar_wait_warp_cluster(&m.acc_empty[b], ((chunk / kAcc) - 1) & 1, a.status);
           if (!ok) break;
           tc::fence_after_sync();
           const uint32_t acc = tmem + b * kN;
           const int c1 = min(a.ktiles, c0 + a.fold);
           for (int kt = c0; kt < c1; ++kt, at.next()) {
             const int s = at.s;
-            ok = __all_sync(0xffffffffu, mbar_wait_cluster(&m.full[s], at.phase, a.status));
+            ok = mbar_wait_warp_cluster(&m.full[s], at.phase, a.status);
             if (!ok) break;
             tc::fence_after_sync();
             if (tc::elect_one()) {

@@ -189,7 +189,12 @@ __device__ __forceinline__ void kv_place(const Args& a, const KvWork& w, KvPlace
     q.len = a.kv_lens[r];
     q.tq = kv_queries(a, r);
     int items = 0;
-    for (int i = 0; i * w.tt < q.tq.y; ++i, ++items) q.tiles += kv_item(a, w, q.len, q.tq, i).tiles;
+    if (Args::kTree) {  // a tree's items see the same rows
+      items = (q.tq.y + w.tt - 1) / w.tt;
+      if (items > 0) q.tiles = (long long)kv_item(a, w, q.len, q.tq, 0).tiles * items;
+    } else {
+      for (int i = 0; i * w.tt < q.tq.y; ++i, ++items) q.tiles += kv_item(a, w, q.len, q.tq, i).tiles;
+    }
     q.units = (q.tiles + (long long)items * w.lead) * (a.c.kv_heads * w.ht);
     q.tiles *= a.c.kv_heads * w.ht;
     if (q.tq.y > 0 && kv_clip(a, q.len) != q.len) flag(a.status, WH_DEV_BADARG);
@@ -201,7 +206,14 @@ __device__ __forceinline__ void kv_place(const Args& a, const KvWork& w, KvPlace
     const int per = a.c.kv_heads * w.ht;  // items of the same tokens
     int i = 0;
     KvItem it = kv_item(a, w, q.len, q.tq, 0);
-    while (off >= (long long)(it.tiles + w.lead) * per) {
+    if (Args::kTree) {
+      const long long each = (long long)(it.tiles + w.lead) * per;
+      i = int(off / each);
+      off -= i * each;
+      tiles += (long long)i * it.tiles * per;
+      if (i > 0) it = kv_item(a, w, q.len, q.tq, i);
+    }
+    while (!Args::kTree && off >= (long long)(it.tiles + w.lead) * per) {
       off -= (long long)(it.tiles + w.lead) * per;
       tiles += (long long)it.tiles * per;
       it = kv_item(a, w, q.len, q.tq, ++i);
