@@ -138,7 +138,7 @@ wh_status wh_act_quant_fp8(wh_ctx* ctx, float* values, size_t n, int block_size,
 /* ------------------------------------------------------------------------ */
 /* FP8 E4M3 x UE8M0(128x128) matrix product of many tokens                    */
 /* ------------------------------------------------------------------------ */
-/* Device scratch bytes of wh_fp8_gemm. */
+/* Device scratch bytes of wh_fp8_gemm; 0 for one or two tokens (scratch may be null). */
 size_t wh_fp8_gemm_scratch_bytes(int cols, int tokens);
 /* The tensor-core form of wh_fp8_gemv with act_quant_block > 0, for any number
  * of tokens (no reference counterpart: the reference runs a batch as GEMVs,
@@ -154,8 +154,8 @@ size_t wh_fp8_gemm_scratch_bytes(int cols, int tokens);
  * reads otherwise: weight bytes 0x7F / 0xFF are NaN (the GEMV: +-480), a scale
  * byte 0 is 2^-127 (the GEMV: 0).  A not-finite value of x makes its token's
  * outputs NaN and no other's.  Sums are f32 in the tensor core's order: for an
- * f32 y over 1024 columns at a time, which are then added in f32; for a 16-bit
- * y over all of them.  Results repeat bit for bit.
+ * f32 y over 1024 columns at a time (32768 for a 16-bit y), which are then added
+ * in f32.  Results repeat bit for bit.
  *   All pointers are of the context's device, which has to be the current one
  * (WH_ERR_CUDA otherwise). */
 wh_status wh_fp8_gemm(wh_ctx* ctx, const uint8_t* weight, const uint8_t* scale, int rows, int cols,
@@ -690,7 +690,7 @@ wh_status wh_kv_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void* q, 
  *   wh_kv_plan, wh_kv_tree, per layer wh_kv_append and wh_kv_tree_attention,
  *   wh_kv_accept, per layer wh_kv_commit,
  * in that order on one stream and without a host synchronisation.  max_nodes is at
- * most 256. */
+ * most 256, tokens at most 2^30. */
 
 /* masks [tokens][ceil(max_nodes/64)]: bit j of token t's is set where node j is t
  * itself or an ancestor of it; positions [tokens].  Tokens of no request get no

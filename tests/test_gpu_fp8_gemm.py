@@ -107,6 +107,59 @@ def test_long_sums(ctx, W, rows, cols, tokens, dtype):
     check(y, real, quantised(x, 64), dtype)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 16), (129, 144), (4096, 2064), (300, 20496), (19200, 2560)])
+@pytest.mark.parametrize("tokens", [1, 2])
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, F32), (F32, F16), (BF16, BF16), (F16, F32)], ids=str)
+def test_one_and_two_tokens(ctx, W, rows, cols, tokens, dtype, out_dtype):
+    # quantised inside the product; 19200 rows leave no CTAs to share a tile's K
+    rng = np.random.default_rng(rows)
+    block = (32, 64, 128)[(rows + tokens) % 3]
+    w, s, real = weight(rng, rows, cols)
+    wide = torch.zeros(tokens, 2 * cols, dtype=dtype, device="cuda")
+    x = wide[:, cols:]
+    x.copy_(inputs(rng, tokens, cols, dtype))
+    y = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x, block, out_dtype)
+    z = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x.contiguous(), block, out_dtype)
+    ctx.sync()
+    check(y, real, quantised(x, block), out_dtype)
+    assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("tokens", [1, 2])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_one_of_two_tokens_that_is_not_finite(ctx, W, tokens, bad):
+    rng = np.random.default_rng(8)
+    w, s, real = weight(rng, 300, 1040)
+    w[w == 0] = 1
+    x = inputs(rng, tokens, 1040, F32)
+    clean = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x)
+    for t in range(tokens):
+        z = x.clone()
+        z[t, 1039] = bad
+        y = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, z)
+        keep = torch.arange(tokens, device="cuda") != t
+        assert y[t].isnan().all() and torch.equal(y[keep], clean[keep])
+    ctx.sync()
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_very_long_rows(ctx, W, tokens, out_dtype):
+    # positive terms, whose sums a tensor core rounds down; added in f32 after 1024 columns
+    # for f32 and 32768 for 16-bit outputs: 2^-24 of the sum for each instruction before
+    rng = np.random.default_rng(9)
+    w, s, _ = weight(rng, 130, 98320)
+    w &= 127
+    real = e4m3(w.cpu().numpy()) * np.repeat(np.repeat(2.0 ** (s.cpu().numpy() - 127.0), 128, 0)[:130], 128, 1)[:, :98320]
+    x = inputs(rng, tokens, 98320, F32).abs() * 2.0**-10
+    y = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x, 64, out_dtype)
+    ctx.sync()
+    want = quantised(x, 64) @ real.T
+    steps = (32 if out_dtype == F32 else 1024) + 98320 / 1024 / 4
+    err = np.abs(y.double().cpu().numpy() - want)
+    assert (err <= np.abs(want) * (2.0**-22 * steps + UNIT[out_dtype])).all(), float((err / want).max())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
 @pytest.mark.parametrize("out_dtype", [F32, BF16, F16], ids=str)
 @pytest.mark.parametrize("tokens", [5, 200])

@@ -16,8 +16,8 @@
 // equal bytes in the tensor core's layout, copied from a table of 256 such rows.
 //
 // Measured, quantisation included (inputs of three calls in turn): 8192 tokens x 4096 x
-// 8192 in bf16 309 us (1780 TFLOP/s), in f32 322; 509 in bf16 35 us; one token x 4096 x
-// 4096 8.1 us.  The quantisation of 8192 x 8192 f32 is 51 us of it, at the copy's rate.  Without
+// 8192 in bf16 280 to 309 us (1780 to 1960 TFLOP/s), in f32 313 to 322; 509 in bf16 29 us; one
+// token x 4096 x 4096 8.1 us.  The quantisation of 8192 x 8192 f32 is 51 us of it, at the copy's rate.  Without
 // any product the loads of the large one alone take 226 us of 250: 10.6 TB/s from L2 to the
 // SMs, which 224 x 256 outputs for 31 KB of operands a CTA and K tile leave as its bound.
 #include <cuda_bf16.h>
@@ -107,8 +107,9 @@ constexpr int kMmMma = kMmEpi, kMmWeights = kMmEpi + 1, kMmTokens = kMmEpi + 2;
 constexpr int kMmThreads = (kMmEpi + 3) * 32;
 // A sum that runs through the tensor core loses up to its last place with each
 // instruction, always downwards.  For f32 outputs it is therefore added in f32 after
-// this many K tiles (1024 columns).
-constexpr int kMmFold = 8;
+// this many K tiles (1024 columns).  16-bit outputs round far above that; 32768 columns
+// lose at most 1024 last places, 2^-14, an eighth of f16's rounding.
+constexpr int kMmFold = 8, kMmFold16 = 256;
 constexpr int kMmBox = 16;   // tokens of an output box
 constexpr int kMmShare = 8;  // most CTAs that share a tile's K
 
@@ -967,7 +968,7 @@ wh_status wh_fp8_gemm(wh_ctx* c, const uint8_t* weight, const uint8_t* scale, in
     WH_CUDA(launch_pdl(fp8_quant_kernel<__half>, grid, kQuantThreads, 0, s, c->pdl(), qa));
   const bool boxes = aligned(y, 16) && ldy * y_size % 16 == 0;
   const Fp8GemmArgs a{scale, c->sf_rows, xsf, y, ldy, rows, tokens, ktiles, y_dtype,
-                      y_dtype == WH_DTYPE_F32 ? kMmFold : 1 << 20, (rows + 127) / 128,
+                      y_dtype == WH_DTYPE_F32 ? kMmFold : kMmFold16, (rows + 127) / 128,
                       (tokens + h.n - 1) / h.n, boxes, x, ldx, cols, act_quant_block / 8, c->status};
   if ((long long)a.mtiles * a.ntiles > 0x7fffffffLL / 8)
     return fail(WH_ERR_UNSUPPORTED, "FP8 GEMM: rows * tokens too large");
