@@ -203,6 +203,29 @@ def test_scale_bytes_over_the_whole_range(ctx, W, lo, hi, tokens):
     assert (err <= size * 2.0**-22 * 18 + 2.0**-149 * 20).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("block", [32, 64, 128])
+@pytest.mark.parametrize("tokens", [1, 2, 50])
+def test_codes_are_the_act_quants_at_ties_and_beside_them(ctx, W, dtype, block, tokens):
+    # a weight of ones on its diagonal gives the quantised tokens back, exactly
+    grid = e4m3(np.arange(127, dtype=np.uint8))
+    near = np.concatenate([grid, (grid[1:] + grid[:-1]) / 2]).astype(np.float32)
+    bits = near[near > 0].view(np.int32)
+    near = np.concatenate([(bits + d).astype(np.int32).view(np.float32) for d in range(-3, 4)] + [np.zeros(9, np.float32)])
+    rng = np.random.default_rng(block + tokens)
+    n = 1040
+    x = rng.choice(near, (tokens, n)) * rng.choice([-1, 1], (tokens, n)).astype(np.float32)
+    x[:, ::block] = 448 * rng.choice([-1, 1], x[:, ::block].shape)  # the block's scale is the token's
+    x *= 2.0 ** rng.integers(-6, 7, (tokens, 1)).astype(np.float32)
+    x = torch.from_numpy(x).cuda().to(dtype)
+    w = torch.zeros(n, n, dtype=torch.uint8, device="cuda")
+    w.fill_diagonal_(0x38)
+    s = torch.full((9, 9), 127, dtype=torch.uint8, device="cuda")
+    y = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x, block, F32)
+    ctx.sync()
+    assert (y.double().cpu().numpy() == quantised(x, block)).all()
+
+
 def test_tiny_huge_and_zero_tokens(ctx, W):
     rng = np.random.default_rng(2)
     w, s, real = weight(rng, 130, 272)
@@ -215,7 +238,7 @@ def test_tiny_huge_and_zero_tokens(ctx, W):
     y = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x)
     ctx.sync()
     check(y, real, quantised(x, 64), F32)
-    assert (y[0] == 0).all()
+    assert (y[0] == 0).all() and not y[0].signbit().any()
 
 
 @pytest.mark.parametrize("tokens", [8, 200])

@@ -61,8 +61,23 @@ struct Fp8QuantArgs {
 };
 constexpr int kQuantThreads = 256;
 
-// 8 values of a block that `lanes` lanes share -> codes; byte: the block's scale.  Every
-// lane of the warp calls it.
+// v * inv (a power of two) as one rounded to the nearest E4M3, ties to even, has to be for the
+// act quant's ties to the lower: the f32 below it, so that a tie is none any more.  For
+// that to reach no tie itself, an f32's last bit goes into the one above it first (16-bit
+// types have none).  A zero becomes -0.
+template <bool kF32>
+__device__ __forceinline__ float fp8_below(float v, float inv) {
+  if (kF32) {
+    const uint32_t u = __float_as_uint(v);
+    v = __uint_as_float((u & ~1u) | (u << 1 & 2u));
+  }
+  return __fmaf_rd(v, inv, -7.888609052210118e-31f);  // 2^-100
+}
+
+// 8 values of a block that `lanes` lanes share -> codes (NaN of a NaN); byte: the block's
+// scale.  Every lane of the warp calls it.  Bound by its instructions before it was by bytes:
+// with the rounding of a value by cases (grouped.cu) 50 of them a value.
+template <bool kF32>
 __device__ __forceinline__ uint2 fp8_quant8(const float (&v)[8], int lanes, uint32_t& byte) {
   float m = 0.0f;
 #pragma unroll
@@ -71,10 +86,9 @@ __device__ __forceinline__ uint2 fp8_quant8(const float (&v)[8], int lanes, uint
   const AqScale s = aq_block_scale(m, c_aq.thr);
   byte = __float_as_uint(s.scale) >> 23;  // an infinite block's is 255, the product's NaN
   uint2 w;
-  w.x = e4m3x2_ref(__fmul_rn(v[0], s.inv), __fmul_rn(v[1], s.inv)) |
-        e4m3x2_ref(__fmul_rn(v[2], s.inv), __fmul_rn(v[3], s.inv)) << 16;
-  w.y = e4m3x2_ref(__fmul_rn(v[4], s.inv), __fmul_rn(v[5], s.inv)) |
-        e4m3x2_ref(__fmul_rn(v[6], s.inv), __fmul_rn(v[7], s.inv)) << 16;
+  auto two = [&](int j) { return e4m3x2_rn(fp8_below<kF32>(v[j], s.inv), fp8_below<kF32>(v[j + 1], s.inv)); };
+  w.x = two(0) | two(2) << 16;
+  w.y = two(4) | two(6) << 16;
   return w;
 }
 
@@ -88,7 +102,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(Fp8QuantArgs a
   float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (on) kv_load8(static_cast<const T*>(a.x) + t * a.ldx + col, v);
   uint32_t byte;
-  const uint2 w = fp8_quant8(v, a.lanes, byte);
+  const uint2 w = fp8_quant8<std::is_same<T, float>::value>(v, a.lanes, byte);
   if (on) *reinterpret_cast<uint2*>(a.xq + (long long)t * a.cols + col) = w;
   if (in && (part & 3) == 0) {  // groups past the row's end get 2^0
     const int nt = t / a.tile, r = t - nt * a.tile;
@@ -474,7 +488,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             for (int j = 0; j < 8; ++j) v[j] = 0.0f;
           }
           uint32_t byte;
-          const uint2 w = fp8_quant8(v, a.lanes, byte);
+          const uint2 w = fp8_quant8<std::is_same<X, float>::value>(v, a.lanes, byte);
           *reinterpret_cast<uint2*>(ring + s * L::kStage + kMmWeight + t * 128 + ((part >> 1 ^ (t & 7)) << 4) +
                                     (part & 1) * 8) = w;
           if ((part & 3) == 0) sfs[s * L::kSf + t * 16 + (part >> 2)] = on ? uint8_t(byte) : 127;
