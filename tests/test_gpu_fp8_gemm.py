@@ -226,6 +226,28 @@ def test_codes_are_the_act_quants_at_ties_and_beside_them(ctx, W, dtype, block, 
     assert (y.double().cpu().numpy() == quantised(x, block)).all()
 
 
+@pytest.mark.parametrize("tokens", [2, 2000])
+def test_scales_around_their_thresholds(ctx, W, tokens):
+    # the largest value of each block lies a few last places from where its scale doubles
+    rng = np.random.default_rng(tokens)
+    n = 1024
+    x = rng.standard_normal((tokens, n // 64, 64)).astype(np.float32)
+    e = rng.integers(-22, 119, (tokens, n // 64))
+    step = np.concatenate([np.arange(-4, 40), 2 ** np.arange(5, 24), -(2 ** np.arange(2, 23))])
+    top = (np.float32(448) * 2.0 ** e.astype(np.float32)).astype(np.float32).view(np.int32) + rng.choice(step, e.shape)
+    top = np.maximum(top.astype(np.int32).view(np.float32), np.float32(1e-5))
+    x *= top[..., None] / 8
+    x[:, :, 5] = top
+    x = torch.from_numpy(x.reshape(tokens, n)).cuda()
+    x = torch.where(x.abs() > torch.from_numpy(top).cuda().repeat_interleave(64, 1), 0.0, x)
+    w = torch.zeros(n, n, dtype=torch.uint8, device="cuda")
+    w.fill_diagonal_(0x38)
+    s = torch.full((8, 8), 127, dtype=torch.uint8, device="cuda")
+    y = W.gemm_fp8_e4m3_ue8m0(ctx, w, s, x)
+    ctx.sync()
+    assert (y.double().cpu().numpy() == quantised(x, 64)).all()
+
+
 def test_tiny_huge_and_zero_tokens(ctx, W):
     rng = np.random.default_rng(2)
     w, s, real = weight(rng, 130, 272)

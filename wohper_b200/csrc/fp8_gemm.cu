@@ -52,10 +52,8 @@ struct Fp8GemmArgs {
 struct Fp8QuantArgs {
   const void* x;
   long long ldx;
-  int cols, ktiles;
-  int lanes;   // 4, 8 or 16 a block
-  int chunks;  // CTAs of a token
-  int tile;    // tokens of the product's tile
+  int tokens, cols, ktiles;
+  int tile, shift;  // tokens of the product's tile; their logarithm, of 224 none
   uint8_t* xq;   // [tokens][cols]
   uint8_t* xsf;
 };
@@ -75,41 +73,54 @@ __device__ __forceinline__ float fp8_below(float v, float inv) {
 }
 
 // 8 values of a block that `lanes` lanes share -> codes (NaN of a NaN); byte: the block's
-// scale.  Every lane of the warp calls it.  Bound by its instructions before it was by bytes:
-// with the rounding of a value by cases (grouped.cu) 50 of them a value.
+// scale.  Every lane of the warp calls it.  Instructions count: with the rounding by cases
+// (grouped.cu) and a division a block 50 a value, and 8192 x 8192 f32 took 118 us.
+// An amax's scale byte k + 127, and 2^-k (aq_block_scale)
+__device__ __forceinline__ float fp8_block_scale(float amax, uint32_t& byte) {
+  const uint32_t u = __float_as_uint(fmaxf(amax, 1.0e-4f)), e = u >> 23;
+  byte = e == 255 ? 255 : e - 8 + (u > c_aq_top[e]);  // an infinite block's is 255, the product's NaN
+  return e == 255 ? 0.0f : __uint_as_float((254 - byte) << 23);
+}
 template <bool kF32>
 __device__ __forceinline__ uint2 fp8_quant8(const float (&v)[8], int lanes, uint32_t& byte) {
   float m = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));  // passes over NaN
   for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const AqScale s = aq_block_scale(m, c_aq.thr);
-  byte = __float_as_uint(s.scale) >> 23;  // an infinite block's is 255, the product's NaN
+  const float inv = fp8_block_scale(m, byte);
   uint2 w;
-  auto two = [&](int j) { return e4m3x2_rn(fp8_below<kF32>(v[j], s.inv), fp8_below<kF32>(v[j + 1], s.inv)); };
+  auto two = [&](int j) { return e4m3x2_rn(fp8_below<kF32>(v[j], inv), fp8_below<kF32>(v[j + 1], inv)); };
   w.x = two(0) | two(2) << 16;
   w.y = two(4) | two(6) << 16;
   return w;
 }
 
-template <class T>
+// kLanes: 4, 8 or 16 a block
+template <class T, int kLanes>
 __global__ void __launch_bounds__(kQuantThreads) fp8_quant_kernel(Fp8QuantArgs a) {
   pdl_wait_prior();
   pdl_launch_dependents();  // what came before is complete: the product may start on its weights
-  const int t = blockIdx.x / a.chunks;
-  const int part = (blockIdx.x - t * a.chunks) * kQuantThreads + threadIdx.x, col = part * 8;
+  const int part = blockIdx.x * kQuantThreads + threadIdx.x, col = part * 8;
   const bool in = part < a.ktiles * 16, on = col < a.cols;  // cols is a multiple of 16
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (on) kv_load8(static_cast<const T*>(a.x) + t * a.ldx + col, v);
-  uint32_t byte;
-  const uint2 w = fp8_quant8<std::is_same<T, float>::value>(v, a.lanes, byte);
-  if (on) *reinterpret_cast<uint2*>(a.xq + (long long)t * a.cols + col) = w;
-  if (in && (part & 3) == 0) {  // groups past the row's end get 2^0
-    const int nt = t / a.tile, r = t - nt * a.tile;
-    uint8_t* at = a.xsf + ((long long)nt * a.ktiles + (part >> 4)) * (a.tile > 128 ? 1024 : 512) + (r >> 7) * 512 +
-                  (r & 31) * 16 + (r >> 5 & 3) * 4;
-    at[(part >> 2) & 3] = on ? uint8_t(byte) : 127;
+  for (uint32_t t = blockIdx.y; t < (uint32_t)a.tokens; t += gridDim.y) {
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (on) kv_load8(static_cast<const T*>(a.x) + t * a.ldx + col, v);
+    uint32_t byte;
+    const uint2 w = fp8_quant8<std::is_same<T, float>::value>(v, kLanes, byte);
+    if (on) *reinterpret_cast<uint2*>(a.xq + (long long)t * a.cols + col) = w;
+    if (in && (part & 3) == 0) {  // groups past the row's end get 2^0
+      const uint32_t nt = a.shift ? t >> a.shift : t / 224, r = t - nt * a.tile;
+      uint8_t* at = a.xsf + ((long long)nt * a.ktiles + (part >> 4)) * (a.tile > 128 ? 1024 : 512) + (r >> 7) * 512 +
+                    (r & 31) * 16 + (r >> 5 & 3) * 4;
+      at[(part >> 2) & 3] = on ? uint8_t(byte) : 127;
+    }
   }
+}
+template <class T>
+static cudaError_t launch_fp8_quant(const Fp8QuantArgs& a, int lanes, dim3 grid, cudaStream_t s, bool pdl) {
+  return lanes == 4   ? launch_pdl(fp8_quant_kernel<T, 4>, grid, kQuantThreads, 0, s, pdl, a)
+         : lanes == 8 ? launch_pdl(fp8_quant_kernel<T, 8>, grid, kQuantThreads, 0, s, pdl, a)
+                      : launch_pdl(fp8_quant_kernel<T, 16>, grid, kQuantThreads, 0, s, pdl, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -968,22 +979,22 @@ wh_status wh_fp8_gemm(wh_ctx* c, const uint8_t* weight, const uint8_t* scale, in
   const cudaStream_t s = (cudaStream_t)stream;
   const int ktiles = (cols + 127) / 128;
   const int chunks = (ktiles * 16 + kQuantThreads - 1) / kQuantThreads;
-  const Fp8QuantArgs qa{x, ldx, cols, ktiles, act_quant_block / 8, chunks, h.n, xq, xsf};
-  const long long blocks = (long long)tokens * chunks;
-  if (blocks > 0x7fffffffLL) return fail(WH_ERR_UNSUPPORTED, "FP8 GEMM: tokens * cols too large");
-  const dim3 grid((unsigned)blocks);
+  const int shift = h.n == 16 ? 4 : h.n == 32 ? 5 : h.n == 64 ? 6 : h.n == 128 ? 7 : 0, lanes = act_quant_block / 8;
+  const Fp8QuantArgs qa{x, ldx, tokens, cols, ktiles, h.n, shift, xq, xsf};
+  if ((long long)tokens * chunks > 0x7fffffffLL) return fail(WH_ERR_UNSUPPORTED, "FP8 GEMM: tokens * cols too large");
+  const dim3 grid(chunks, std::min(tokens, 65535));
   if (h.quant)
     ;
   else if (dtype == WH_DTYPE_F32)
-    WH_CUDA(launch_pdl(fp8_quant_kernel<float>, grid, kQuantThreads, 0, s, c->pdl(), qa));
+    WH_CUDA(launch_fp8_quant<float>(qa, lanes, grid, s, c->pdl()));
   else if (dtype == WH_DTYPE_BF16)
-    WH_CUDA(launch_pdl(fp8_quant_kernel<__nv_bfloat16>, grid, kQuantThreads, 0, s, c->pdl(), qa));
+    WH_CUDA(launch_fp8_quant<__nv_bfloat16>(qa, lanes, grid, s, c->pdl()));
   else
-    WH_CUDA(launch_pdl(fp8_quant_kernel<__half>, grid, kQuantThreads, 0, s, c->pdl(), qa));
+    WH_CUDA(launch_fp8_quant<__half>(qa, lanes, grid, s, c->pdl()));
   const bool boxes = aligned(y, 16) && ldy * y_size % 16 == 0;
   const Fp8GemmArgs a{scale, c->sf_rows, xsf, y, ldy, rows, tokens, ktiles, y_dtype,
                       y_dtype == WH_DTYPE_F32 ? kMmFold : kMmFold16, (rows + 127) / 128,
-                      (tokens + h.n - 1) / h.n, boxes, x, ldx, cols, act_quant_block / 8, c->status};
+                      (tokens + h.n - 1) / h.n, boxes, x, ldx, cols, lanes, c->status};
   if ((long long)a.mtiles * a.ntiles > 0x7fffffffLL / 8)
     return fail(WH_ERR_UNSUPPORTED, "FP8 GEMM: rows * tokens too large");
   const bool pdl = c->pdl();

@@ -23,6 +23,8 @@
 //     non-finite; such rows are recomputed with the exact bit decoder.
 // Shapes the fast path does not cover (col_group != 128, cols % 16 != 0) run
 // fp8_gemv_generic_kernel, one thread per (row, input), same arithmetic.
+#include <array>
+#include <cstring>
 #include <map>
 #include <mutex>
 
@@ -38,6 +40,9 @@ __device__ __forceinline__ const float* fp8_x_rows(const Fp8GemvArgs& a, int row
 
 
 __constant__ ActQuantTable c_aq;
+// The same thresholds on amax itself, without the division by 448 = 1.75 * 2^8: an amax of
+// biased exponent E has k = E - 135 up to the float of bits c_aq_top[E], E - 134 above it.
+__constant__ uint32_t c_aq_top[256];
 
 cudaError_t ensure_smem_attr(const void* kernel, size_t bytes) {
   static std::mutex mu;
@@ -62,6 +67,25 @@ __device__ ActQuantTable g_aq;
 void set_act_quant_table(const ActQuantTable& t, cudaStream_t s) {
   cudaMemcpyToSymbolAsync(c_aq, &t, sizeof(t), 0, cudaMemcpyHostToDevice, s);
   cudaMemcpyToSymbolAsync(g_aq, &t, sizeof(t), 0, cudaMemcpyHostToDevice, s);
+  auto low = [&](uint32_t u) {  // ceil_log2f_thr(amax / 448) == E - 135
+    float amax;
+    std::memcpy(&amax, &u, 4);
+    const float q = amax / 448.0f;
+    uint32_t b;
+    std::memcpy(&b, &q, 4);
+    const uint32_t e = b >> 23, m = b & 0x7FFFFF;
+    return int(e) - 127 + (m != 0 && m >= t.thr[e]) <= int(u >> 23) - 135;
+  };
+  std::array<uint32_t, 256> top;
+  for (uint32_t e = 0; e < 256; ++e) {
+    uint32_t lo = e << 23, hi = lo | 0x7FFFFF;  // low(lo), not low(hi), for 1e-4 and above
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      (low(mid) ? lo : hi) = mid;
+    }
+    top[e] = lo;
+  }
+  cudaMemcpyToSymbol(c_aq_top, top.data(), sizeof(top));
 }
 const ActQuantTable* act_quant_table_device() {
   void* p = nullptr;
