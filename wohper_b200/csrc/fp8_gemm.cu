@@ -16,10 +16,10 @@
 // equal bytes in the tensor core's layout, copied from a table of 256 such rows.
 //
 // Measured, quantisation included (inputs of three calls in turn): 8192 tokens x 4096 x
-// 8192 in bf16 280 to 309 us (1780 to 1960 TFLOP/s), in f32 313 to 322; 509 in bf16 29 us; one
-// token x 4096 x 4096 8.1 us.  The quantisation of 8192 x 8192 f32 is 51 us of it, at the copy's rate.  Without
-// any product the loads of the large one alone take 226 us of 250: 10.6 TB/s from L2 to the
-// SMs, which 224 x 256 outputs for 31 KB of operands a CTA and K tile leave as its bound.
+// 8192 in bf16 235 us (2340 TFLOP/s), in f32 270; 2048 in bf16 72; 509 in bf16 25; one token x
+// 4096 x 4096 6.7.  The quantisation of 8192 x 8192 f32 is 57 us of it (51 at the copy's rate), its
+// product 200: the tensor pipe is active in 77 % of the cycles, at a clock that the power limit
+// holds at 1.55 GHz.
 #include <cuda_bf16.h>
 
 #include "kvcache.cuh"
@@ -902,7 +902,8 @@ struct MmHow {
 };
 // Tokens that the product quantises itself: a launch less, but each CTA quantises them anew
 // (4096 x 4096, us of device time, inside / by fp8_quant_kernel: 1 token 7.6 / 7.2, 2 7.3 / 7.1,
-// 4 8.4 / 7.4, 8 10.6 / 8.0; the launch and its scratch cost the host some 3 us).
+// 4 8.4 / 7.4, 8 10.6 / 8.0, with a slower rounding in both; the launch and its scratch cost the
+// host some 3 us).
 constexpr int kMmInside = 2;
 MmHow mm_how(const wh_ctx* c, int rows, int cols, int tokens) {
   MmHow h{};
