@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 
 #include "kvcache.cuh"
+#include "mm_steps.cuh"
 #include "tc.cuh"
 
 namespace wh {
@@ -151,7 +152,7 @@ struct Mm {
   static constexpr int kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
   static constexpr int kPer = kN / 2;                  // columns of an epilogue warp
   struct Misc {
-    uint64_t full[kStages], empty[kStages], acc_full[kAcc], acc_empty[kAcc], done;
+    uint64_t full[kStages], empty[2 * kStages], acc_full[kAcc], acc_empty[kAcc], done;
     uint32_t tmem;
   };
   static constexpr int kBytes = 1024 + kStages * (kStage + kSf) + (int)sizeof(Misc);
@@ -326,12 +327,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr bool kQuant = !std::is_same<X, void>::value;
   static_assert(!kQuant || kN == 16, "few tokens");
+  using Free = MmFree<kStages, kQuant ? 2 * kStages : kStages>;
   const int rank = (int)cluster_rank(), share = (int)cluster_size();
 
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&m.full[i], 2);
       mbar_init(&m.empty[i], 1);
+      mbar_init(&m.empty[kStages + i], 1);
     }
     for (int i = 0; i < kAcc; ++i) {
       mbar_init(&m.acc_full[i], 1);
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     for (int kt = k0; kt < k1; ++kt, ++g, at.next()) {
       const int s = at.s;
       const uint32_t byte = sc.at(kt);
-      if (g >= kStages) ok = mbar_wait_warp(&m.empty[s], at.phase ^ 1, a.status);
+      if (g >= kStages) ok = mbar_wait_warp(&m.empty[Free::bar(g - kStages)], Free::parity(g - kStages), a.status);
       if (!ok) break;
       if (tc::elect_one()) {
         mbar_arrive_expect_tx(&m.full[s], kMmWeight + 512);
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     const uint8_t* sf = a.xsf + (long long)(tile / a.mtiles) * a.ktiles * 512;
     for (int kt = k0; kt < k1; ++kt, ++g, at.next()) {
       const int s = at.s;
-      if (g >= kStages) ok = mbar_wait_warp(&m.empty[s], at.phase ^ 1, a.status);
+      if (g >= kStages) ok = mbar_wait_warp(&m.empty[Free::bar(g - kStages)], Free::parity(g - kStages), a.status);
       if (!ok) break;
       if (tc::elect_one()) {
         mbar_arrive_expect_tx(&m.full[s], L::kTokens + L::kSfb);
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
           for (int k = 0; k < 4; ++k)
             tc::mma_mxf8(acc, dw + 2 * k, dx + 2 * k, tc::idesc_mxf8(kN, k, k), wsf | (uint32_t(k) << 30),
                          xsf | (uint32_t(k) << 30), kt != c0 || k != 0);
-          tc::commit(&m.empty[s]);
+          tc::commit(&m.empty[Free::bar(kt - k0)]);
         }
         __syncwarp();
       }
@@ -480,13 +483,10 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         // The product goes on to sum `chunk` + 2 only after sum `chunk` has been taken, for
         // which it has (or gets from the other warps) all of the codes.
         while (ok && kt - c0 >= kAcc * a.fold) take();
-        // The stage's fills in turn: this warp's own last one, two before, then the one between.
-        // (A phase is told from the next but one only by one who has seen it end.)
-        static_assert(kMmEpi == 2 * L::kStages || !kQuant, "two fills between a warp's own");
-        if (ok && g >= 2 * kStages)
-          ok = mbar_wait_warp(&m.empty[s], (g / kStages) & 1, a.status);
+        // two warps fill a stage in turn (MmFree)
+        static_assert(kMmEpi == 2 * L::kStages || !kQuant, "every second tile of a stage is this warp's");
         if (ok && g >= kStages)
-          ok = mbar_wait_warp(&m.empty[s], ((g / kStages) - 1) & 1, a.status);
+          ok = mbar_wait_warp(&m.empty[Free::bar(g - kStages)], Free::parity(g - kStages), a.status);
         if (!ok) break;
         for (int p = 0; 2 * p < a.tokens; ++p) {
           const int t = 2 * p + (lane >> 4);
