@@ -237,6 +237,18 @@ __device__ __forceinline__ void mm_store_boxes(const Fp8GemmArgs& a, const CUten
   }
 }
 
+// Whether all four warps of a column half say so (named barrier `bar`)
+__device__ __forceinline__ bool mm_all_of_half(int bar, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n bar.red.and.pred q, %1, 128, p;\n"
+      " selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(all)
+      : "r"(bar), "r"((uint32_t)ok)
+      : "memory");
+  return all != 0;
+}
+
 // A place in a ring of kCount stages
 template <int kCount>
 struct MmRing {
@@ -778,28 +790,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmThreads, 1)
     bool ok = true;
     for (int tile = tile0; ok && tile < tiles; tile += step) {
       float acc[kPer];
-      for (int c0 = 0; c0 < a.ktiles; c0 += a.fold, ++chunk) {
+      auto sum = [&](bool first) {
         const int b = chunk % kAcc;
-        ok = __all_sync(0xffffffffu, mbar_wait(&m.acc_full[b], (chunk / kAcc) & 1, a.status));
-        if (!ok) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(&m.acc_full[b], (chunk / kAcc) & 1, a.status))) return false;
         tc::fence_after_sync();
-        mm_sum<kPer>(at + b * kN, acc, c0 == 0);
+        mm_sum<kPer>(at + b * kN, acc, first);
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(map_to_rank(&m.acc_empty[b], 0));
-      }
-      if (!ok) break;
-      const int row = (tile % mpairs * 2 + rank) * 128 + quad * 32 + lane;
-      const int n0 = tile / mpairs * kN + half * kPer;
-      if (!a.boxes) {
-        mm_store<kPer>(a, row, n0, acc);
-      } else if (a.dtype == WH_DTYPE_F32) {
-        mm_store_boxes<float, kPer>(a, &ymap, outs + half * (L::kOut / 2), turn, row, n0, acc);
-      } else if (a.dtype == WH_DTYPE_BF16) {
-        mm_store_boxes<__nv_bfloat16, kPer>(a, &ymap, outs + half * (L::kOut / 2), turn, row, n0, acc);
-      } else {
-        mm_store_boxes<__half, kPer>(a, &ymap, outs + half * (L::kOut / 2), turn, row, n0, acc);
-      }
+        ++chunk;
+        return true;
+      };
+      auto agree = [&](bool fine) { return mm_all_of_half(1 + half, fine); };
+      auto store = [&] {
+        const int row = (tile % mpairs * 2 + rank) * 128 + quad * 32 + lane;
+        const int n0 = tile / mpairs * kN + half * kPer;
+        if (!a.boxes) {
+          mm_store<kPer>(a, row, n0, acc);
+        } else if (a.dtype == WH_DTYPE_F32) {
+          mm_store_boxes<float, kPer>(a, &ymap, outs + half * (L::kOut / 2), turn, row, n0, acc);
+        } else if (a.dtype == WH_DTYPE_BF16) {
+          mm_store_boxes<__nv_bfloat16, kPer>(a, &ymap, outs + half * (L::kOut / 2), turn, row, n0, acc);
+        } else {
+          mm_store_boxes<__half, kPer>(a, &ymap, outs + half * (L::kOut / 2), turn, row, n0, acc);
+        }
+      };
+      ok = mm_tile(a.ktiles, a.fold, sum, agree, store);
     }
     bulk_stores_done();
   }

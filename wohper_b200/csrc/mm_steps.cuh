@@ -1,6 +1,7 @@
-// mm_steps.cuh -- which barrier and phase the warps of the FP8 product (fp8_gemm.cu)
-// wait for before they fill a stage of its ring.  Plain arithmetic: a CPU test
-// compiles it too and runs through every order in which the warps can come.
+// mm_steps.cuh -- by which steps the warps of the FP8 product (fp8_gemm.cu) wait for one
+// another: the barrier and phase before a stage of its ring is filled, and what an
+// epilogue's warps do together.  Plain C++: CPU tests compile it too, and run through
+// every order in which the warps can come and through waits that run out.
 #pragma once
 #include <stdint.h>
 
@@ -28,5 +29,18 @@ struct MmFree {
   static WH_STEP int bar(int f) { return f % kBars; }
   static WH_STEP uint32_t parity(int f) { return uint32_t(f / kBars) & 1u; }
 };
+
+// One tile of an epilogue warp: `sum` takes each of its sums from the tensor core (false:
+// the wait ran out), `store` writes the tile together with the other warps of its column half.
+// Those wait for one another without a limit, so the warps `agree` first: all of them store
+// the tile or, where one has given up, none.
+template <class Sum, class Agree, class Store>
+WH_STEP bool mm_tile(int ktiles, int fold, Sum sum, Agree agree, Store store) {
+  bool ok = true;
+  for (int c0 = 0; ok && c0 < ktiles; c0 += fold) ok = sum(c0 == 0);
+  ok = agree(ok);
+  if (ok) store();
+  return ok;
+}
 
 }  // namespace wh
