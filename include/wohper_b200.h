@@ -149,7 +149,7 @@ size_t wh_fp8_gemm_scratch_bytes(int cols, int tokens);
  * (WH_DTYPE_*), ldx elements apart, each on a 16-byte boundary; aq is
  * wh_act_quant_fp8 over blocks of act_quant_block (32, 64 or 128) values of a
  * row.  y [tokens] rows of rows values of y_dtype, ldy elements apart; may not
- * overlap an input.
+ * overlap an input.  rows, cols and tokens are at most 2^30.
  *   Operands are those of the GEMV bit for bit, but for what the tensor core
  * reads otherwise: weight bytes 0x7F / 0xFF are NaN (the GEMV: +-480), a scale
  * byte 0 is 2^-127 (the GEMV: 0).  A not-finite value of x makes its token's

@@ -137,6 +137,7 @@ constexpr int kMmThreads = (kMmEpi + 3) * 32;
 // lose at most 1024 last places, 2^-14, an eighth of f16's rounding.
 constexpr int kMmFold = 8, kMmFold16 = 256;
 constexpr int kMmBox = 16;   // tokens of an output box
+constexpr int kMmMost = 1 << 30;  // rows, columns, tokens: rounded up to tiles they fit an int
 constexpr int kMmShare = 8;  // most CTAs that share a tile's K
 
 template <int kN>
@@ -944,8 +945,8 @@ MmHow mm_how(const wh_ctx* c, int rows, int cols, int tokens) {
 // has 1024 bytes a K tile, smaller ones have 512 and a call has at most one of them that
 // is smaller than 128.
 size_t mm_sf_bytes(int cols, int tokens) {
-  const size_t wide = (size_t)((tokens + 223) / 224) * 1024, narrow = (size_t)((tokens + 127) / 128) * 512;
-  return std::max(wide, narrow) * ((cols + 127) / 128);
+  const size_t wide = ((size_t)tokens + 223) / 224 * 1024, narrow = ((size_t)tokens + 127) / 128 * 512;
+  return std::max(wide, narrow) * (((size_t)cols + 127) / 128);
 }
 
 }  // namespace
@@ -966,6 +967,8 @@ wh_status wh_fp8_gemm(wh_ctx* c, const uint8_t* weight, const uint8_t* scale, in
   if (!kv_dtype_size(dtype, &size) || !kv_dtype_size(y_dtype, &y_size))
     return fail(WH_ERR_UNSUPPORTED, "FP8 GEMM: dtype");
   if (rows < 1 || cols < 1) return fail(WH_ERR_EMPTY_SHAPE, "FP8 GEMM: rows, cols");
+  if (rows > kMmMost || cols > kMmMost || tokens > kMmMost)
+    return fail(WH_ERR_UNSUPPORTED, "FP8 GEMM: rows, cols or tokens > 2^30");
   if (scale_rows != (rows + 127) / 128 || scale_cols != (cols + 127) / 128)
     return fail(WH_ERR_INVALID_SHAPE, "FP8 GEMM: a scale for each block of 128 x 128");
   if (cols % 16 != 0) return fail(WH_ERR_UNSUPPORTED, "FP8 GEMM: cols % 16 != 0");

@@ -6,7 +6,7 @@ import torch
 
 from . import Context, _check, _ptr, lib
 from .kvcache import (_INVALID_POINTER, _INVALID_SHAPE, _UNSUPPORTED, _dense, _dtype_code, _fail,
-                      _handle, _on, _on_gpu)
+                      _handle, _int, _on, _on_gpu)
 
 
 def _rows(x, rows: int, cols: int, what: str) -> int:
@@ -46,11 +46,13 @@ def gemm_fp8_e4m3_ue8m0(ctx: Context, weight, scale, x, act_quant_block: int = 6
     Returns out [tokens, rows] of out_dtype (by default x's), f32 sums: those of the
     GEMV in another order.  out may not overlap an input; its rows may lie apart."""
     dev = weight.device
-    _on_gpu(ctx, dev, "weight")
     if weight.dim() != 2 or scale.dim() != 2 or x.dim() != 2:
         _fail(_INVALID_SHAPE, "weight [rows, cols], scale, x [tokens, cols]")
     rows, cols = weight.shape
     tokens = x.shape[0]
+    _int(max(rows, cols), "weight")
+    _int(tokens, "x")
+    _on_gpu(ctx, dev, "weight")
     _dense(weight, torch.uint8, rows * cols, dev, "weight")
     srows, scols = scale.shape
     if srows != (rows + 127) // 128 or scols != (cols + 127) // 128:

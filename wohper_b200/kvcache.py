@@ -46,6 +46,11 @@ def _fail(status: int, why: str):
     raise WohperError(status, why)
 
 
+def _int(n: int, what: str) -> None:
+    if n > _INT_MAX:
+        _fail(_INVALID_SHAPE, f"{what}: {n} is past 32 bits")
+
+
 def _dtype_code(dtype) -> int:
     code = _DTYPES.get(dtype)
     if code is None:
@@ -190,6 +195,8 @@ def kv_plan(ctx: Context, page: int, kv_lens, q_lens, block_table, free_blocks, 
     larger fixed one (a captured graph).  A step that does not fit changes
     nothing, gives no tokens, and ctx.sync() raises DeviceArg."""
     n, dev = kv_lens.numel(), kv_lens.device
+    _int(n, "kv_lens")
+    _int(free_blocks.numel(), "free_blocks")
     _on_gpu(ctx, dev, "kv_lens")
     i32 = torch.int32
     _dense(kv_lens, i32, n, dev, "kv_lens")
@@ -197,6 +204,7 @@ def kv_plan(ctx: Context, page: int, kv_lens, q_lens, block_table, free_blocks, 
     if block_table.dim() != 2 or block_table.shape[0] != n:
         _fail(_INVALID_SHAPE, "block_table: [requests, max_blocks]")
     _dense(block_table, i32, block_table.numel(), dev, "block_table")
+    _int(block_table.shape[1], "block_table")
     capacity = free_blocks.numel()
     _dense(free_blocks, i32, capacity, dev, "free_blocks")
     _dense(free_top, i32, 1, dev, "free_top")
@@ -311,13 +319,14 @@ def kv_attention(ctx: Context, cache: PagedKvCache, q, cu_q, kv_lens, block_tabl
 def _attend(ctx, cache, q, cu_q, kv_lens, block_table, scale, window, first, sink, out, scratch,
             stream, masks=None, positions=None):
     """kv_attention; with masks [tokens, words] and positions [tokens] kv_tree_attention."""
-    dev = cache.keys.device
+    dev, n = cache.keys.device, kv_lens.numel()
+    _int(n, "kv_lens")
     _on_gpu(ctx, dev, "cache")
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         _fail(_INVALID_SHAPE, "q: [tokens, heads, head_dim]")
     code = _dtype_code(q.dtype)
     tokens, heads, d = q.shape
-    n = kv_lens.numel()
+    _int(tokens, "q")
     if q.device != dev:
         _fail(_INVALID_POINTER, f"q: on {q.device}, not {dev}")
     _dense(kv_lens, torch.int32, n, dev, "kv_lens")
@@ -326,6 +335,7 @@ def _attend(ctx, cache, q, cu_q, kv_lens, block_table, scale, window, first, sin
     if block_table.dim() != 2 or block_table.shape[0] != n:
         _fail(_INVALID_SHAPE, "block_table: [requests, max_blocks]")
     _dense(block_table, torch.int32, block_table.numel(), dev, "block_table")
+    _int(block_table.shape[1], "block_table")
     if sink is not None:
         _dense(sink, torch.float32, heads, dev, "sink")
     if masks is not None:

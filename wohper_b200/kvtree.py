@@ -26,7 +26,7 @@ import torch
 
 from . import Context, _check, lib
 from .kvcache import (_INT_MAX, _INVALID_SHAPE, _UNSUPPORTED, PagedKvCache, _attend, _dense, _fail,
-                      _handle, _on, _on_gpu)
+                      _handle, _int, _on, _on_gpu)
 
 _I32 = torch.int32
 
@@ -54,6 +54,7 @@ class KvAccept:
 def _table(block_table, n: int, dev) -> int:
     if block_table.dim() != 2 or block_table.shape[0] != n:
         _fail(_INVALID_SHAPE, "block_table: [requests, max_blocks]")
+    _int(block_table.shape[1], "block_table")
     _dense(block_table, _I32, block_table.numel(), dev, "block_table")
     return block_table.shape[1]
 
@@ -64,6 +65,8 @@ def kv_tree(ctx: Context, parents, cu_q, kv_lens, max_nodes: int, stream=None) -
     -1; cu_q and kv_lens as kv_plan gives them; max_nodes (at most 256): the most
     nodes of a request.  Bad parents and larger requests: ctx.sync() raises DeviceArg."""
     n, tokens, dev = kv_lens.numel(), parents.numel(), kv_lens.device
+    _int(n, "kv_lens")
+    _int(tokens, "parents")
     _on_gpu(ctx, dev, "kv_lens")
     _dense(kv_lens, _I32, n, dev, "kv_lens")
     _dense(cu_q, _I32, n + 1, dev, "cu_q")
@@ -102,6 +105,9 @@ def kv_accept(ctx: Context, page: int, parents, drafts, targets, cu_q, kv_lens, 
     which is updated in place; a stack that does not fit them changes nothing, keeps
     nothing, and ctx.sync() raises DeviceArg."""
     n, tokens, dev = kv_lens.numel(), parents.numel(), kv_lens.device
+    _int(n, "kv_lens")
+    _int(tokens, "parents")
+    _int(free_blocks.numel(), "free_blocks")
     _on_gpu(ctx, dev, "kv_lens")
     _dense(kv_lens, _I32, n, dev, "kv_lens")
     _dense(cu_q, _I32, n + 1, dev, "cu_q")
@@ -132,6 +138,8 @@ def kv_commit(ctx: Context, cache: PagedKvCache, counts, path, cu_q, kv_lens, bl
     is the step's, before kv_accept.  A pool [blocks, layers, kv_heads, page, ..]
     may be given as one cache of layers * kv_heads heads."""
     n, dev = kv_lens.numel(), cache.keys.device
+    _int(n, "kv_lens")
+    _int(path.numel(), "path")
     _on_gpu(ctx, dev, "cache")
     _dense(kv_lens, _I32, n, dev, "kv_lens")
     _dense(counts, _I32, n, dev, "counts")
