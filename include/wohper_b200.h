@@ -154,8 +154,9 @@ size_t wh_fp8_gemm_scratch_bytes(int cols, int tokens);
  * reads otherwise: weight bytes 0x7F / 0xFF are NaN (the GEMV: +-480), a scale
  * byte 0 is 2^-127 (the GEMV: 0).  A not-finite value of x makes its token's
  * outputs NaN and no other's.  Sums are f32 in the tensor core's order: for an
- * f32 y over 1024 columns at a time (32768 for a 16-bit y), which are then added
- * in f32.  Results repeat bit for bit.
+ * f32 y over 1024 columns at a time (8192 for a 16-bit y), which are then added
+ * in f32.  The tensor core cuts its sums off downwards: with terms of one sign 1024
+ * columns lose 2e-6 of their sum, 8192 2e-5.  Results repeat bit for bit.
  *   All pointers are of the context's device, which has to be the current one
  * (WH_ERR_CUDA otherwise). */
 wh_status wh_fp8_gemm(wh_ctx* ctx, const uint8_t* weight, const uint8_t* scale, int rows, int cols,

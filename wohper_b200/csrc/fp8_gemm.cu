@@ -131,11 +131,14 @@ constexpr int kMmWeight = 128 * 128;  // a weight tile: 128 rows x 128 K
 constexpr int kMmEpi = 8;             // epilogue warps: TMEM quadrant w % 4, column half w / 4
 constexpr int kMmMma = kMmEpi, kMmWeights = kMmEpi + 1, kMmTokens = kMmEpi + 2;
 constexpr int kMmThreads = (kMmEpi + 3) * 32;
-// A sum that runs through the tensor core loses up to its last place with each
-// instruction, always downwards.  For f32 outputs it is therefore added in f32 after
-// this many K tiles (1024 columns).  16-bit outputs round far above that; 32768 columns
-// lose at most 1024 last places, 2^-14, an eighth of f16's rounding.
-constexpr int kMmFold = 8, kMmFold16 = 256;
+// A sum that runs through the tensor core is cut off with each instruction of 32 columns, always
+// downwards.  Measured with terms of one sign, relative to the sum (of mixed signs: to its
+// largest partial sum, so cancellation enlarges it relative to the result): 1024 columns lose
+// 1.9e-6 on average and 3.6e-6 at most, 8192 lose 1.4e-5 to 1.9e-5, 32768 7.8e-5, 393216 1.1e-3.
+// f32 outputs are therefore added in f32 after kMmFold K tiles (1024 columns), 16-bit ones
+// after kMmFold16 (8192 columns): a twenty-fifth of f16's rounding, 2^-11.  32768 columns would be
+// a sixth, and were no faster (509 tokens x 4096 x 32768 bf16 76.8 us, by 8192 columns 76.7).
+constexpr int kMmFold = 8, kMmFold16 = 64;
 constexpr int kMmBox = 16;   // tokens of an output box
 constexpr int kMmMost = 1 << 30;  // rows, columns, tokens: rounded up to tiles they fit an int
 constexpr int kMmShare = 8;  // most CTAs that share a tile's K
