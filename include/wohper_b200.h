@@ -668,10 +668,11 @@ size_t wh_kv_attention_scratch_bytes(const wh_ctx* ctx, const wh_kv_cache* cache
  *   Sums, maxima and normalisers are f32.  Heads 64, 128, 256 and 512 wide are
  * multiplied in f16 parts, which hold the cache's values exactly.  A 16-bit query
  * is one part (exact down to 2^-28 of its row's largest element) and its weights
- * have 11 bits.  An f32 query is two parts, 22 bits (fewer below 2^-16 of its
- * row's largest element), as are its weights (down to 2^-23 of its row's largest
- * weight); its outputs are as exact as those of f32 products.  Other widths are
- * computed in f32 throughout. */
+ * have 11 bits; its sums run on in the tensor core, which cuts them off downwards
+ * (values of one sign: by up to 2e-7 of the sum for each 64 rows).  An f32 query is
+ * two parts, 22 bits (fewer below 2^-16 of its row's largest element), as are its
+ * weights (down to 2^-23 of its row's largest weight); its outputs are as exact as
+ * those of f32 products.  Other widths are computed in f32 throughout. */
 wh_status wh_kv_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void* q, int dtype,
                           int tokens, int heads, long long q_token_stride,
                           long long q_head_stride, int requests, const int32_t* cu_q,
@@ -730,7 +731,8 @@ wh_status wh_kv_tree_attention(wh_ctx* ctx, const wh_kv_cache* cache, const void
  * a length below its nodes or past max_blocks * page (treated as one without
  * nodes); a stack height outside [0, capacity] or that would outgrow it (no request
  * keeps anything, no block moves, lengths as they were).
- *   kv_lens_out and free_top_out may not be their inputs. */
+ *   kv_lens_out and free_top_out may not be their inputs (refused); no other output
+ * may overlap an input either. */
 wh_status wh_kv_accept(wh_ctx* ctx, int requests, int page, int max_blocks, int tokens,
                        const int32_t* parents, const int32_t* drafts, const int32_t* targets,
                        const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,

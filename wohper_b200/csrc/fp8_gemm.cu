@@ -16,7 +16,8 @@
 // equal bytes in the tensor core's layout, copied from a table of 256 such rows.
 //
 // Measured, quantisation included (inputs of three calls in turn): 8192 tokens x 4096 x
-// 8192 in bf16 235 us (2340 TFLOP/s), in f32 270; 2048 in bf16 72; 509 in bf16 25; one token x
+// 8192 in bf16 233 us (2360 TFLOP/s), in f32 270 (315 after a second of such calls, at the clock
+// of 1.44 GHz that the power limit then leaves); 2048 in bf16 72; 509 in bf16 24.5; one token x
 // 4096 x 4096 6.7.  The quantisation of 8192 x 8192 f32 is 57 us of it (51 at the copy's rate), its
 // product 200: the tensor pipe is active in 77 % of the cycles, at a clock that the power limit
 // holds at 1.55 GHz.
@@ -73,15 +74,15 @@ __device__ __forceinline__ float fp8_below(float v, float inv) {
   return __fmaf_rd(v, inv, -7.888609052210118e-31f);  // 2^-100
 }
 
-// 8 values of a block that `lanes` lanes share -> codes (NaN of a NaN); byte: the block's
-// scale.  Every lane of the warp calls it.  Instructions count: with the rounding by cases
-// (grouped.cu) and a division a block 50 a value, and 8192 x 8192 f32 took 118 us.
 // An amax's scale byte k + 127, and 2^-k (aq_block_scale)
 __device__ __forceinline__ float fp8_block_scale(float amax, uint32_t& byte) {
   const uint32_t u = __float_as_uint(fmaxf(amax, 1.0e-4f)), e = u >> 23;
   byte = e == 255 ? 255 : e - 8 + (u > c_aq_top[e]);  // an infinite block's is 255, the product's NaN
   return e == 255 ? 0.0f : __uint_as_float((254 - byte) << 23);
 }
+// 8 values of a block that `lanes` lanes share -> codes (NaN of a NaN); byte: the block's
+// scale.  Every lane of the warp calls it.  Instructions count: with the rounding by cases
+// (grouped.cu) and a division a block 50 a value, and 8192 x 8192 f32 took 118 us.
 template <bool kF32>
 __device__ __forceinline__ uint2 fp8_quant8(const float (&v)[8], int lanes, uint32_t& byte) {
   float m = 0.0f;
@@ -216,8 +217,9 @@ __device__ __forceinline__ void bulk_stores_commit() { asm volatile("cp.async.bu
 __device__ __forceinline__ void bulk_stores_read() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-// The same by the four warps of a column half together: 16 tokens x 128 rows at a time
-// through shared memory (two buffers at outs, in turn), written by bulk stores.  Whole lines: a
+// Row `row` of tokens n0 .. as mm_store writes it, by the four warps of a column half together: 16
+// tokens x 128 rows at a time through shared memory (two buffers at outs, in turn), written by
+// bulk stores.  All four call it (mm_tile).  Whole lines: a
 // warp's own stores are 64 or 128 bytes at a token, which took 6.7 us a tile of 128 x 224
 // in bf16, more than its products over 1024 columns.
 template <class T, int kPer>
@@ -904,26 +906,27 @@ wh_status make_y_map(CUtensorMap* map, void* y, int size, uint64_t rows, uint64_
 }
 
 // How a call is cut: tokens of a tile; pairs of CTAs that walk tiles, or clusters of
-// `share` CTAs with a tile each.  Measured, us:
-//  - one token: 4096 x 4096 in 1 / 2 / 4 / 8 shares 13.4 / 9.6 / 7.7 / 7.3, 4096 x 8192 23.5 / 15.0
-//    / 11.2 / 9.4, 32768 x 1024 (256 tiles) in 1 / 2 shares 9.6 / 13.7: as many CTAs as two an SM
-//    hold.  Behind fp8_quant_kernel, whose CTAs are in their way, as many clusters of 8 at times
-//    take two turns (16 x 4096 x 4096 12.1, in 4 shares 9.3), so
-//  - more tokens get one CTA an SM: 17 x 4096 x 4096 in 4 / 8 shares 8.4 / 12.3, 128 x 4096 x 4096
-//    11.0 / 23.5 (clusters of 8 no longer all fit), 128 x 512 x 4096 (4 tiles) 9.9 / 9.7;
-//  - shares or pairs: 256 x 4096 x 4096 in 2 shares 14.4, pairs 16.6; 509 in 1 share 22.2, pairs 18.7;
-//    64 x 32768 x 1024 in 1 share 19.1, pairs 14;
-//  - pairs of 128 / 224 tokens a tile: 509 x 4096 x 8192 29.3 / 32.8, 1024 52 / 57, 2048 97 / 90: a tile
-//    of 224 costs four thirds of one of 128.
+// `share` CTAs with a tile each.  Measured (tokens x rows x cols, f32 up to 16 tokens, bf16 from
+// there on; device us, a CUDA graph of calls over three inputs):
+//  - one token: 4096 x 4096 in 1 / 2 / 4 / 8 shares 12.3 / 8.1 / 6.2 / 6.5, 4096 x 8192 22.2 / 13.4
+//    / 9.2 / 8.7, 32768 x 1024 (256 tiles) in 1 / 2 shares 8.6 / 12.5: as many CTAs as two an SM
+//    hold.  Behind fp8_quant_kernel, whose CTAs are in their way, as many clusters of 8
+//    take longer (16 x 4096 x 4096 8.1, in 4 shares 7.3), so
+//  - more tokens get one CTA an SM: 17 x 4096 x 4096 in 4 / 8 shares 7.4 / 8.3, 128 x 4096 x 4096
+//    9.7 / 22.2 (clusters of 8 no longer all fit), 128 x 512 x 4096 (4 tiles) 8.7 / 8.5;
+//  - shares or pairs: 256 x 4096 x 4096 in 2 shares 12.7, pairs 14.2; 509 in 1 share 19.0, pairs 15.2;
+//    64 x 32768 x 1024 in 1 share 18.4, pairs 13.5;
+//  - pairs of 128 / 224 tokens a tile: 509 x 4096 x 8192 23.7 / 28.0, 1024 40.3 / 46.9, 2048 75.3 / 71.8: a
+//    tile of 224 costs up to four thirds of one of 128.
 struct MmHow {
   int n, share;
   bool pair;
   bool quant;  // by the product itself
 };
-// Tokens that the product quantises itself: a launch less, but each CTA quantises them anew
-// (4096 x 4096, us of device time, inside / by fp8_quant_kernel: 1 token 7.6 / 7.2, 2 7.3 / 7.1,
-// 4 8.4 / 7.4, 8 10.6 / 8.0, with a slower rounding in both; the launch and its scratch cost the
-// host some 3 us).
+// Tokens that the product quantises itself: a launch less, but each CTA quantises them anew.
+// Inside / by fp8_quant_kernel, device us: 4096 x 4096 1 token 6.5 / 6.4, 2 6.6 / 6.3, 4 6.9 / 6.4, 8
+// 7.9 / 6.7; 4096 x 8192 1 token 8.7 / 10.4, 2 8.9 / 10.3; 512 x 4096 1 token 5.0 / 5.2, 32768 x 1024 8.6 / 9.0.
+// A call from Python, by the host: 12.3 / 16.8, for the launch and its scratch.
 constexpr int kMmInside = 2;
 MmHow mm_how(const wh_ctx* c, int rows, int cols, int tokens) {
   MmHow h{};

@@ -34,7 +34,8 @@
 // with the join, 32 x 4096 of f32 57 us.  M = 128 keys a product would
 // read 14 % fewer operand bytes but leave room for one tile only.
 // The forms whose values are the keys spill nothing; those with values of their own
-// 4-16 bytes, but for 16-bit queries of 256 columns.
+// 4-16 bytes, but for 16-bit queries of 64 to 256 columns, which spill nothing (of a
+// tree 64 and 128 columns: 4 bytes).
 #include "kvattn.cuh"
 #include "tc.cuh"
 
