@@ -205,7 +205,8 @@ __device__ __forceinline__ void mm_put(void* y, long long at, int dtype, float v
 __device__ __forceinline__ void mm_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void mm_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void mm_put(__half* p, float v) { *p = __float2half_rn(v); }
-// 2-D tiled store; the box may reach past the tensor's ends
+// 2-D tiled store; the box may reach past the tensor's ends.  What lies past the end of a row is
+// left out by 16 bytes: up to there zeros are written behind a row that ends in between.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int32_t c0, int32_t c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -811,7 +812,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmThreads, 1)
       auto store = [&] {
         const int row = (tile % mpairs * 2 + rank) * 128 + quad * 32 + lane;
         const int n0 = tile / mpairs * kN + half * kPer;
-        if (!a.boxes) {
+        // a last tile whose rows end between two 16 bytes of y would zero what lies behind them
+        const bool ends = (a.rows & (a.dtype == WH_DTYPE_F32 ? 3 : 7)) == 0 || (row | 127) < a.rows;
+        if (!a.boxes || !ends) {
           mm_store<kPer>(a, row, n0, acc);
         } else if (a.dtype == WH_DTYPE_F32) {
           mm_store_boxes<float, kPer>(a, &ymap, outs + half * (L::kOut / 2), turn, row, n0, acc);
